@@ -1,0 +1,644 @@
+// Attention of few query rows over many keys (decoding): fpk_attention_paged
+// and fpk_attention_packed where a sequence has at most a few dozen query rows
+// (tokens x query heads to a key head).
+//
+// Bound by the keys' and values' bytes, each read once from HBM, so everything
+// serves the stream of loads:
+// * Keys and values go from global memory straight into matrix fragments (mma
+//   m16n8k16, 16 query rows). A contraction does not care for the order of its
+//   index, so the order is chosen such that a thread's 16-byte record is its
+//   fragment: scores contract 8 channels of a record in two products; a
+//   score column c of 8-column block j stands for key 8j + 4(c%2) + c/2, so that
+//   a thread's four probabilities belong to keys t, 4+t, 8+t, 12+t (t = lane%4)
+//   and its four value records, one of each key and of plane lane/4, need only a
+//   byte permute to become fragments of the second product. No shared
+//   memory and no barrier in the loop; every load instruction covers whole
+//   sectors.
+// * e4m3 records become fp16 (exact) in registers. The key's scale multiplies
+//   its scores; the value's scale v joins the exponent: P' = 2^(s + log2 v - m),
+//   O = sum P' code, l = sum P'/v, so P' is at most 2^8 whatever the scales are
+//   (rows of one sequence may differ by up to 2^126). Queries become fp16 with a
+//   power of two taken out of each row, exact down to 2^-14 of its maximum.
+// * Softmax in one pass, statistics and sums in fp32. A row's reference m moves
+//   only when a score exceeds it by 2^8, a warp vote, so most steps need no
+//   shuffle.
+// * The key axis is split evenly: all (sequence, row tile, key head) units of 64
+//   keys form one line that the CTAs share out, each finding its part from the
+//   lengths on the device. A tile that crosses CTAs leaves fp32 partials that a
+//   second launch joins in order (deterministic, no atomics).
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include "fp_attention_seq.cuh"
+#include "fp_launch.hpp"
+#include "fp_profile.hpp"
+#include "fp_tc.cuh"
+
+namespace fpb {
+namespace seqattn {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kUnitKeys = 64;     // one unit of the split: 16 keys of each warp
+constexpr int kMinUnits = 4;      // a CTA takes at least 256 keys
+constexpr float kGrowLog2 = 8.0f;
+
+// The tile that a CTA's range begins inside, for the joining launch.
+struct Split {
+  long long first_unit, last_unit;  // of the tile; first_unit < 0: nothing to join here
+  int seq, tile, head, rows;        // rows: valid query rows of the tile
+};
+
+constexpr size_t partialFloats(int d) { return static_cast<size_t>(kStreamRows) * d + 2 * kStreamRows; }
+
+struct Share {
+  long long units, ctas;
+};
+
+__device__ __forceinline__ long long shareBegin(const Share& s, long long c) { return c * s.units / s.ctas; }
+__device__ __forceinline__ long long shareOwner(const Share& s, long long u) { return ((u + 1) * s.ctas - 1) / s.units; }
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float exp2Approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Keys and values are read once: no room in L1 for them.
+__device__ __forceinline__ uint4 loadOnce16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 loadOnce8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+// Shapes of one 16-key step.
+template <int D, bool kE4m3>
+struct Step {
+  static constexpr int kKRecords = kE4m3 ? D / 64 : D / 32;  // K records of a thread per 8 keys
+  static constexpr int kVCh = kE4m3 && D == 128 ? 16 : 8;    // channels of a thread's V record
+  static constexpr int kVRecords = D / (8 * kVCh);           // V records of a thread per key
+  static constexpr int kVRegs = kE4m3 ? kVCh / 4 : 4;
+};
+
+template <int D, bool kE4m3>
+struct StepData {
+  uint4 k[2][Step<D, kE4m3>::kKRecords];
+  uint32_t v[Step<D, kE4m3>::kVRecords][4][Step<D, kE4m3>::kVRegs];
+  float ks[4], vs[4];
+  int key0, lim;  // first key, valid keys of the 16
+};
+
+}  // namespace
+
+template <typename T, int D, KvKind kKind>
+__global__ void __launch_bounds__(kThreads) attentionStreamKernel(const Args a) {
+  constexpr bool kE4m3 = kKind == kPagedE4m3;
+  using S = Step<D, kE4m3>;
+  using M = std::conditional_t<kE4m3, __half, T>;  // type of the products
+  __shared__ float o_s[kWarps][kStreamRows][D + 4];
+  __shared__ float ml_s[kWarps][2][kStreamRows];
+  __shared__ long long scan_s[kWarps + 1];
+  __shared__ long long found_s[2];
+
+  tc::pdlTrigger();
+  tc::pdlWait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+
+  // ---- this CTA's part of the line ----
+  auto unitsOf = [&](int s, Sequence* out) -> long long {
+    const Sequence q = sequence<kKind>(a, s);
+    if (out != nullptr) *out = q;
+    const long long tiles = (static_cast<long long>(q.nq) * a.group + kStreamRows - 1) / kStreamRows;
+    return tiles * a.kv_heads * max((q.nk + kUnitKeys - 1) / kUnitKeys, 1);  // no keys: still zeros to write
+  };
+  long long sum = 0;
+  for (int s = tid; s < a.n_seq; s += kThreads) sum += unitsOf(s, nullptr);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) scan_s[warp] = sum;
+  __syncthreads();
+  Share share;
+  share.units = 0;
+  for (int w = 0; w < kWarps; ++w) share.units += scan_s[w];
+  share.ctas = min(static_cast<long long>(gridDim.x), (share.units + kMinUnits - 1) / kMinUnits);
+  Split* splits = reinterpret_cast<Split*>(a.workspace);
+  float* partials = reinterpret_cast<float*>(a.workspace + sizeof(Split) * kStreamCtas);
+  Split* split = splits + blockIdx.x;
+  if (static_cast<long long>(blockIdx.x) >= share.ctas) {
+    if (tid == 0) split->first_unit = -1;
+    return;
+  }
+  const long long begin = shareBegin(share, blockIdx.x), end = shareBegin(share, blockIdx.x + 1LL);
+  // The sequence that holds unit `begin`.
+  long long before = 0;
+  for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) {
+    const int s = s0 + tid;
+    const long long mine = s < a.n_seq ? unitsOf(s, nullptr) : 0;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    __syncthreads();
+    if (lane == 31) scan_s[warp] = upto;
+    __syncthreads();
+    long long base = before, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) base += scan_s[w];
+      all += scan_s[w];
+    }
+    if (begin >= base + upto - mine && begin < base + upto) {
+      found_s[0] = s;
+      found_s[1] = base + upto - mine;
+    }
+    before += all;
+    if (begin < before) break;
+  }
+  __syncthreads();
+  int seq = static_cast<int>(found_s[0]);
+  long long seq_first = found_s[1];
+  Sequence q;
+  long long seq_units = unitsOf(seq, &q);
+
+  const int q_heads_per = a.group;
+  bool first_piece = true;
+  for (long long u = begin; u < end;) {
+    while (u >= seq_first + seq_units) {  // the next sequence with rows
+      seq_first += seq_units;
+      seq_units = unitsOf(++seq, &q);
+    }
+    const int blocks = max((q.nk + kUnitKeys - 1) / kUnitKeys, 1);
+    const long long tile_head = (u - seq_first) / blocks;
+    const int tile = static_cast<int>(tile_head / a.kv_heads);
+    const int head = static_cast<int>(tile_head - static_cast<long long>(tile) * a.kv_heads);
+    const long long tile_first = seq_first + tile_head * blocks;
+    const int b0 = static_cast<int>(u - tile_first);
+    const int b1 = static_cast<int>(min(static_cast<long long>(blocks), end - tile_first));
+    const int rows = static_cast<int>(min(static_cast<long long>(kStreamRows), static_cast<long long>(q.nq) * a.group - static_cast<long long>(tile) * kStreamRows));
+
+    // Rows g and g + 8 of the tile.
+    int vis[2];
+    const unsigned char* qp[2];
+    int min_vis = q.nk;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int rr = g + 8 * i;
+      const long long r = static_cast<long long>(tile) * kStreamRows + rr;
+      const int token = static_cast<int>(r / q_heads_per);
+      vis[i] = rr < rows ? visible(a, q, token) : q.nk;
+      qp[i] = rr < rows ? record(a.q, head * q_heads_per + static_cast<int>(r - static_cast<long long>(token) * q_heads_per), q.q0 + token, 0) : nullptr;
+      min_vis = min(min_vis, vis[i]);
+    }
+    const int last_vis = visible(a, q, static_cast<int>((static_cast<long long>(tile) * kStreamRows + rows - 1) / q_heads_per));
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) min_vis = min(min_vis, __shfl_xor_sync(0xffffffffu, min_vis, o));
+
+    // Query fragments: the records of the channels that this thread's K records hold.
+    uint32_t qf[D / 16][4];
+    float row_scale[2] = {1.0f, 1.0f};
+    {
+      uint4 raw[2][D / 32];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+          const int plane = kE4m3 ? 2 * (4 * (n / 2) + t) + n % 2 : 4 * n + t;
+          raw[i][n] = qp[i] != nullptr ? *reinterpret_cast<const uint4*>(qp[i] + plane * a.q.plane_stride) : make_uint4(0, 0, 0, 0);
+        }
+      }
+      if constexpr (kE4m3) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float m = 0.0f;
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) {
+            float x[8];
+            unpack8<T>(raw[i][n], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+          }
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          // 2^(exponent of m), kept where its inverse is a normal number.
+          const int e = min(max((__float_as_int(m) >> 23) & 0xff, 1), 253) - 127;
+          row_scale[i] = m > 0.0f ? __int_as_float((e + 127) << 23) : 1.0f;
+          const float inv = m > 0.0f ? __int_as_float((127 - e) << 23) : 1.0f;
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) {
+            float x[8];
+            unpack8<T>(raw[i][n], x);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[c] *= inv;
+            raw[i][n] = pack8<__half>(x);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < D / 32; ++n) {
+        const uint4 lo = raw[0][n], hi = raw[1][n];
+        qf[2 * n][0] = lo.x, qf[2 * n][1] = hi.x, qf[2 * n][2] = lo.y, qf[2 * n][3] = hi.y;
+        qf[2 * n + 1][0] = lo.z, qf[2 * n + 1][1] = hi.z, qf[2 * n + 1][2] = lo.w, qf[2 * n + 1][3] = hi.w;
+      }
+    }
+
+    float o[S::kVRecords][S::kVCh][4];
+#pragma unroll
+    for (int i = 0; i < S::kVRecords; ++i) {
+#pragma unroll
+      for (int e = 0; e < S::kVCh; ++e) o[i][e][0] = o[i][e][1] = o[i][e][2] = o[i][e][3] = 0.0f;
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    // Steps of 16 keys, one warp after the other, up to the last visible key.
+    const int step_end = min(b1 * (kUnitKeys / 16), (last_vis + 15) >> 4);
+    StepData<D, kE4m3> d;
+    const unsigned char* vb = nullptr;
+    auto pageAt = [&](int step) -> int {
+      if constexpr (kKind == kPacked16) return 0;
+      return step < step_end ? pageOf(a, seq, step * 16) : 0;
+    };
+    auto loadK = [&](int step, int page) {
+      d.key0 = step * 16;
+      d.lim = min(16, last_vis - d.key0);
+      const unsigned char* kb;
+      if constexpr (kKind == kPacked16) {
+        kb = record(a.k, head, static_cast<long long>(q.k0) + d.key0, 0);
+        vb = record(a.v, head, static_cast<long long>(q.k0) + d.key0, 0);
+      } else {
+        if (page < 0) {
+          reportIndex(a.error_flag, FPK_ERROR_PAGE);
+          d.lim = 0;
+          page = 0;
+        }
+        const int r = d.key0 & ((1 << a.page_shift) - 1);
+        kb = record(a.k, head, r, 0) + page * a.page_stride;
+        vb = record(a.v, head, r, 0) + page * a.page_stride;
+        if constexpr (kE4m3) {
+          const long long at = ((static_cast<long long>(page) * a.kv_heads + head) << a.page_shift) + r + t;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool in = 4 * i + t < d.lim;
+            d.ks[i] = in ? __ldg(a.k_scale + at + 4 * i) : 0.0f;
+            d.vs[i] = in ? __ldg(a.v_scale + at + 4 * i) : 1.0f;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int key = 8 * j + 4 * (g & 1) + (g >> 1);
+#pragma unroll
+        for (int n = 0; n < S::kKRecords; ++n) {
+          d.k[j][n] = key < d.lim ? loadOnce16(kb + key * a.k.row_stride + (4 * n + t) * a.k.plane_stride) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    };
+    auto loadV = [&]() {
+#pragma unroll
+      for (int i = 0; i < S::kVRecords; ++i) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const int key = 4 * kk + t;
+          if constexpr (S::kVRegs == 4) {
+            const uint4 w = key < d.lim ? loadOnce16(vb + key * a.v.row_stride + (8 * i + g) * a.v.plane_stride) : make_uint4(0, 0, 0, 0);
+            d.v[i][kk][0] = w.x, d.v[i][kk][1] = w.y, d.v[i][kk][2] = w.z, d.v[i][kk][3] = w.w;
+          } else {
+            const uint2 w = key < d.lim ? loadOnce8(vb + key * a.v.row_stride + (g >> 1) * a.v.plane_stride + (g & 1) * 8) : make_uint2(0, 0);
+            d.v[i][kk][0] = w.x, d.v[i][kk][1] = w.y;
+          }
+        }
+      }
+    };
+
+    int step = b0 * (kUnitKeys / 16) + warp;
+    int page_next = 0;
+    if (step < step_end) {
+      loadK(step, pageAt(step));
+      loadV();
+      page_next = pageAt(step + kWarps);
+    }
+    for (; step < step_end; step += kWarps) {
+      const int key0 = d.key0, lim = d.lim;
+      float sc[2][4] = {};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if constexpr (kE4m3) {
+#pragma unroll
+          for (int n = 0; n < S::kKRecords; ++n) {
+            const uint32_t w[4] = {d.k[j][n].x, d.k[j][n].y, d.k[j][n].z, d.k[j][n].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma<M>(sc[j], qf[4 * n + e], e4m3x2ToHalf2(w[e]), e4m3x2ToHalf2(w[e] >> 16));
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < S::kKRecords; ++n) {
+            mma<M>(sc[j], qf[2 * n], d.k[j][n].x, d.k[j][n].y);
+            mma<M>(sc[j], qf[2 * n + 1], d.k[j][n].z, d.k[j][n].w);
+          }
+        }
+      }
+      float x[2][4];  // [row][key t, 4+t, 8+t, 12+t], log2 domain
+      float inv_v[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float s = sc[c >> 1][2 * i + (c & 1)];
+          if constexpr (kE4m3) {
+            const int ve = (__float_as_int(d.vs[c]) >> 23) - 127;
+            x[i][c] = fmaf(s * row_scale[i], d.ks[c] * a.scale_log2, static_cast<float>(ve));
+            inv_v[c] = __int_as_float((127 - ve) << 23);
+          } else {
+            x[i][c] = s * a.scale_log2;
+          }
+        }
+      }
+      const int next = step + kWarps;
+      if (next < step_end) loadK(next, page_next);
+      if (key0 + lim > min_vis || lim < 16) {  // the causal edge, the last keys, a bad page
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (4 * c + t >= lim || key0 + 4 * c + t >= vis[i]) x[i][c] = -INFINITY;
+          }
+        }
+      }
+      bool grow = false;
+      float mx[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
+        grow |= mx[i] > m[i] + kGrowLog2;
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+          const float m_new = fmaxf(m[i], mx[i]);
+          const float f = m[i] == m_new ? 1.0f : exp2Approx(m[i] - m_new);  // -inf stays: nothing to scale
+          m[i] = m_new;
+          l[i] *= f;
+#pragma unroll
+          for (int r = 0; r < S::kVRecords; ++r) {
+#pragma unroll
+            for (int e = 0; e < S::kVCh; ++e) {
+              o[r][e][2 * i] *= f;
+              o[r][e][2 * i + 1] *= f;
+            }
+          }
+        }
+      }
+      uint32_t p[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float neg = m[i] == -INFINITY ? 0.0f : -m[i];  // a row that has seen no key yet
+        float e[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          e[c] = exp2Approx(x[i][c] + neg);
+          l[i] = kE4m3 ? fmaf(e[c], inv_v[c], l[i]) : l[i] + e[c];
+        }
+        p[i] = pack2<M>(e[0], e[1]);
+        p[2 + i] = pack2<M>(e[2], e[3]);
+      }
+      // O += P V. Byte permutes bring two keys of one channel together.
+#pragma unroll
+      for (int i = 0; i < S::kVRecords; ++i) {
+        if constexpr (kE4m3) {
+#pragma unroll
+          for (int e = 0; e < S::kVCh; e += 2) {
+            uint32_t h[4];
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) h[kk] = e4m3x2ToHalf2(d.v[i][kk][e >> 2] >> ((e & 2) * 8));
+            mma<M>(o[i][e], p, __byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
+            mma<M>(o[i][e + 1], p, __byte_perm(h[0], h[1], 0x7632), __byte_perm(h[2], h[3], 0x7632));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const uint32_t h0 = d.v[i][0][e >> 1], h1 = d.v[i][1][e >> 1], h2 = d.v[i][2][e >> 1], h3 = d.v[i][3][e >> 1];
+            mma<M>(o[i][e], p, __byte_perm(h0, h1, 0x5410), __byte_perm(h2, h3, 0x5410));
+            mma<M>(o[i][e + 1], p, __byte_perm(h0, h1, 0x7632), __byte_perm(h2, h3, 0x7632));
+          }
+        }
+      }
+      if (next < step_end) {
+        loadV();
+        page_next = pageAt(next + kWarps);
+      }
+    }
+
+    // ---- join the warps ----
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      if (t == 0) {
+        ml_s[warp][0][g + 8 * i] = m[i];
+        ml_s[warp][1][g + 8 * i] = l[i];
+      }
+#pragma unroll
+      for (int r = 0; r < S::kVRecords; ++r) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+          for (int e = 0; e < S::kVCh; ++e) o_s[warp][g + 8 * i][(8 * r + 2 * t + n) * S::kVCh + e] = o[r][e][2 * i + n];
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = b0 == 0 && b1 == blocks;
+    float* part = partials + (2 * static_cast<size_t>(blockIdx.x) + (first_piece && b0 > 0 ? 0 : 1)) * partialFloats(D);
+    for (int i = tid; i < kStreamRows * (D / 8); i += kThreads) {
+      const int rr = i / (D / 8), grp = i % (D / 8);
+      if (rr >= rows) continue;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml_s[w][0][rr]);
+      float ll = 0.0f, acc[8] = {};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = ml_s[w][0][rr];
+        const float f = mw == mm ? 1.0f : exp2Approx(mw - mm);
+        ll = fmaf(ml_s[w][1][rr], f, ll);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(o_s[w][rr][grp * 8 + e], f, acc[e]);
+      }
+      if (whole) {
+        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] *= inv;
+        const long long r = static_cast<long long>(tile) * kStreamRows + rr;
+        const int token = static_cast<int>(r / q_heads_per);
+        const int h = head * q_heads_per + static_cast<int>(r - static_cast<long long>(token) * q_heads_per);
+        *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(acc);
+      } else {
+        float4* dst = reinterpret_cast<float4*>(part + rr * D + grp * 8);
+        dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        if (grp == 0) {
+          part[kStreamRows * D + rr] = mm;
+          part[kStreamRows * D + kStreamRows + rr] = ll;
+        }
+      }
+    }
+    if (first_piece && tid == 0) {
+      if (b0 > 0) {
+        split->first_unit = tile_first;
+        split->last_unit = tile_first + blocks - 1;
+        split->seq = seq;
+        split->tile = tile;
+        split->head = head;
+        split->rows = rows;
+      } else {
+        split->first_unit = -1;
+      }
+      // The joining launch needs the shares too.
+      if (blockIdx.x == 0) *reinterpret_cast<Share*>(partials + 2 * static_cast<size_t>(kStreamCtas) * partialFloats(D)) = share;
+    }
+    first_piece = false;
+    u = tile_first + b1;
+    __syncthreads();
+  }
+}
+
+constexpr int kJoinWarps = 16;
+
+// Joins the partials of a tile that several CTAs worked on: CTA c looks after
+// the tile in which share c begins, if it is the first share to begin there.
+template <typename T, int D, KvKind kKind>
+__global__ void __launch_bounds__(kJoinWarps * 32) joinStreamKernel(const Args a) {
+  __shared__ float acc_s[kJoinWarps][D];
+  __shared__ float ml_s[kJoinWarps][2];
+  tc::pdlTrigger();
+  tc::pdlWait();
+  const float* partials = reinterpret_cast<const float*>(a.workspace + sizeof(Split) * kStreamCtas);
+  const Split split = reinterpret_cast<const Split*>(a.workspace)[blockIdx.x];
+  if (split.first_unit < 0) return;
+  const Share share = *reinterpret_cast<const Share*>(partials + 2 * static_cast<size_t>(kStreamCtas) * partialFloats(D));
+  const long long c0 = shareOwner(share, split.first_unit);
+  if (c0 != static_cast<long long>(blockIdx.x) - 1) return;
+  const int n = static_cast<int>(shareOwner(share, split.last_unit) - c0) + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Warps of one row: kJoinWarps over the rows, rounded down to a power of two.
+  int per_row = 1;
+  while (per_row * 2 * split.rows <= kJoinWarps) per_row *= 2;
+  const int row = warp / per_row, sub = warp - row * per_row;
+  constexpr int kPer = D / 32;  // channels of a lane
+  float acc[kPer] = {}, m = -INFINITY, l = 0.0f;
+  if (row < split.rows) {
+    // Piece i of the tile is CTA c0 + i's: its last piece (1) for i = 0, its first (0) after.
+    auto piece = [&](int i) { return partials + (2 * static_cast<size_t>(c0 + i) + (i == 0 ? 1 : 0)) * partialFloats(D); };
+    for (int i = sub; i < n; i += per_row) m = fmaxf(m, __ldcg(piece(i) + kStreamRows * D + row));
+#pragma unroll 4
+    for (int i = sub; i < n; i += per_row) {
+      const float* p = piece(i);
+      const float pm = __ldcg(p + kStreamRows * D + row);
+      const float pl = __ldcg(p + kStreamRows * D + kStreamRows + row);
+      const float f = pm == m ? 1.0f : exp2Approx(pm - m);
+      l = fmaf(pl, f, l);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = fmaf(__ldcg(p + row * D + e * 32 + lane), f, acc[e]);
+    }
+    if (lane == 0) {
+      ml_s[warp][0] = m;
+      ml_s[warp][1] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc_s[warp][e * 32 + lane] = acc[e];
+  }
+  __syncthreads();
+  const Sequence q = sequence<kKind>(a, split.seq);
+  for (int i = threadIdx.x; i < split.rows * (D / 8); i += kJoinWarps * 32) {
+    const int rr = i / (D / 8), grp = i % (D / 8);
+    float mm = -INFINITY;
+    for (int w = 0; w < per_row; ++w) mm = fmaxf(mm, ml_s[rr * per_row + w][0]);
+    float ll = 0.0f, x[8] = {};
+    for (int w = 0; w < per_row; ++w) {
+      const float mw = ml_s[rr * per_row + w][0];
+      const float f = mw == mm ? 1.0f : exp2Approx(mw - mm);
+      ll = fmaf(ml_s[rr * per_row + w][1], f, ll);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = fmaf(acc_s[rr * per_row + w][grp * 8 + e], f, x[e]);
+    }
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= inv;
+    const long long r = static_cast<long long>(split.tile) * kStreamRows + rr;
+    const int token = static_cast<int>(r / a.group);
+    const int h = split.head * a.group + static_cast<int>(r - static_cast<long long>(token) * a.group);
+    *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(x);
+  }
+}
+
+long long streamWorkspaceBytes(int head_dim) {
+  return static_cast<long long>(sizeof(Split) * kStreamCtas + 2 * kStreamCtas * partialFloats(head_dim) * sizeof(float) + sizeof(Share));
+}
+
+namespace {
+
+template <typename T, int D, KvKind kKind>
+cudaError_t launchOne(const Args& a, cudaStream_t s) {
+  // As many CTAs as stay resident, so that equal shares end together.
+  static DeviceValue resident;
+  const int ctas = resident.get([](int dev) {
+    int sms = 148, per = 1;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attentionStreamKernel<T, D, kKind>, kThreads, 0);
+    return std::min(kStreamCtas, sms * std::max(per, 1));
+  });
+  prof::countLaunch(prof::kAttention, 2);
+  cudaError_t e = launchPdl(attentionStreamKernel<T, D, kKind>, dim3(ctas), dim3(kThreads), 0, s, a);
+  if (e != cudaSuccess) return e;
+  return launchPdl(joinStreamKernel<T, D, kKind>, dim3(ctas), dim3(kJoinWarps * 32), 0, s, a);
+}
+
+template <typename T, int D>
+cudaError_t launchKind(const Args& a, KvKind kind, cudaStream_t s) {
+  switch (kind) {
+    case kPacked16: return launchOne<T, D, kPacked16>(a, s);
+    case kPaged16: return launchOne<T, D, kPaged16>(a, s);
+    default: return launchOne<T, D, kPagedE4m3>(a, s);
+  }
+}
+
+}  // namespace
+
+cudaError_t launchStream(const Args& a, KvKind kind, int head_dim, int dtype, cudaStream_t s) {
+  if (dtype == FPK_DTYPE_BF16) {
+    return head_dim == 64 ? launchKind<__nv_bfloat16, 64>(a, kind, s) : launchKind<__nv_bfloat16, 128>(a, kind, s);
+  }
+  return head_dim == 64 ? launchKind<__half, 64>(a, kind, s) : launchKind<__half, 128>(a, kind, s);
+}
+
+}  // namespace seqattn
+}  // namespace fpb

@@ -1,0 +1,124 @@
+// Rows of heads, packed sequences and pages of cached rows: what the kernels
+// behind fpk_qk_norm_rotary, fpk_cache_write / _read, fpk_attention_packed and
+// fpk_attention_paged share. Device addressing, 16-bit and e4m3 conversions,
+// and the host's checks of the descriptors (include/fpk.h).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+#include "fpk.h"
+
+namespace fpb {
+
+int fail(const std::string& msg);
+int checkLaunch(const char* what);
+
+namespace heads {
+
+// Address of 16-byte group g of head h in row r.
+__device__ __forceinline__ unsigned char* record(const fpk_heads_t& v, int h, long long r, int g) {
+  return static_cast<unsigned char*>(v.data) + h * v.head_stride + r * v.row_stride + g * v.plane_stride;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t x);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t x) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) {
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<T>(u[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+}
+
+// Two e4m3 values as fp16 pairs (exact).
+__device__ __forceinline__ uint32_t e4m3x2ToHalf2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
+  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+
+__device__ __forceinline__ void reportIndex(int* error_flag, int code) {
+  if (error_flag != nullptr) atomicCAS(error_flag, 0, code);
+}
+
+// ---- host checks ----
+
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// nullptr if the heads can be addressed, else what is wrong with them.
+inline const char* headsProblem(const fpk_heads_t& v) {
+  if (v.data == nullptr) return "null pointer";
+  if (!aligned16(v.data) || v.head_stride % 16 || v.row_stride % 16 || v.plane_stride % 16) {
+    return "data and strides must be multiples of 16 bytes";
+  }
+  return nullptr;
+}
+
+inline bool is16Bit(int dtype) { return dtype == FPK_DTYPE_F16 || dtype == FPK_DTYPE_BF16; }
+
+inline std::string cacheProblem(const fpk_kv_cache_t& c, int dtype) {
+  if (c.k == nullptr || c.v == nullptr) return "the cache is null";
+  if (!aligned16(c.k) || !aligned16(c.v)) return "the cache must be 16-byte aligned";
+  if (c.dtype != FPK_DTYPE_E4M3 && c.dtype != dtype) return "a 16-bit cache must have the rows' type";
+  if (c.dtype == FPK_DTYPE_E4M3 && (c.k_scale == nullptr || c.v_scale == nullptr)) return "an e4m3 cache needs k_scale and v_scale";
+  if (c.head_dim != 64 && c.head_dim != 128) return "head_dim must be 64 or 128";
+  if (c.page_rows < 16 || c.page_rows > 1024 || (c.page_rows & (c.page_rows - 1)) != 0) {
+    return "page_rows must be a power of two from 16 to 1024";
+  }
+  if (c.n_pages <= 0 || c.kv_heads <= 0) return "n_pages and kv_heads must be positive";
+  if (static_cast<long long>(c.n_pages) * c.page_rows >= (1LL << 31)) return "n_pages * page_rows must be below 2^31";
+  return std::string();
+}
+
+// The launch goes to the current device: memory of another one is refused here
+// instead of faulting there.
+inline std::string deviceProblem(const void* p) {
+  cudaPointerAttributes at{};
+  if (cudaPointerGetAttributes(&at, p) != cudaSuccess) return std::string("pointer: ") + cudaGetErrorString(cudaGetLastError());
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return std::string("current device: ") + cudaGetErrorString(e);
+  if (at.type == cudaMemoryTypeUnregistered || at.type == cudaMemoryTypeHost) return "data is not in device memory";
+  if (at.type == cudaMemoryTypeDevice && at.device != dev) {
+    return "data is on device " + std::to_string(at.device) + ", the current device is " + std::to_string(dev);
+  }
+  return std::string();
+}
+
+}  // namespace heads
+}  // namespace fpb

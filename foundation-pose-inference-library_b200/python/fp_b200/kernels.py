@@ -7,6 +7,7 @@ Every wrapper raises :class:`FpkError` with the library's message on failure.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 from pathlib import Path
 
@@ -17,6 +18,11 @@ FPK_DTYPE_F32 = 0
 FPK_DTYPE_F16 = 1
 FPK_DTYPE_BF16 = 2
 FPK_DTYPE_F32_EXACT = 3  # fp32 kept exact (strict-FP32 networks)
+FPK_DTYPE_E4M3 = 4  # element type of a KvCache only
+FPK_ERROR_SLOT = 41  # codes that the calls with device-side indexes leave in their error flag
+FPK_ERROR_PAGE = 42
+FPK_ERROR_STARTS = 43
+FPK_ERROR_LENGTH = 44
 FPK_STATS_INTS = 8 + 65536
 
 
@@ -74,6 +80,13 @@ _SIGS = {
     "fpk_gemm_test_withhold_loads": (C.c_int, [C.c_int]),
     "fpk_attention": (C.c_int, [_P, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int, _P, C.c_longlong,
                                 C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P]),
+    "fpk_qk_norm_rotary": (C.c_int, [_P, _P]),
+    "fpk_cache_write": (C.c_int, [_P, _P]),
+    "fpk_cache_read": (C.c_int, [_P, _P]),
+    "fpk_attention_packed_workspace_bytes": (C.c_longlong, [_P]),
+    "fpk_attention_packed": (C.c_int, [_P, _P]),
+    "fpk_attention_paged_workspace_bytes": (C.c_longlong, [_P]),
+    "fpk_attention_paged": (C.c_int, [_P, _P]),
     "fpk_net_create": (C.c_void_p, [C.c_char_p, C.c_char_p, C.c_int, C.c_int]),
     "fpk_net_destroy": (None, [_P]),
     "fpk_net_refine": (C.c_int, [_P, _P, _P, C.c_int, _P, _P, _P]),
@@ -197,6 +210,116 @@ def attention(fl: FpkLibrary, qkv: int, qkv_plane_stride: int, qkv_layer_channel
     fl._check(fl.lib.fpk_attention(qkv, qkv_plane_stride, qkv_layer_channels, q_channel, k_channel, v_channel,
                                    out, out_plane_stride, out_layer_channels, layers, heads, seq_len, n_seq,
                                    dtype, error_flag, stream or None), "fpk_attention")
+
+
+class Heads(C.Structure):
+    """fpk_heads_t: rows of heads, strides in bytes. Heads.planar and Heads.rows fill it in."""
+    _fields_ = [("data", C.c_void_p), ("head_stride", C.c_longlong), ("row_stride", C.c_longlong),
+                ("plane_stride", C.c_longlong)]
+
+    @classmethod
+    def planar(cls, data: int, plane_stride: int, head_dim: int, channel: int = 0) -> "Heads":
+        """Heads from `channel` on of 16-bit planar activations (row 0 of plane 0 at `data`)."""
+        return cls(data + channel // 8 * plane_stride, head_dim // 8 * plane_stride, 16, plane_stride)
+
+    @classmethod
+    def rows(cls, data: int, row_channels: int, head_dim: int, channel: int = 0) -> "Heads":
+        """Heads from `channel` on of 16-bit rows of `row_channels` channels."""
+        return cls(data + channel * 2, head_dim * 2, row_channels * 2, 16)
+
+
+class QkRotaryDesc(C.Structure):
+    _fields_ = [
+        ("q", Heads), ("k", Heads), ("q_out", Heads), ("k_out", Heads), ("rows", C.c_int), ("q_heads", C.c_int),
+        ("kv_heads", C.c_int), ("head_dim", C.c_int), ("rotary_dim", C.c_int), ("interleaved", C.c_int),
+        ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("eps", C.c_float), ("positions", C.c_void_p),
+        ("inv_freq", C.c_void_p), ("rotary_scale", C.c_float), ("dtype", C.c_int),
+    ]
+
+
+class KvCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("n_pages", C.c_int),
+        ("page_rows", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("dtype", C.c_int),
+    ]
+
+
+class CacheCopyDesc(C.Structure):
+    _fields_ = [("cache", KvCache), ("k", Heads), ("v", Heads), ("rows", C.c_int), ("slots", C.c_void_p),
+                ("dtype", C.c_int), ("error_flag", C.c_void_p)]
+
+
+class PackedAttentionDesc(C.Structure):
+    _fields_ = [
+        ("q", Heads), ("k", Heads), ("v", Heads), ("out", Heads), ("q_heads", C.c_int), ("kv_heads", C.c_int),
+        ("head_dim", C.c_int), ("n_seq", C.c_int), ("q_rows", C.c_int), ("kv_rows", C.c_int), ("q_starts", C.c_void_p),
+        ("kv_starts", C.c_void_p), ("causal", C.c_int), ("scale", C.c_float), ("dtype", C.c_int),
+        ("error_flag", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong),
+    ]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = [
+        ("q", Heads), ("out", Heads), ("cache", KvCache), ("q_heads", C.c_int), ("n_seq", C.c_int), ("q_rows", C.c_int),
+        ("q_starts", C.c_void_p), ("kv_lengths", C.c_void_p), ("page_table", C.c_void_p), ("table_pages", C.c_int),
+        ("causal", C.c_int), ("scale", C.c_float), ("dtype", C.c_int), ("error_flag", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong),
+    ]
+
+
+def qk_norm_rotary(fl: FpkLibrary, desc: QkRotaryDesc, stream=0) -> None:
+    """fpk_qk_norm_rotary: RMS norm of query and key heads and rotary positions (include/fpk.h)."""
+    fl._check(fl.lib.fpk_qk_norm_rotary(C.byref(desc), stream or None), "fpk_qk_norm_rotary")
+
+
+def cache_write(fl: FpkLibrary, desc: CacheCopyDesc, stream=0) -> None:
+    """fpk_cache_write: rows of keys and values into slots of a paged cache."""
+    fl._check(fl.lib.fpk_cache_write(C.byref(desc), stream or None), "fpk_cache_write")
+
+
+def cache_read(fl: FpkLibrary, desc: CacheCopyDesc, stream=0) -> None:
+    """fpk_cache_read: slots of a paged cache back into rows of keys and values."""
+    fl._check(fl.lib.fpk_cache_read(C.byref(desc), stream or None), "fpk_cache_read")
+
+
+def attention_packed_workspace_bytes(fl: FpkLibrary, desc: PackedAttentionDesc) -> int:
+    return int(fl.lib.fpk_attention_packed_workspace_bytes(C.byref(desc)))
+
+
+def attention_packed(fl: FpkLibrary, desc: PackedAttentionDesc, stream=0) -> None:
+    """fpk_attention_packed: attention within packed sequences of different lengths."""
+    fl._check(fl.lib.fpk_attention_packed(C.byref(desc), stream or None), "fpk_attention_packed")
+
+
+def attention_paged_workspace_bytes(fl: FpkLibrary, desc: PagedAttentionDesc) -> int:
+    return int(fl.lib.fpk_attention_paged_workspace_bytes(C.byref(desc)))
+
+
+def attention_paged(fl: FpkLibrary, desc: PagedAttentionDesc, stream=0) -> None:
+    """fpk_attention_paged: attention of each sequence's newest rows over its cached keys and values."""
+    fl._check(fl.lib.fpk_attention_paged(C.byref(desc), stream or None), "fpk_attention_paged")
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, factor: float = 1.0, trained_length: int = 0,
+                       slow_turns: float = 1.0, fast_turns: float = 32.0) -> list[float]:
+    """The table inv_freq of fpk_qk_norm_rotary: base^(-2i/rotary_dim), i < rotary_dim/2.
+
+    For contexts `factor` times as long as the trained ones: with trained_length 0 every frequency
+    is divided by factor (positions are interpolated). With trained_length given, only slow
+    frequencies are: those that turn fewer than slow_turns times over the trained length are divided
+    whole, those above fast_turns are kept, and between the two the share kept grows linearly.
+    """
+    if rotary_dim <= 0 or rotary_dim % 2 or base <= 0 or factor <= 0 or fast_turns <= slow_turns:
+        raise ValueError("rotary_frequencies: rotary_dim must be even, base and factor positive, fast_turns above slow_turns")
+    out = []
+    for i in range(rotary_dim // 2):
+        f = base ** (-2.0 * i / rotary_dim)
+        kept = 0.0
+        if trained_length > 0:
+            turns = trained_length * f / (2.0 * math.pi)
+            kept = min(1.0, max(0.0, (turns - slow_turns) / (fast_turns - slow_turns)))
+        out.append(f * kept + f / factor * (1.0 - kept))
+    return out
 
 
 class Networks:

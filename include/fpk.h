@@ -62,6 +62,9 @@ typedef struct fpk_mesh {
  * exact-FP32 layers, which sum three TF32 products of split operands);
  * fpk_attention runs fp32 FMA arithmetic; fpk_render_pack stores plain fp32. */
 #define FPK_DTYPE_F32_EXACT 3
+/* 8-bit floating point (4 exponent, 3 mantissa bits, largest value 448): only as
+ * the element type of an fpk_kv_cache_t. */
+#define FPK_DTYPE_E4M3 4
 
 /* Size in int32 of the translation-statistics scratch (bbox, count, 65,536-bin histogram). */
 #define FPK_STATS_INTS (8 + 65536)
@@ -273,6 +276,159 @@ FP_API int fpk_attention(const void* qkv, long long qkv_plane_stride, int qkv_la
                          int q_channel, int k_channel, int v_channel, void* out,
                          long long out_plane_stride, int out_layer_channels, int layers, int heads,
                          int seq_len, int n_seq, int dtype, int* error_flag, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Attention over heads, packed sequences and a paged cache (FP16 / BF16; no
+ * counterpart in the reference, whose engines attend within sequences of one
+ * length). In the order of a transformer block: fpk_qk_norm_rotary on the
+ * projected queries and keys, then either fpk_attention_packed over whole
+ * sequences, or fpk_cache_write and fpk_attention_paged for sequences that
+ * grow from call to call.
+ *
+ * fpk_heads_t names the rows of several heads in memory. Channels
+ * 8g..8g+7 of head h in row r are the 16 bytes at
+ *   data + h*head_stride + r*row_stride + g*plane_stride.
+ * The planar layout of fpk_gemm is {row_stride 16, head_stride
+ * (head_dim/8)*plane_stride}; row-major [rows][heads][head_dim] is
+ * {row_stride of the tensor, head_stride head_dim*2, plane_stride 16}. data and
+ * all strides are multiples of 16 bytes. Outputs may not overlap inputs except
+ * where an entry point says so, nor themselves.
+ *
+ * Row indexes, lengths and page numbers are read on the device, so captured
+ * graphs follow their current values. Kernels check them against the sizes of
+ * the descriptor: a call never reads or writes outside the buffers it was
+ * given, and records one of these codes in *error_flag (device int32, zeroed by
+ * the caller beforehand; NULL to do without) when it met a bad one: */
+#define FPK_ERROR_SLOT 41   /* a slot >= n_pages*page_rows: that row was skipped */
+#define FPK_ERROR_PAGE 42   /* a page number outside the cache: its keys were treated as masked */
+#define FPK_ERROR_STARTS 43 /* starts that decrease or pass the buffer: clamped */
+#define FPK_ERROR_LENGTH 44 /* a length outside [0, table_pages*page_rows]: clamped */
+/* 51..59: a bounded wait inside the tensor-core kernel ran out; the tile was not stored. */
+
+typedef struct fpk_heads {
+  void* data;
+  long long head_stride, row_stride, plane_stride; /* bytes */
+} fpk_heads_t;
+
+/* RMS normalisation of every query and key head followed by the rotary
+ * position, one pass, fp32 arithmetic, one rounding:
+ *   x'    = x * rsqrt(mean(x^2) + eps) * weight          (weight NULL: x' = x)
+ *   a, b -> a cos - b sin, b cos + a sin                  on pairs of channels,
+ *   cos, sin = rotary_scale * (cos, sin)(positions[row] * inv_freq[i])
+ * pairing channels (i, i + rotary_dim/2), or (2i, 2i+1) with interleaved != 0,
+ * for i < rotary_dim/2; channels from rotary_dim on are only normalised. The
+ * angle is formed in double precision, so far positions keep fp32 accuracy.
+ * inv_freq carries any scaling for long contexts (fp_b200.kernels.
+ * rotary_frequencies); rotary_scale is its factor on the logits' square root.
+ * head_dim: a multiple of 8 up to 256; rotary_dim: a multiple of 16 up to
+ * head_dim, 0 for the norm alone (positions and inv_freq are then not read).
+ * q_heads or kv_heads may be 0. q_out / k_out may be q / k themselves. */
+typedef struct fpk_qk_rotary_desc {
+  fpk_heads_t q, k, q_out, k_out;
+  int rows, q_heads, kv_heads, head_dim, rotary_dim, interleaved;
+  const float* q_weight; /* [head_dim] or NULL */
+  const float* k_weight;
+  float eps;
+  const int32_t* positions; /* [rows] */
+  const float* inv_freq;    /* [rotary_dim/2], radians per position */
+  float rotary_scale;
+  int dtype; /* FPK_DTYPE_F16 or FPK_DTYPE_BF16 */
+} fpk_qk_rotary_desc_t;
+
+FP_API int fpk_qk_norm_rotary(const fpk_qk_rotary_desc_t* desc, void* stream);
+
+/* Keys and values of many sequences in pages of page_rows rows (a power of two,
+ * 16 to 1024). Slot i is row i % page_rows of page i / page_rows. k and v each
+ * hold [n_pages][kv_heads][group][page_rows] records of 16 bytes: 8 channels of
+ * FP16 / BF16, or 16 channels of E4M3 with one scale (a power of two) per row
+ * and head in k_scale / v_scale [n_pages][kv_heads][page_rows]; an element's
+ * value is e4m3 * scale. head_dim is 64 or 128; n_pages*page_rows < 2^31. */
+typedef struct fpk_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale; /* E4M3 only, else NULL */
+  float* v_scale;
+  int n_pages, page_rows, kv_heads, head_dim;
+  int dtype; /* FPK_DTYPE_F16, FPK_DTYPE_BF16 or FPK_DTYPE_E4M3 */
+} fpk_kv_cache_t;
+
+/* fpk_cache_write stores row i of k and v in slot slots[i] of the cache;
+ * fpk_cache_read brings it back (into k and v). Rows with a negative slot are
+ * left out (a padded batch), and rows and slots not named are left as they
+ * were. A 16-bit cache has the rows' type and holds them bit for bit. For E4M3 the
+ * scale is the smallest power of two (2^-100 at least) with max|row| <=
+ * 448*scale, 1 for a row of zeros; elements are rounded to nearest even, and an
+ * infinity or NaN is kept as NaN and does not count in the maximum. Reading
+ * rounds value*scale to the rows' type, saturating at its largest finite value.
+ * A slot that is written twice in one call holds a mixture of the two rows. */
+typedef struct fpk_cache_copy_desc {
+  fpk_kv_cache_t cache;
+  fpk_heads_t k, v;
+  int rows;
+  const int32_t* slots; /* [rows] */
+  int dtype;            /* of k and v: FPK_DTYPE_F16 or FPK_DTYPE_BF16 */
+  int* error_flag;
+} fpk_cache_copy_desc_t;
+
+FP_API int fpk_cache_write(const fpk_cache_copy_desc_t* desc, void* stream);
+FP_API int fpk_cache_read(const fpk_cache_copy_desc_t* desc, void* stream);
+
+/* Attention over n_seq packed sequences: sequence s has query rows
+ * [q_starts[s], q_starts[s+1]) of q / out and key rows [kv_starts[s],
+ * kv_starts[s+1]) of k / v. Query head h attends to key head h / (q_heads /
+ * kv_heads): out = softmax(scale * q k^T) v over the keys that it sees, all of
+ * the sequence's, or with causal != 0 keys 0 .. kv_length - q_length + i for its
+ * query i (the last query sees the last key). A query that sees no key gets
+ * zeros. Rows of no sequence are neither read into a result nor written, whatever they
+ * hold. scale 0 means 1/sqrt(head_dim). head_dim is 64 or 128, q_heads a
+ * multiple of kv_heads, at most 128 query heads to a key head. Products run on
+ * the tensor cores with probabilities rounded to the element type; scores,
+ * softmax statistics and sums are fp32. An infinity or NaN in V reaches, besides the
+ * queries that see its key, those of its tile whose causal mask hides it.
+ * workspace (fpk_attention_packed_workspace_bytes, 16-byte aligned, needs no
+ * initialising) holds the partial results of sequences that are split over
+ * several CTAs; calls that may overlap on the GPU need one each. */
+typedef struct fpk_attention_packed_desc {
+  fpk_heads_t q, k, v, out;
+  int q_heads, kv_heads, head_dim, n_seq;
+  int q_rows, kv_rows;       /* rows of the buffers */
+  const int32_t* q_starts;   /* [n_seq + 1] */
+  const int32_t* kv_starts;  /* [n_seq + 1] */
+  int causal;
+  float scale;
+  int dtype; /* FPK_DTYPE_F16 or FPK_DTYPE_BF16 */
+  int* error_flag;
+  void* workspace;
+  long long workspace_bytes;
+} fpk_attention_packed_desc_t;
+
+FP_API long long fpk_attention_packed_workspace_bytes(const fpk_attention_packed_desc_t* desc);
+FP_API int fpk_attention_packed(const fpk_attention_packed_desc_t* desc, void* stream);
+
+/* Attention of the newest rows of n_seq sequences over their cached keys and
+ * values (the new rows' own among them, written beforehand): as
+ * fpk_attention_packed, with key j of sequence s in row j % page_rows of page
+ * page_table[s*table_pages + j / page_rows] and kv_lengths[s] keys. Any number
+ * of query rows per sequence: one, or a chunk. Entries of the table past a
+ * sequence's last page are not read. */
+typedef struct fpk_attention_paged_desc {
+  fpk_heads_t q, out;
+  fpk_kv_cache_t cache;
+  int q_heads, n_seq, q_rows;
+  const int32_t* q_starts;   /* [n_seq + 1] */
+  const int32_t* kv_lengths; /* [n_seq] */
+  const int32_t* page_table; /* [n_seq][table_pages] */
+  int table_pages;
+  int causal;
+  float scale;
+  int dtype; /* of q and out; a 16-bit cache has the same */
+  int* error_flag;
+  void* workspace;
+  long long workspace_bytes;
+} fpk_attention_paged_desc_t;
+
+FP_API long long fpk_attention_paged_workspace_bytes(const fpk_attention_paged_desc_t* desc);
+FP_API int fpk_attention_paged(const fpk_attention_paged_desc_t* desc, void* stream);
 
 /* ---------------------------------------------------------------------------
  * RefineNet / ScoreNet as a unit: the built-in inference backend behind
