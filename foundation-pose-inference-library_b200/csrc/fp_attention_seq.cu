@@ -36,10 +36,20 @@ float scaleLog2(float scale, int head_dim) {
   return kLog2e * (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(head_dim)));
 }
 
-long long workspaceBytes(const Shape& n) { return streamWorkspaceBytes(n.head_dim); }
+// Rows (tokens x query heads to a key head) of a sequence on average, the
+// longest that the streaming kernel takes. Lengths are on the device, so the
+// choice goes by the average; either kernel is right for any lengths.
+constexpr int kStreamMostRows = 64;
+
+bool useTiles(const Shape& n) {
+  return static_cast<long long>(n.q_rows) * (n.q_heads / n.kv_heads) > static_cast<long long>(kStreamMostRows) * n.n_seq;
+}
+
+long long workspaceBytes(const Shape& n) { return useTiles(n) ? tilesWorkspaceBytes(n.head_dim) : streamWorkspaceBytes(n.head_dim); }
 
 int launch(const std::string& name, const Args& a, KvKind kind, const Shape& n, int dtype, void* stream) {
-  const cudaError_t e = launchStream(a, kind, n.head_dim, dtype, static_cast<cudaStream_t>(stream));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = useTiles(n) ? launchTiles(a, kind, n.head_dim, dtype, s) : launchStream(a, kind, n.head_dim, dtype, s);
   if (e != cudaSuccess) return fail(name + ": " + cudaGetErrorString(e));
   return 0;
 }
@@ -100,6 +110,7 @@ extern "C" int fpk_attention_packed(const fpk_attention_packed_desc_t* d, void* 
   a.kv_rows = d->kv_rows;
   a.kv_heads = d->kv_heads;
   a.group = d->q_heads / d->kv_heads;
+  a.group_inv = (65536 + a.group - 1) / a.group;
   a.causal = d->causal != 0;
   a.scale_log2 = scaleLog2(d->scale, d->head_dim);
   a.error_flag = d->error_flag;
@@ -152,6 +163,7 @@ extern "C" int fpk_attention_paged(const fpk_attention_paged_desc_t* d, void* st
   a.q_rows = d->q_rows;
   a.kv_heads = c.kv_heads;
   a.group = d->q_heads / c.kv_heads;
+  a.group_inv = (65536 + a.group - 1) / a.group;
   a.causal = d->causal != 0;
   a.scale_log2 = scaleLog2(d->scale, c.head_dim);
   a.error_flag = d->error_flag;

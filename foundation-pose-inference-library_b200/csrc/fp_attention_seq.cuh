@@ -30,6 +30,7 @@ struct Args {
   long long page_stride;      // bytes of one page, all heads
   int table_pages, n_pages, page_shift;
   int n_seq, q_rows, kv_rows, kv_heads, group;
+  int group_inv;              // ceil(2^16 / group): x * group_inv >> 16 = x / group for x * group < 2^16
   int causal;
   float scale_log2;           // scale * log2(e)
   int* error_flag;
@@ -84,7 +85,12 @@ __device__ __forceinline__ int pageOf(const Args& a, int s, int key) {
 constexpr int kStreamCtas = 592;  // most CTAs of the streaming kernel: 4 on each of 148 SMs
 constexpr int kStreamRows = 16;   // query rows of its tile
 
+constexpr int kTileCtas = 148;    // most CTAs of the tile kernel: one on each SM
+constexpr int kTileRows = 256;    // query rows of its tile
+
 long long streamWorkspaceBytes(int head_dim);
+long long tilesWorkspaceBytes(int head_dim);
+cudaError_t launchTiles(const Args& a, KvKind kind, int head_dim, int dtype, cudaStream_t s);
 cudaError_t launchStream(const Args& a, KvKind kind, int head_dim, int dtype, cudaStream_t s);
 
 }  // namespace seqattn

@@ -1,0 +1,893 @@
+// Attention of many query rows (prompts, chunks over a cache) on tcgen05 tensor
+// cores: fpk_attention_packed and fpk_attention_paged where a sequence has more
+// than a few dozen query rows (tokens x query heads to a key head).
+//
+// Bound by the tensor cores (4 d FLOP for each query row and key) and, as
+// closely, by the exponential unit: for d = 128 a 128 x 128 block of scores
+// takes 1,024 cycles of MMA and 16,384 / 16 = 1,024 cycles of ex2.
+//
+// One persistent CTA per SM, 512 threads. Its tile is 256 query rows of one
+// (sequence, key head), two halves of 128 rows that take turns: while the
+// softmax of one half runs, the tensor core works for the other.
+//   warps 0-3, 4-7  softmax of half 0 and 1, one query row per thread: the
+//                   row's 128 scores from TMEM, running maximum and sum in
+//                   fp32, P = 2^(s - m) rounded to the element type over the
+//                   scores' own TMEM columns. O is rescaled only when a row's
+//                   maximum grows by more than 2^8. After the last block, O / l.
+//   warps 8-11      loads: Q, K and V records into no-swizzle core-matrix
+//                   tiles [group of 8 channels][row][16 B], K and V in four
+//                   stages of 128 rows. 16-bit rows by cp.async, which takes any
+//                   strides, pages that end inside a block and zero fill of
+//                   keys that nobody sees, and arrives on the stage's barrier by
+//                   itself; e4m3 rows through registers, where they become the
+//                   element type (exact in bf16). A group's rows are padded by
+//                   16 bytes so that row-major sources write without bank
+//                   conflicts.
+//   warp 12         MMA issue: S_t = Q_t K^T, O_t += P_t V, in the order
+//                   PV_0(n) S_0(n+1) PV_1(n) S_1(n+1), across tiles too: the
+//                   next tile's first scores do not wait for this tile's output.
+//   warp 13         the walk: the next pieces of work for the others.
+// Registers go to the softmax warps, which hold a row of scores each
+// (setmaxnreg: 2 x 128 x 168 + 128 x 96 + 128 x 80 = 65,536).
+// TMEM: S_0 S_1 (128 columns each) O_0 O_1 (d each), one CTA per SM.
+//
+// The work of all tiles is laid on one line (a tile's length: the keys that it
+// sees) and cut into one share per CTA, so that causal and ragged batches and
+// few long rows all end together. A tile cut inside leaves fp32 partials that a
+// second launch joins in order; where tiles are short against a share, cuts
+// move to tile ends and nothing is joined. All mbarrier waits are bounded.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "fp_attention_seq.cuh"
+#include "fp_launch.hpp"
+#include "fp_profile.hpp"
+#include "fp_tc.cuh"
+
+namespace fpb {
+namespace seqattn {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kHalf = 128;       // rows of a half tile = TMEM lanes
+constexpr int kKeys = 128;       // keys of a block
+constexpr int kStages = 4;       // K 0, V 0, K 1, V 1
+constexpr int kItems = 4;        // work items in flight between the roles
+constexpr int kLoadWarps = 4;
+constexpr int kThreads = 512;
+constexpr uint32_t kPlane = kKeys * 16 + 16;  // a group's rows, padded
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kOCol = 256;
+constexpr uint32_t kPCol = 64;   // P among a half's 128 score columns
+constexpr float kGrowLog2 = 8.0f;
+constexpr int kMinShare = 256;   // keys
+constexpr int kSnap = 8;         // a tile shorter than 1/8 share is not cut
+
+struct Item {
+  int halves;                  // halves with rows; 0: no more work
+  int seq, head, tile;
+  int q0, nq, k0, nk;
+  int jb, je;                  // key blocks of this piece
+  int lim;                     // keys that the tile sees
+  int part;                    // -1: the whole tile; else the partial's index
+};
+
+// What the joining launch needs of a CTA: the tile that its share begins inside.
+struct Cut {
+  long long tile_at;           // the tile's place on the line, -1: nothing cut
+  int jb, blocks;
+  int seq, head, tile, pad;
+};
+
+struct Smem {
+  uint64_t item_full[kItems], item_empty[kItems];
+  uint64_t q_full[2], q_empty[2];
+  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t s_full[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t drained;
+  Item items[kItems];
+  long long scan[kThreads / 32 + 1];
+  long long found[2];
+  uint32_t tmem;
+  int stop;                    // a wait ran out: every role leaves
+};
+
+template <int D>
+struct Geo {
+  static constexpr int kPlanes = D / 8;
+  static constexpr uint32_t kTileBytes = kPlanes * kPlane;  // 128 rows
+  static constexpr size_t kSmem = 1024 + (2 + kStages) * static_cast<size_t>(kTileBytes) + 128;
+};
+static_assert(sizeof(Smem) <= 1024, "barrier block");
+
+// fp32 partial of a piece: [D/4][256 rows][4], m [256], l [256].
+constexpr size_t partialFloats(int d) { return static_cast<size_t>(kTileRows) * d + 2 * kTileRows; }
+
+// ---- the line of work ----
+
+// Tile i of a sequence and head is long w(i): 1 + the keys that its last full
+// token row sees (causal: growing by the tokens of a tile), in closed form.
+struct Line {
+  int tiles;
+  int first, step;  // w(i) = 1 + clamp(first + i * step, 0, nk)
+  int nk;
+};
+
+__device__ __forceinline__ Line lineOf(const Args& a, const Sequence& q) {
+  Line n;
+  n.tiles = static_cast<int>((static_cast<long long>(q.nq) * a.group + kTileRows - 1) / kTileRows);
+  n.nk = q.nk;
+  n.step = a.causal ? max(kTileRows / a.group, 1) : 0;
+  n.first = a.causal ? q.nk - q.nq + n.step : q.nk;
+  return n;
+}
+
+__device__ __forceinline__ long long tileLength(const Line& n, int i) {
+  return 1 + min(max(n.first + static_cast<long long>(i) * n.step, 0LL), static_cast<long long>(n.nk));
+}
+
+// Sum of tileLength over tiles 0 .. i-1.
+__device__ __forceinline__ long long lengthBefore(const Line& n, int i) {
+  if (n.step == 0) return i * tileLength(n, 0);
+  // first + k*step >= 0 from k0 on, >= nk from k1 on.
+  const long long k0 = n.first >= 0 ? 0 : (-static_cast<long long>(n.first) + n.step - 1) / n.step;
+  const long long k1 = n.first >= n.nk ? 0 : (static_cast<long long>(n.nk) - n.first + n.step - 1) / n.step;
+  const long long lo = min(k0, static_cast<long long>(i)), hi = min(max(k1, k0), static_cast<long long>(i));
+  const long long ramp = hi - lo;
+  return i + ramp * n.first + n.step * ((lo + hi - 1) * ramp / 2) + (i - hi) * static_cast<long long>(n.nk);
+}
+
+// The tile that holds place x of a head's line.
+__device__ __forceinline__ int tileAt(const Line& n, long long x) {
+  int lo = 0, hi = n.tiles - 1;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo + 1) / 2;
+    if (lengthBefore(n, mid) <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int blocksOf(int lim) { return max((lim + kKeys - 1) / kKeys, 1); }
+
+// Keys that a tile sees: those of its last row.
+__device__ __forceinline__ int tileLimit(const Args& a, const Sequence& q, int tile) {
+  const long long last = min(static_cast<long long>(q.nq) * a.group, (tile + 1LL) * kTileRows) - 1;
+  return visible(a, q, static_cast<int>(last / a.group));
+}
+
+// Key block at which place y of a tile of length w cuts it.
+__device__ __forceinline__ int cutBlock(long long y, long long w, int blocks, long long share) {
+  if (w * kSnap <= share) return 2 * y < w ? 0 : blocks;
+  return static_cast<int>(blocks * y / w);
+}
+
+// ---- waits ----
+
+__device__ __forceinline__ bool waitSlow(uint64_t* bar, uint32_t parity, volatile int* stop, int* err, int code) {
+  const long long start = clock64();
+  for (uint32_t i = 0;; ++i) {
+    if (mbarTryWait(bar, parity)) return true;
+    if ((i & 255u) == 255u) {
+      if (*stop != 0) return false;
+      if (clock64() - start > kTimeoutCycles) {
+        *stop = 1;
+        reportIndex(err, code);
+        return false;
+      }
+    }
+  }
+}
+
+// By a whole (converged) warp; lane 0's outcome is the warp's.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Smem& sm, int* err, int code) {
+  const bool ok = mbarTryWait(bar, parity) || waitSlow(bar, parity, &sm.stop, err, code);
+  return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+}
+
+__host__ __device__ constexpr uint32_t idesc(uint32_t fmt, int n, bool b_mn_major) {
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn_major ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kHalf >> 4) << 24);
+}
+
+__device__ __forceinline__ float exp2Approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void copyAsync16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+// One arrival of this thread on `bar` once its earlier copyAsync16 have landed.
+__device__ __forceinline__ void copyArrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smemU32(bar)) : "memory");
+}
+__device__ __forceinline__ void copyDrain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void moreRegisters() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewerRegisters() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ void storeShared16(uint32_t dst, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+}  // namespace
+
+template <typename T, int D, KvKind kKind>
+__global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a) {
+  using G = Geo<D>;
+  constexpr int kPlanes = G::kPlanes;
+  constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
+  Smem& sm = *reinterpret_cast<Smem*>(base);
+  const uint32_t q_s = smemU32(base + 1024);
+  const uint32_t kv_s = q_s + 2 * G::kTileBytes;
+
+  tc::pdlTrigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < kItems; ++i) {
+      mbarInit(&sm.item_full[i], 1);
+      mbarInit(&sm.item_empty[i], 8 + 1 + kLoadWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbarInit(&sm.q_full[i], kLoadWarps * 32);
+      mbarInit(&sm.q_empty[i], 1);
+      mbarInit(&sm.s_full[i], 1);
+      mbarInit(&sm.p_full[i], 4);
+      mbarInit(&sm.pv_done[i], 1);
+      mbarInit(&sm.o_free[i], 4);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbarInit(&sm.kv_full[i], kLoadWarps * 32);
+      mbarInit(&sm.kv_empty[i], 1);
+    }
+    mbarInit(&sm.drained, 1);
+    sm.stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smemU32(&sm.tmem)), "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc::pdlWait();
+
+  // ---- this CTA's share of the line ----
+  Cut* cuts = reinterpret_cast<Cut*>(a.workspace);
+  float* partials = reinterpret_cast<float*>(a.workspace + sizeof(Cut) * kTileCtas);
+  auto lengthOf = [&](int s) -> long long {
+    if (s >= a.n_seq) return 0;
+    const Line n = lineOf(a, sequence<kKind>(a, s));
+    return lengthBefore(n, n.tiles) * a.kv_heads;
+  };
+  // Lengths of kThreads sequences and their sums up to each thread's.
+  long long mine = 0, at = 0, total = 0;
+  auto scan = [&](int s0) -> long long {
+    mine = lengthOf(s0 + tid);
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    __syncthreads();
+    if (lane == 31) sm.scan[warp] = upto;
+    __syncthreads();
+    long long all = 0;
+    at = upto - mine;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) at += sm.scan[w];
+      all += sm.scan[w];
+    }
+    return all;
+  };
+  for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) total += scan(s0);
+  // Shares of kMinShare keys or more: none is empty, and a tile's cuts differ.
+  const long long n_cta = max(1LL, min(static_cast<long long>(gridDim.x), total / kMinShare));
+  const long long begin = min(static_cast<long long>(blockIdx.x), n_cta) * total / n_cta;
+  const long long end = min(blockIdx.x + 1LL, n_cta) * total / n_cta;
+  const long long share = total / n_cta;
+  if (begin < end) {
+    long long before = 0;
+    for (int s0 = 0; s0 < a.n_seq && before <= begin; s0 += kThreads) {
+      const long long all = a.n_seq > kThreads ? scan(s0) : total;  // one pass: still at hand
+      if (begin >= before + at && begin < before + at + mine) {
+        sm.found[0] = s0 + tid;
+        sm.found[1] = before + at;
+      }
+      before += all;
+    }
+  }
+  tcFenceBefore();
+  __syncthreads();
+  tcFenceAfter();
+  const uint32_t tmem = sm.tmem;
+  int* err = a.error_flag;
+
+  if (warp >= 12) {
+    fewerRegisters<80>();
+    if (warp == 12) {
+      // ---------------- MMA issue ----------------
+      const uint32_t idesc_o = idesc(kFmt, D, true);
+      bool ok = true;
+      Item cur{}, nxt{};
+      int i_next = 0;                 // items read so far
+      auto readItem = [&](Item& it) -> bool {
+        const int slot = i_next % kItems;
+        if (!wait(&sm.item_full[slot], (i_next / kItems) & 1, sm, err, 55)) return false;
+        it = sm.items[slot];
+        __syncwarp();
+        if (lane == 0) mbarArrive(&sm.item_empty[slot]);
+        ++i_next;
+        return true;
+      };
+      int n = 0;                                  // key blocks before the current one
+      int s_count[2] = {0, 0}, q_count[2] = {0, 0};  // score blocks issued, tiles begun
+      int pv_count[2] = {0, 0}, o_count[2] = {0, 0};
+      auto issueS = [&](const Item& it, int t, int j, int block) -> bool {
+        if (j == it.jb) {
+          if (!wait(&sm.q_full[t], q_count[t] & 1, sm, err, 56)) return false;
+          ++q_count[t];
+        }
+        const int stage = (block & 1) * 2;
+        if (t == 0 && !wait(&sm.kv_full[stage], (block >> 1) & 1, sm, err, 57)) return false;
+        fenceProxyAsyncSmem();  // what the loading warps' copies wrote
+        tcFenceAfter();
+        const int keys = min(kKeys, max(it.lim - j * kKeys, 1));
+        const uint32_t id = idesc(kFmt, (keys + 15) & ~15, false);
+        const uint32_t d = tmem + t * kKeys;
+        const uint32_t qa = q_s + t * G::kTileBytes, ka = kv_s + stage * G::kTileBytes;
+  #pragma unroll
+        for (int ks = 0; ks < kPlanes / 2; ++ks) {
+          tcMmaElect(d, smemDesc(qa + ks * 2 * kPlane, kPlane, 128, kLayoutNone), smemDesc(ka + ks * 2 * kPlane, kPlane, 128, kLayoutNone), id,
+                     ks > 0 ? 1u : 0u);
+        }
+        tcCommitElect(&sm.s_full[t]);
+        if (t == it.halves - 1) tcCommitElect(&sm.kv_empty[stage]);
+        if (j == it.je - 1) tcCommitElect(&sm.q_empty[t]);
+        ++s_count[t];
+        return true;
+      };
+      auto issuePV = [&](const Item& it, int t, int j, int block) -> bool {
+        if (!wait(&sm.p_full[t], pv_count[t] & 1, sm, err, 58)) return false;
+        const int stage = (block & 1) * 2 + 1;
+        if (t == 0 && !wait(&sm.kv_full[stage], (block >> 1) & 1, sm, err, 57)) return false;
+        if (j == it.jb) {
+          if (o_count[t] > 0 && !wait(&sm.o_free[t], (o_count[t] - 1) & 1, sm, err, 59)) return false;
+          ++o_count[t];
+        }
+        fenceProxyAsyncSmem();  // what the loading warps' copies wrote
+        tcFenceAfter();
+        const int keys = min(kKeys, max(it.lim - j * kKeys, 1));
+        const int steps = (keys + 15) >> 4;
+        const uint32_t va = kv_s + stage * G::kTileBytes;
+        for (int ks = 0; ks < steps; ++ks) {
+          tcMmaTmemAElect(tmem + kOCol + t * D, tmem + t * kKeys + kPCol + ks * 8, smemDesc(va + ks * 256, 128, kPlane, kLayoutNone), idesc_o,
+                          (j > it.jb || ks > 0) ? 1u : 0u);
+        }
+        tcCommitElect(&sm.pv_done[t]);
+        if (t == it.halves - 1) tcCommitElect(&sm.kv_empty[stage]);
+        ++pv_count[t];
+        return true;
+      };
+      ok = readItem(cur);
+      if (ok && cur.halves > 0) {
+        for (int t = 0; t < cur.halves && ok; ++t) ok = issueS(cur, t, cur.jb, 0);
+        while (ok && cur.halves > 0) {
+          for (int j = cur.jb; j < cur.je && ok; ++j, ++n) {
+            const bool last = j + 1 == cur.je;
+            if (last) ok = readItem(nxt);
+            const int halves_next = last ? nxt.halves : cur.halves;
+            for (int t = 0; t < 2 && ok; ++t) {
+              if (t < cur.halves) ok = issuePV(cur, t, j, n);
+              if (ok && t < halves_next) ok = last ? issueS(nxt, t, nxt.jb, n + 1) : issueS(cur, t, j + 1, n + 1);
+            }
+          }
+          cur = nxt;
+        }
+      }
+      // Everything issued has completed before TMEM and shared memory go.
+      tcCommitElect(&sm.drained);
+      if (lane == 0) drainBar(&sm.drained, 0);
+      __syncwarp();
+    } else if (warp == 13) {
+      // ---------------- the walk ----------------
+      // The walk.
+      long long pos = begin;
+      int seq = static_cast<int>(sm.found[0]);
+      long long seq_at = sm.found[1];
+      Sequence q{};
+      Line line{};
+      long long head_length = 0;
+      if (begin < end) {
+        q = sequence<kKind>(a, seq);
+        line = lineOf(a, q);
+        head_length = lengthBefore(line, line.tiles);
+      }
+      bool first = true;
+      auto nextItem = [&](Item& it) {
+        for (;;) {
+          if (pos >= end) {
+            it.halves = 0;
+            return;
+          }
+          while (pos >= seq_at + head_length * a.kv_heads) {
+            seq_at += head_length * a.kv_heads;
+            q = sequence<kKind>(a, ++seq);
+            line = lineOf(a, q);
+            head_length = lengthBefore(line, line.tiles);
+          }
+          const int head = static_cast<int>((pos - seq_at) / head_length);
+          const long long head_at = seq_at + head * head_length;
+          const int tile = tileAt(line, pos - head_at);
+          const long long tile_at = head_at + lengthBefore(line, tile);
+          const long long length = tileLength(line, tile);
+          it.lim = tileLimit(a, q, tile);
+          const int blocks = blocksOf(it.lim);
+          it.jb = pos == tile_at ? 0 : cutBlock(pos - tile_at, length, blocks, share);
+          it.je = end >= tile_at + length ? blocks : cutBlock(end - tile_at, length, blocks, share);
+          if (first && lane == 0) {
+            Cut cut{};
+            cut.tile_at = it.jb > 0 && it.jb < blocks ? tile_at : -1;
+            cut.jb = it.jb;
+            cut.blocks = blocks;
+            cut.seq = seq;
+            cut.head = head;
+            cut.tile = tile;
+            cuts[blockIdx.x] = cut;
+          }
+          first = false;
+          pos = tile_at + length;
+          if (it.jb >= it.je) continue;
+          it.seq = seq;
+          it.head = head;
+          it.tile = tile;
+          it.q0 = q.q0;
+          it.nq = q.nq;
+          it.k0 = q.k0;
+          it.nk = q.nk;
+          const long long rows = static_cast<long long>(q.nq) * a.group - static_cast<long long>(tile) * kTileRows;
+          it.halves = rows > kHalf ? 2 : 1;
+          it.part = it.jb == 0 && it.je == blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (it.jb > 0 ? 0 : 1);
+          return;
+        }
+      };
+      if (begin >= end && lane == 0) cuts[blockIdx.x].tile_at = -1;
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const int slot = i % kItems;
+        if (i >= kItems) ok = wait(&sm.item_empty[slot], ((i / kItems) - 1) & 1, sm, err, 51);
+        if (!ok) break;
+        Item it{};
+        nextItem(it);
+        if (lane == 0) {
+          sm.items[slot] = it;
+          mbarArrive(&sm.item_full[slot]);
+        }
+        __syncwarp();
+        if (it.halves == 0) break;
+      }
+    }
+  } else if (warp >= 8) {
+    fewerRegisters<96>();
+    // ---------------- loads ----------------
+    constexpr int kWarpPlanes = kPlanes / kLoadWarps;  // planes of a warp where lanes take rows
+    constexpr int kRowsAtOnce = 32 / kPlanes;          // rows of a warp's copy where lanes take planes
+    constexpr int kRowStep = kLoadWarps * kRowsAtOnce;
+    const int w = warp - 8;
+    const int p_lane = lane % kPlanes;
+    const int r_lane = w * kRowsAtOnce + lane / kPlanes;
+    bool ok = true;
+    int n = 0;             // key blocks so far
+    int used[2] = {0, 0};  // times that Q's halves were loaded
+    for (int i = 0; ok; ++i) {
+      const int slot = i % kItems;
+      ok = wait(&sm.item_full[slot], (i / kItems) & 1, sm, err, 52);
+      if (!ok) break;
+      const Item it = sm.items[slot];
+      __syncwarp();
+      if (lane == 0) mbarArrive(&sm.item_empty[slot]);
+      if (it.halves == 0) break;
+
+      // Pages of a block: lane x holds that of its rows 16 x .. 16 x + 15.
+      auto pagesOf = [&](int j) -> int {
+        if constexpr (kKind == kPacked16) return 0;
+        const int key = j * kKeys + lane * 16;
+        return lane < kKeys / 16 && key < it.lim ? pageOf(a, it.seq, key) : 0;
+      };
+      int page_next = pagesOf(it.jb);
+
+      // Q: rows r = token * group + g, counted from the tile's first token.
+      const long long row0 = static_cast<long long>(it.tile) * kTileRows;
+      const int token0 = static_cast<int>(row0 / a.group);
+      const int rest0 = static_cast<int>(row0 - static_cast<long long>(token0) * a.group);
+      const int rows = static_cast<int>(min(static_cast<long long>(kTileRows), static_cast<long long>(it.nq) * a.group - row0));
+      auto rowOf = [&](int rr, int p) -> const unsigned char* {
+        const int x = rest0 + rr;  // below 256 + 128: the reciprocal's quotient is exact
+        const int tok = (x * a.group_inv) >> 16;
+        return record(a.q, it.head * a.group + x - tok * a.group, static_cast<long long>(it.q0) + token0 + tok, p);
+      };
+      for (int t = 0; t < it.halves && ok; ++t) {
+        if (used[t] > 0) ok = wait(&sm.q_empty[t], (used[t] - 1) & 1, sm, err, 53);
+        if (!ok) break;
+        ++used[t];
+        const uint32_t dst = q_s + t * G::kTileBytes;
+        if (a.q.row_stride == 16) {
+#pragma unroll
+          for (int rr = 0; rr < kHalf; rr += 32) {
+            const bool in = t * kHalf + rr + lane < rows;
+            const unsigned char* src = rowOf(in ? t * kHalf + rr + lane : 0, w * kWarpPlanes);
+#pragma unroll
+            for (int p = 0; p < kWarpPlanes; ++p) {
+              copyAsync16(dst + (w * kWarpPlanes + p) * kPlane + (rr + lane) * 16, src, in);
+              src += a.q.plane_stride;
+            }
+          }
+        } else {
+#pragma unroll 4
+          for (int rr = r_lane; rr < kHalf; rr += kRowStep) {
+            const bool in = t * kHalf + rr < rows;
+            copyAsync16(dst + p_lane * kPlane + rr * 16, rowOf(in ? t * kHalf + rr : 0, p_lane), in);
+          }
+        }
+        copyArrive(&sm.q_full[t]);
+      }
+
+      for (int j = it.jb; j < it.je && ok; ++j, ++n) {
+        const int page = page_next;
+        if (j + 1 < it.je) page_next = pagesOf(j + 1);
+        if (kKind != kPacked16 && page < 0) reportIndex(err, FPK_ERROR_PAGE);
+        const int lim = it.lim - j * kKeys;  // rows of the block that somebody sees
+        // Paged: offsets of this lane's four rows, the same in keys and values.
+        long long off[4];
+        bool in[4];
+        if constexpr (kKind != kPacked16) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int rr = c * 32 + lane;
+            const int pg = __shfl_sync(0xffffffffu, page, rr >> 4);
+            in[c] = rr < lim && pg >= 0;
+            off[c] = in[c] ? it.head * a.k.head_stride + pg * a.page_stride + ((j * kKeys + rr) & ((1 << a.page_shift) - 1)) * 16LL : 0;
+          }
+        }
+        for (int side = 0; side < 2 && ok; ++side) {
+          const int stage = (n & 1) * 2 + side;
+          const uint32_t dst = kv_s + stage * G::kTileBytes;
+          const fpk_heads_t& v = side == 0 ? a.k : a.v;
+          const unsigned char* data = static_cast<const unsigned char*>(v.data);
+          if constexpr (kKind == kPagedE4m3) {
+            // Records in flight before there is room for them.
+            constexpr int kWarpRecords = kPlanes / 2 / kLoadWarps;  // of a row: 2 or 1
+            const float* scales = side == 0 ? a.k_scale : a.v_scale;
+            uint4 codes[4][kWarpRecords];
+            float sc[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int rr = c * 32 + lane;
+              const int pg = __shfl_sync(0xffffffffu, page, rr >> 4);
+              sc[c] = in[c] ? __ldg(scales + (((static_cast<long long>(pg) * a.kv_heads + it.head) << a.page_shift) +
+                                              ((j * kKeys + rr) & ((1 << a.page_shift) - 1))))
+                            : 0.0f;
+#pragma unroll
+              for (int p = 0; p < kWarpRecords; ++p) {
+                codes[c][p] = in[c] ? __ldg(reinterpret_cast<const uint4*>(data + off[c] + (w * kWarpRecords + p) * v.plane_stride))
+                                    : make_uint4(0, 0, 0, 0);
+              }
+            }
+            if (n >= 2) ok = wait(&sm.kv_empty[stage], ((n >> 1) - 1) & 1, sm, err, 54);
+            if (!ok) break;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+#pragma unroll
+              for (int p = 0; p < kWarpRecords; ++p) {
+                uint4 out[2];
+                dequantise16<T>(codes[c][p], sc[c], out);
+                const uint32_t at = dst + 2 * (w * kWarpRecords + p) * kPlane + (c * 32 + lane) * 16;
+                storeShared16(at, out[0]);
+                storeShared16(at + kPlane, out[1]);
+              }
+            }
+            mbarArrive(&sm.kv_full[stage]);
+          } else {
+            if (n >= 2) ok = wait(&sm.kv_empty[stage], ((n >> 1) - 1) & 1, sm, err, 54);
+            if (!ok) break;
+            if (kKind == kPaged16 || v.row_stride == 16) {
+              const uint32_t to = dst + w * kWarpPlanes * kPlane + lane * 16;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                bool yes;
+                const unsigned char* src;
+                if constexpr (kKind == kPaged16) {
+                  yes = in[c];
+                  src = data + off[c] + w * kWarpPlanes * v.plane_stride;
+                } else {
+                  yes = c * 32 + lane < lim;
+                  src = yes ? record(v, it.head, static_cast<long long>(it.k0) + j * kKeys + c * 32 + lane, w * kWarpPlanes) : data;
+                }
+#pragma unroll
+                for (int p = 0; p < kWarpPlanes; ++p) {
+                  copyAsync16(to + p * kPlane + c * 512, src, yes);
+                  if (yes) src += v.plane_stride;
+                }
+              }
+            } else {
+              const long long step = kRowStep * v.row_stride;
+              const unsigned char* src = record(v, it.head, static_cast<long long>(it.k0) + j * kKeys + r_lane, p_lane);
+              const uint32_t to = dst + p_lane * kPlane + r_lane * 16;
+#pragma unroll
+              for (int x = 0; x < kKeys / kRowStep; ++x) {
+                const bool yes = r_lane + x * kRowStep < lim;
+                copyAsync16(to + x * kRowStep * 16, yes ? src : data, yes);
+                src += step;
+              }
+            }
+            copyArrive(&sm.kv_full[stage]);
+          }
+        }
+      }
+    }
+    copyDrain();
+  } else {
+    moreRegisters<168>();
+    // ---------------- softmax and output ----------------
+    const int t = warp >> 2;
+    const int rr = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_base = lane_base + t * kKeys;
+    const uint32_t o_base = lane_base + kOCol + t * D;
+    bool ok = true;
+    int count = 0;  // blocks of this half
+    for (int i = 0; ok; ++i) {
+      const int slot = i % kItems;
+      ok = wait(&sm.item_full[slot], (i / kItems) & 1, sm, err, 55);
+      if (!ok) break;
+      const Item it = sm.items[slot];
+      __syncwarp();
+      if (lane == 0) mbarArrive(&sm.item_empty[slot]);
+      if (it.halves == 0) break;
+      if (t >= it.halves) continue;
+      const Sequence q{it.q0, it.nq, it.k0, it.nk};
+      const long long rows = static_cast<long long>(it.nq) * a.group;
+      const long long row_first = static_cast<long long>(it.tile) * kTileRows + t * kHalf;
+      const long long r = row_first + rr;
+      const bool valid = r < rows;
+      const int token = valid ? static_cast<int>(r / a.group) : 0;
+      const int vis = valid ? visible(a, q, token) : it.nk;
+      const int min_vis = visible(a, q, static_cast<int>(row_first / a.group));
+      float m = -INFINITY, l = 0.0f;
+      int page_next = 0;
+      auto pagesOf = [&](int j) -> int {
+        if constexpr (kKind == kPacked16) return 0;
+        const int key = j * kKeys + lane * 16;
+        return lane < kKeys / 16 && key < it.lim ? pageOf(a, it.seq, key) : 0;
+      };
+      page_next = pagesOf(it.jb);
+      for (int j = it.jb; j < it.je && ok; ++j, ++count) {
+        const uint32_t bad = kKind == kPacked16 ? 0u : __ballot_sync(0xffffffffu, page_next < 0);
+        if (j + 1 < it.je) page_next = pagesOf(j + 1);
+        ok = wait(&sm.s_full[t], count & 1, sm, err, 58);
+        if (!ok) break;
+        tcFenceAfter();
+        // The maximum over both halves of the row, the second of which stays in
+        // registers; the first is read again once the maximum is known.
+        const bool edge = (j + 1) * kKeys > min_vis || bad != 0;  // the causal edge, the last keys, bad pages
+        const int lim = vis - j * kKeys;
+        uint32_t sv[64];
+        auto load = [&](int c) {
+          FPB_TMEM_LD32(s_base + 64 * c, sv);
+          FPB_TMEM_LD32(s_base + 64 * c + 32, (sv + 32));
+          tmemWaitLd();
+          if (edge) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) {
+              if (64 * c + e >= lim || ((bad >> (4 * c + (e >> 4))) & 1u) != 0) sv[e] = __float_as_uint(-INFINITY);
+            }
+          }
+        };
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          load(c);
+#pragma unroll
+          for (int e = 0; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sv[e]));
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+        if (j == it.jb) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, top > m + kGrowLog2)) {
+          const float m_new = top > m + kGrowLog2 ? top : m;
+          const float f = m_new == m ? 1.0f : exp2Approx(m - m_new);
+          ok = wait(&sm.pv_done[t], (count - 1) & 1, sm, err, 59);
+          if (!ok) break;
+          tcFenceAfter();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t ov[32];
+            FPB_TMEM_LD32(o_base + c, ov);
+            tmemWaitLd();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * f);
+            FPB_TMEM_ST32(o_base + c, ov);
+          }
+          tmemStoreWait();
+          l *= f;
+          m = m_new;
+        }
+        // P over the second half's columns: keys 64 .. 127 go to the last 32,
+        // keys 0 .. 63 to the 32 before.
+        const float neg = m == -INFINITY ? 0.0f : -m;  // a row that has seen no key yet
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 1; c >= 0; --c) {
+          if (c == 0) load(0);
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float p0 = exp2Approx(fmaf(__uint_as_float(sv[2 * e]), a.scale_log2, neg));
+            const float p1 = exp2Approx(fmaf(__uint_as_float(sv[2 * e + 1]), a.scale_log2, neg));
+            part[(e & 1) * 2] += p0;
+            part[(e & 1) * 2 + 1] += p1;
+            pk[e] = pack2<T>(p0, p1);
+          }
+          FPB_TMEM_ST32(s_base + kPCol + 32 * c, pk);
+        }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
+        tmemStoreWait();
+        tcFenceBefore();
+        __syncwarp();
+        if (lane == 0) mbarArrive(&sm.p_full[t]);
+      }
+      if (ok) ok = wait(&sm.pv_done[t], (count - 1) & 1, sm, err, 59);
+      if (!ok) break;
+      tcFenceAfter();
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int h = it.head * a.group + (valid ? static_cast<int>(r - static_cast<long long>(token) * a.group) : 0);
+      float* part_at = it.part >= 0 ? partials + static_cast<size_t>(it.part) * partialFloats(D) : nullptr;
+      const int tile_row = t * kHalf + rr;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t ov[32];
+        FPB_TMEM_LD32(o_base + c, ov);
+        tmemWaitLd();
+        if (!valid) continue;
+        if (part_at == nullptr) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(ov[g * 8 + e]) * inv;
+            // A row that saw no key: whatever V held, the sum is empty.
+            if (l == 0.0f) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+            }
+            *reinterpret_cast<uint4*>(record(a.out, h, it.q0 + token, (c >> 3) + g)) = pack8<T>(x);
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            reinterpret_cast<uint4*>(part_at)[((c >> 2) + g) * kTileRows + tile_row] =
+                make_uint4(ov[4 * g], ov[4 * g + 1], ov[4 * g + 2], ov[4 * g + 3]);
+          }
+        }
+      }
+      if (part_at != nullptr && valid) {
+        part_at[kTileRows * D + tile_row] = m;
+        part_at[kTileRows * D + kTileRows + tile_row] = l;
+      }
+      tcFenceBefore();
+      __syncwarp();
+      if (lane == 0) mbarArrive(&sm.o_free[t]);
+    }
+  }
+  tcFenceBefore();
+  __syncthreads();
+  if (warp == 12) {
+    tcFenceAfter();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+// Joins the pieces of a tile: CTA c looks after the tile that share c begins
+// inside, if it is the first share to. A thread joins 8 channels of a row.
+template <typename T, int D, KvKind kKind>
+__global__ void __launch_bounds__(kTileRows) joinTilesKernel(const Args a, int n_cta) {
+  tc::pdlTrigger();
+  tc::pdlWait();
+  const Cut* cuts = reinterpret_cast<const Cut*>(a.workspace);
+  const float* partials = reinterpret_cast<const float*>(a.workspace + sizeof(Cut) * kTileCtas);
+  const int c = blockIdx.x;
+  const Cut cut = cuts[c];
+  if (cut.tile_at < 0 || (c > 0 && cuts[c - 1].tile_at == cut.tile_at)) return;
+  const Sequence q = sequence<kKind>(a, cut.seq);
+  const int row = threadIdx.x, grp = blockIdx.y;
+  const long long r = static_cast<long long>(cut.tile) * kTileRows + row;
+  if (r >= static_cast<long long>(q.nq) * a.group) return;
+  // The first piece is the last of CTA c - 1, the others are first pieces.
+  float m = -INFINITY, l = 0.0f, x[8] = {};
+  auto add = [&](int part) {
+    const float* p = partials + static_cast<size_t>(part) * partialFloats(D);
+    const float pm = p[kTileRows * D + row], pl = p[kTileRows * D + kTileRows + row];
+    const float4 u = reinterpret_cast<const float4*>(p)[(2 * grp) * kTileRows + row];
+    const float4 v = reinterpret_cast<const float4*>(p)[(2 * grp + 1) * kTileRows + row];
+    const float m_new = fmaxf(m, pm);
+    const float f = m == m_new ? 1.0f : exp2Approx(m - m_new), g = pm == m_new ? 1.0f : exp2Approx(pm - m_new);
+    m = m_new;
+    l = l * f + pl * g;
+    const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * f + y[e] * g;
+  };
+  add(2 * (c - 1) + 1);
+  int from = cut.jb;
+  for (int d = c; d < n_cta; ++d) {
+    const Cut next = d + 1 < n_cta ? cuts[d + 1] : Cut{-1, 0, 0, 0, 0, 0, 0};
+    const bool more = next.tile_at == cut.tile_at;
+    const int to = more ? next.jb : cut.blocks;
+    if (to > from) add(2 * d);
+    from = to;
+    if (!more) break;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = l == 0.0f ? 0.0f : x[e] * inv;
+  const int token = static_cast<int>(r / a.group);
+  const int h = cut.head * a.group + static_cast<int>(r - static_cast<long long>(token) * a.group);
+  *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(x);
+}
+
+long long tilesWorkspaceBytes(int head_dim) {
+  return static_cast<long long>(sizeof(Cut) * kTileCtas + 2 * kTileCtas * partialFloats(head_dim) * sizeof(float));
+}
+
+namespace {
+
+template <typename T, int D, KvKind kKind>
+cudaError_t launchOne(const Args& a, cudaStream_t s) {
+  static DeviceOnce smem_attr;
+  static DeviceValue sms;
+  cudaError_t e = smem_attr.run([] {
+    return cudaFuncSetAttribute(attentionTilesKernel<T, D, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Geo<D>::kSmem));
+  });
+  if (e != cudaSuccess) return e;
+  const int ctas = sms.get([](int dev) {
+    int n = kTileCtas;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return std::min(n, kTileCtas);
+  });
+  prof::countLaunch(prof::kAttention, 2);
+  e = launchPdl(attentionTilesKernel<T, D, kKind>, dim3(ctas), dim3(kThreads), Geo<D>::kSmem, s, a);
+  if (e != cudaSuccess) return e;
+  return launchPdl(joinTilesKernel<T, D, kKind>, dim3(ctas, D / 8), dim3(kTileRows), 0, s, a, ctas);
+}
+
+template <typename T, int D>
+cudaError_t launchKind(const Args& a, KvKind kind, cudaStream_t s) {
+  switch (kind) {
+    case kPacked16: return launchOne<T, D, kPacked16>(a, s);
+    case kPaged16: return launchOne<T, D, kPaged16>(a, s);
+    default: return launchOne<T, D, kPagedE4m3>(a, s);
+  }
+}
+
+}  // namespace
+
+cudaError_t launchTiles(const Args& a, KvKind kind, int head_dim, int dtype, cudaStream_t s) {
+  if (dtype == FPK_DTYPE_BF16) {
+    return head_dim == 64 ? launchKind<__nv_bfloat16, 64>(a, kind, s) : launchKind<__nv_bfloat16, 128>(a, kind, s);
+  }
+  return head_dim == 64 ? launchKind<__half, 64>(a, kind, s) : launchKind<__half, 128>(a, kind, s);
+}
+
+}  // namespace seqattn
+}  // namespace fpb

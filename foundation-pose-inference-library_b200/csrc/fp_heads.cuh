@@ -11,6 +11,7 @@
 
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "fpk.h"
 
@@ -70,6 +71,34 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 __device__ __forceinline__ uint32_t e4m3x2ToHalf2(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
   return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+}
+
+template <typename T>
+__device__ __forceinline__ float largest() {
+  return std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
+}
+
+// One 16-byte e4m3 record as two groups of 8 elements of T.
+template <typename T>
+__device__ __forceinline__ void dequantise16(const uint4& codes, float scale, uint4 (&out)[2]) {
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t h = e4m3x2ToHalf2(w[half * 2 + (i >> 1)] >> ((i & 1) * 16));
+      const float2 f = unpack2<__half>(h);
+      x[2 * i] = f.x * scale;
+      x[2 * i + 1] = f.y * scale;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // NaN passes (both comparisons are false).
+      x[i] = x[i] > largest<T>() ? largest<T>() : (x[i] < -largest<T>() ? -largest<T>() : x[i]);
+    }
+    out[half] = pack8<T>(x);
+  }
 }
 
 __device__ __forceinline__ void reportIndex(int* error_flag, int code) {

@@ -95,34 +95,6 @@ __device__ __forceinline__ int slotOf(const Args& a, int row) {
   return slot;
 }
 
-template <typename T>
-__device__ __forceinline__ float largest() {
-  return std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
-}
-
-// One 16-byte e4m3 record as two groups of 8 elements of T.
-template <typename T>
-__device__ __forceinline__ void dequantise16(const uint4& codes, float scale, uint4 (&out)[2]) {
-  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t h = e4m3x2ToHalf2(w[half * 2 + (i >> 1)] >> ((i & 1) * 16));
-      const float2 f = unpack2<__half>(h);
-      x[2 * i] = f.x * scale;
-      x[2 * i + 1] = f.y * scale;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // NaN passes (both comparisons are false).
-      x[i] = x[i] > largest<T>() ? largest<T>() : (x[i] < -largest<T>() ? -largest<T>() : x[i]);
-    }
-    out[half] = pack8<T>(x);
-  }
-}
-
 constexpr int kThreads = 256;
 
 // Row-major rows: kGroups lanes per (row, keys or values, head).
