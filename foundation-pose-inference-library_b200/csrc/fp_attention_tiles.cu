@@ -63,6 +63,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
 constexpr uint32_t kPCol = 64;   // P among a half's 128 score columns
 constexpr float kGrowLog2 = 8.0f;
+constexpr int kTileCost = 384;   // a tile's work beside its keys, in keys
 constexpr int kMinShare = 256;   // keys
 constexpr int kSnap = 8;         // a tile shorter than 1/8 share is not cut
 
@@ -108,36 +109,36 @@ constexpr size_t partialFloats(int d) { return static_cast<size_t>(kTileRows) * 
 
 // ---- the line of work ----
 
-// Tile i of a sequence and head is long w(i): 1 + the keys that its last full
-// token row sees (causal: growing by the tokens of a tile), in closed form.
+// Tile i of a sequence and head is long w(i): the keys that its last full token
+// row sees (causal: growing by the tokens of a tile) and kTileCost for what a
+// tile costs beside its keys, in closed form.
 struct Line {
   int tiles;
-  int first, step;  // w(i) = 1 + clamp(first + i * step, 0, nk)
+  int first, step;  // w(i) = kTileCost + clamp(first + i * step, 0, nk)
   int nk;
+  int k0, k1;       // the clamp is 0 below tile k0, nk from tile k1 on
 };
 
 __device__ __forceinline__ Line lineOf(const Args& a, const Sequence& q) {
   Line n;
-  n.tiles = static_cast<int>((static_cast<long long>(q.nq) * a.group + kTileRows - 1) / kTileRows);
+  n.tiles = (q.nq * a.group + kTileRows - 1) / kTileRows;  // below 2^31: checked by the host
   n.nk = q.nk;
   n.step = a.causal ? max(kTileRows / a.group, 1) : 0;
   n.first = a.causal ? q.nk - q.nq + n.step : q.nk;
+  n.k0 = n.first >= 0 ? 0 : (-n.first + n.step - 1) / n.step;
+  n.k1 = n.first >= n.nk ? 0 : (n.nk - n.first + n.step - 1) / n.step;
   return n;
 }
 
-__device__ __forceinline__ long long tileLength(const Line& n, int i) {
-  return 1 + min(max(n.first + static_cast<long long>(i) * n.step, 0LL), static_cast<long long>(n.nk));
+__device__ __forceinline__ int tileLength(const Line& n, int i) {
+  return kTileCost + (i < n.k0 ? 0 : i >= n.k1 ? n.nk : n.first + i * n.step);
 }
 
 // Sum of tileLength over tiles 0 .. i-1.
 __device__ __forceinline__ long long lengthBefore(const Line& n, int i) {
-  if (n.step == 0) return i * tileLength(n, 0);
-  // first + k*step >= 0 from k0 on, >= nk from k1 on.
-  const long long k0 = n.first >= 0 ? 0 : (-static_cast<long long>(n.first) + n.step - 1) / n.step;
-  const long long k1 = n.first >= n.nk ? 0 : (static_cast<long long>(n.nk) - n.first + n.step - 1) / n.step;
-  const long long lo = min(k0, static_cast<long long>(i)), hi = min(max(k1, k0), static_cast<long long>(i));
+  const long long lo = min(n.k0, i), hi = min(max(n.k1, n.k0), i);
   const long long ramp = hi - lo;
-  return i + ramp * n.first + n.step * ((lo + hi - 1) * ramp / 2) + (i - hi) * static_cast<long long>(n.nk);
+  return static_cast<long long>(i) * kTileCost + ramp * n.first + n.step * ((lo + hi - 1) * ramp / 2) + (i - hi) * n.nk;
 }
 
 // The tile that holds place x of a head's line.
@@ -154,8 +155,7 @@ __device__ __forceinline__ int blocksOf(int lim) { return max((lim + kKeys - 1) 
 
 // Keys that a tile sees: those of its last row.
 __device__ __forceinline__ int tileLimit(const Args& a, const Sequence& q, int tile) {
-  const long long last = min(static_cast<long long>(q.nq) * a.group, (tile + 1LL) * kTileRows) - 1;
-  return visible(a, q, static_cast<int>(last / a.group));
+  return visible(a, q, (min(q.nq * a.group, (tile + 1) * kTileRows) - 1) / a.group);
 }
 
 // Key block at which place y of a tile of length w cuts it.
@@ -294,9 +294,9 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) total += scan(s0);
   // Shares of kMinShare keys or more: none is empty, and a tile's cuts differ.
   const long long n_cta = max(1LL, min(static_cast<long long>(gridDim.x), total / kMinShare));
-  const long long begin = min(static_cast<long long>(blockIdx.x), n_cta) * total / n_cta;
-  const long long end = min(blockIdx.x + 1LL, n_cta) * total / n_cta;
-  const long long share = total / n_cta;
+  const long long share = total / n_cta, rest = total - share * n_cta;
+  auto shareBegin = [&](long long c) { return c >= n_cta ? total : c * share + min(c, rest); };
+  const long long begin = shareBegin(blockIdx.x), end = shareBegin(blockIdx.x + 1LL);
   if (begin < end) {
     long long before = 0;
     for (int s0 = 0; s0 < a.n_seq && before <= begin; s0 += kThreads) {
@@ -402,43 +402,48 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       __syncwarp();
     } else if (warp == 13) {
       // ---------------- the walk ----------------
-      // The walk.
-      long long pos = begin;
-      int seq = static_cast<int>(sm.found[0]);
-      long long seq_at = sm.found[1];
+      int seq = static_cast<int>(sm.found[0]), head = 0, tile = 0;
+      long long at = end;  // of the tile; a CTA without a share is at its end already
       Sequence q{};
       Line line{};
-      long long head_length = 0;
       if (begin < end) {
         q = sequence<kKind>(a, seq);
         line = lineOf(a, q);
-        head_length = lengthBefore(line, line.tiles);
+        const long long head_length = lengthBefore(line, line.tiles);
+        const long long inside = begin - sm.found[1];
+        head = static_cast<int>(inside / head_length);
+        tile = tileAt(line, inside - head * head_length);
+        at = sm.found[1] + head * head_length + lengthBefore(line, tile);
+      } else if (lane == 0) {
+        cuts[blockIdx.x].tile_at = -1;
       }
       bool first = true;
       auto nextItem = [&](Item& it) {
-        for (;;) {
-          if (pos >= end) {
-            it.halves = 0;
-            return;
+        it.halves = 0;
+        while (it.halves == 0) {
+          if (!first) {
+            at += tileLength(line, tile);
+            ++tile;
           }
-          while (pos >= seq_at + head_length * a.kv_heads) {
-            seq_at += head_length * a.kv_heads;
-            q = sequence<kKind>(a, ++seq);
-            line = lineOf(a, q);
-            head_length = lengthBefore(line, line.tiles);
+          if (at >= end) return;
+          if (tile >= line.tiles) {
+            tile = 0;
+            if (++head >= a.kv_heads) {
+              head = 0;
+              do {  // at < end: a sequence with rows follows
+                q = sequence<kKind>(a, ++seq);
+                line = lineOf(a, q);
+              } while (line.tiles == 0);
+            }
           }
-          const int head = static_cast<int>((pos - seq_at) / head_length);
-          const long long head_at = seq_at + head * head_length;
-          const int tile = tileAt(line, pos - head_at);
-          const long long tile_at = head_at + lengthBefore(line, tile);
-          const long long length = tileLength(line, tile);
+          const int length = tileLength(line, tile);
           it.lim = tileLimit(a, q, tile);
           const int blocks = blocksOf(it.lim);
-          it.jb = pos == tile_at ? 0 : cutBlock(pos - tile_at, length, blocks, share);
-          it.je = end >= tile_at + length ? blocks : cutBlock(end - tile_at, length, blocks, share);
+          it.jb = begin <= at ? 0 : cutBlock(begin - at, length, blocks, share);
+          it.je = end >= at + length ? blocks : cutBlock(end - at, length, blocks, share);
           if (first && lane == 0) {
             Cut cut{};
-            cut.tile_at = it.jb > 0 && it.jb < blocks ? tile_at : -1;
+            cut.tile_at = it.jb > 0 && it.jb < blocks ? at : -1;
             cut.jb = it.jb;
             cut.blocks = blocks;
             cut.seq = seq;
@@ -447,7 +452,6 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             cuts[blockIdx.x] = cut;
           }
           first = false;
-          pos = tile_at + length;
           if (it.jb >= it.je) continue;
           it.seq = seq;
           it.head = head;
@@ -456,13 +460,10 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           it.nq = q.nq;
           it.k0 = q.k0;
           it.nk = q.nk;
-          const long long rows = static_cast<long long>(q.nq) * a.group - static_cast<long long>(tile) * kTileRows;
-          it.halves = rows > kHalf ? 2 : 1;
+          it.halves = q.nq * a.group - tile * kTileRows > kHalf ? 2 : 1;
           it.part = it.jb == 0 && it.je == blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (it.jb > 0 ? 0 : 1);
-          return;
         }
       };
-      if (begin >= end && lane == 0) cuts[blockIdx.x].tile_at = -1;
       bool ok = true;
       for (int i = 0; ok; ++i) {
         const int slot = i % kItems;
@@ -508,40 +509,42 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       int page_next = pagesOf(it.jb);
 
       // Q: rows r = token * group + g, counted from the tile's first token.
-      const long long row0 = static_cast<long long>(it.tile) * kTileRows;
-      const int token0 = static_cast<int>(row0 / a.group);
-      const int rest0 = static_cast<int>(row0 - static_cast<long long>(token0) * a.group);
-      const int rows = static_cast<int>(min(static_cast<long long>(kTileRows), static_cast<long long>(it.nq) * a.group - row0));
+      const int row0 = it.tile * kTileRows;
+      const int token0 = row0 / a.group;
+      const int rest0 = row0 - token0 * a.group;
+      const int rows = min(kTileRows, it.nq * a.group - row0);
       auto rowOf = [&](int rr, int p) -> const unsigned char* {
         const int x = rest0 + rr;  // below 256 + 128: the reciprocal's quotient is exact
         const int tok = (x * a.group_inv) >> 16;
         return record(a.q, it.head * a.group + x - tok * a.group, static_cast<long long>(it.q0) + token0 + tok, p);
       };
-      for (int t = 0; t < it.halves && ok; ++t) {
-        if (used[t] > 0) ok = wait(&sm.q_empty[t], (used[t] - 1) & 1, sm, err, 53);
-        if (!ok) break;
-        ++used[t];
-        const uint32_t dst = q_s + t * G::kTileBytes;
-        if (a.q.row_stride == 16) {
-#pragma unroll
-          for (int rr = 0; rr < kHalf; rr += 32) {
-            const bool in = t * kHalf + rr + lane < rows;
-            const unsigned char* src = rowOf(in ? t * kHalf + rr + lane : 0, w * kWarpPlanes);
-#pragma unroll
-            for (int p = 0; p < kWarpPlanes; ++p) {
-              copyAsync16(dst + (w * kWarpPlanes + p) * kPlane + (rr + lane) * 16, src, in);
-              src += a.q.plane_stride;
+      auto loadQ = [&]() {
+        for (int t = 0; t < it.halves && ok; ++t) {
+          if (used[t] > 0) ok = wait(&sm.q_empty[t], (used[t] - 1) & 1, sm, err, 53);
+          if (!ok) break;
+          ++used[t];
+          const uint32_t dst = q_s + t * G::kTileBytes;
+          if (a.q.row_stride == 16) {
+  #pragma unroll
+            for (int rr = 0; rr < kHalf; rr += 32) {
+              const bool in = t * kHalf + rr + lane < rows;
+              const unsigned char* src = rowOf(in ? t * kHalf + rr + lane : 0, w * kWarpPlanes);
+  #pragma unroll
+              for (int p = 0; p < kWarpPlanes; ++p) {
+                copyAsync16(dst + (w * kWarpPlanes + p) * kPlane + (rr + lane) * 16, src, in);
+                src += a.q.plane_stride;
+              }
+            }
+          } else {
+  #pragma unroll 4
+            for (int rr = r_lane; rr < kHalf; rr += kRowStep) {
+              const bool in = t * kHalf + rr < rows;
+              copyAsync16(dst + p_lane * kPlane + rr * 16, rowOf(in ? t * kHalf + rr : 0, p_lane), in);
             }
           }
-        } else {
-#pragma unroll 4
-          for (int rr = r_lane; rr < kHalf; rr += kRowStep) {
-            const bool in = t * kHalf + rr < rows;
-            copyAsync16(dst + p_lane * kPlane + rr * 16, rowOf(in ? t * kHalf + rr : 0, p_lane), in);
-          }
+          copyArrive(&sm.q_full[t]);
         }
-        copyArrive(&sm.q_full[t]);
-      }
+      };
 
       for (int j = it.jb; j < it.je && ok; ++j, ++n) {
         const int page = page_next;
@@ -561,6 +564,9 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           }
         }
         for (int side = 0; side < 2 && ok; ++side) {
+          // Q after the first keys: its room is free only after the last tile's last scores.
+          if (side == 1 && j == it.jb) loadQ();
+          if (!ok) break;
           const int stage = (n & 1) * 2 + side;
           const uint32_t dst = kv_s + stage * G::kTileBytes;
           const fpk_heads_t& v = side == 0 ? a.k : a.v;
@@ -657,13 +663,12 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       if (it.halves == 0) break;
       if (t >= it.halves) continue;
       const Sequence q{it.q0, it.nq, it.k0, it.nk};
-      const long long rows = static_cast<long long>(it.nq) * a.group;
-      const long long row_first = static_cast<long long>(it.tile) * kTileRows + t * kHalf;
-      const long long r = row_first + rr;
-      const bool valid = r < rows;
-      const int token = valid ? static_cast<int>(r / a.group) : 0;
+      const int row_first = it.tile * kTileRows + t * kHalf;
+      const int r = row_first + rr;
+      const bool valid = r < it.nq * a.group;
+      const int token = valid ? r / a.group : 0;
       const int vis = valid ? visible(a, q, token) : it.nk;
-      const int min_vis = visible(a, q, static_cast<int>(row_first / a.group));
+      const int min_vis = visible(a, q, row_first / a.group);
       float m = -INFINITY, l = 0.0f;
       int page_next = 0;
       auto pagesOf = [&](int j) -> int {
@@ -690,7 +695,13 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           if (edge) {
 #pragma unroll
             for (int e = 0; e < 64; ++e) {
-              if (64 * c + e >= lim || ((bad >> (4 * c + (e >> 4))) & 1u) != 0) sv[e] = __float_as_uint(-INFINITY);
+              if (64 * c + e >= lim) sv[e] = __float_as_uint(-INFINITY);
+            }
+            if (bad != 0) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e) {
+                if (((bad >> (4 * c + (e >> 4))) & 1u) != 0) sv[e] = __float_as_uint(-INFINITY);
+              }
             }
           }
         };
@@ -751,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       if (!ok) break;
       tcFenceAfter();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int h = it.head * a.group + (valid ? static_cast<int>(r - static_cast<long long>(token) * a.group) : 0);
+      const int h = it.head * a.group + (valid ? r - token * a.group : 0);
       float* part_at = it.part >= 0 ? partials + static_cast<size_t>(it.part) * partialFloats(D) : nullptr;
       const int tile_row = t * kHalf + rr;
 #pragma unroll 1
@@ -810,40 +821,41 @@ __global__ void __launch_bounds__(kTileRows) joinTilesKernel(const Args a, int n
   const Cut cut = cuts[c];
   if (cut.tile_at < 0 || (c > 0 && cuts[c - 1].tile_at == cut.tile_at)) return;
   const Sequence q = sequence<kKind>(a, cut.seq);
-  const int row = threadIdx.x, grp = blockIdx.y;
-  const long long r = static_cast<long long>(cut.tile) * kTileRows + row;
-  if (r >= static_cast<long long>(q.nq) * a.group) return;
-  // The first piece is the last of CTA c - 1, the others are first pieces.
-  float m = -INFINITY, l = 0.0f, x[8] = {};
-  auto add = [&](int part) {
-    const float* p = partials + static_cast<size_t>(part) * partialFloats(D);
-    const float pm = p[kTileRows * D + row], pl = p[kTileRows * D + kTileRows + row];
-    const float4 u = reinterpret_cast<const float4*>(p)[(2 * grp) * kTileRows + row];
-    const float4 v = reinterpret_cast<const float4*>(p)[(2 * grp + 1) * kTileRows + row];
-    const float m_new = fmaxf(m, pm);
-    const float f = m == m_new ? 1.0f : exp2Approx(m - m_new), g = pm == m_new ? 1.0f : exp2Approx(pm - m_new);
-    m = m_new;
-    l = l * f + pl * g;
-    const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+  const int row = threadIdx.x;
+  const int r = cut.tile * kTileRows + row;
+  if (r >= q.nq * a.group) return;
+  const int token = r / a.group;
+  const int h = cut.head * a.group + r - token * a.group;
+  for (int grp = blockIdx.y; grp < D / 8; grp += gridDim.y) {
+    // The first piece is the last of CTA c - 1, the others are first pieces.
+    float m = -INFINITY, l = 0.0f, x[8] = {};
+    auto add = [&](int part) {
+      const float* p = partials + static_cast<size_t>(part) * partialFloats(D);
+      const float pm = p[kTileRows * D + row], pl = p[kTileRows * D + kTileRows + row];
+      const float4 u = reinterpret_cast<const float4*>(p)[(2 * grp) * kTileRows + row];
+      const float4 v = reinterpret_cast<const float4*>(p)[(2 * grp + 1) * kTileRows + row];
+      const float m_new = fmaxf(m, pm);
+      const float f = m == m_new ? 1.0f : exp2Approx(m - m_new), g = pm == m_new ? 1.0f : exp2Approx(pm - m_new);
+      m = m_new;
+      l = l * f + pl * g;
+      const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = x[e] * f + y[e] * g;
-  };
-  add(2 * (c - 1) + 1);
-  int from = cut.jb;
-  for (int d = c; d < n_cta; ++d) {
-    const Cut next = d + 1 < n_cta ? cuts[d + 1] : Cut{-1, 0, 0, 0, 0, 0, 0};
-    const bool more = next.tile_at == cut.tile_at;
-    const int to = more ? next.jb : cut.blocks;
-    if (to > from) add(2 * d);
-    from = to;
-    if (!more) break;
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * f + y[e] * g;
+    };
+    add(2 * (c - 1) + 1);
+    int from = cut.jb;
+    for (int d = c; d < n_cta; ++d) {
+      const bool more = d + 1 < n_cta && cuts[d + 1].tile_at == cut.tile_at;
+      const int to = more ? cuts[d + 1].jb : cut.blocks;
+      if (to > from) add(2 * d);
+      from = to;
+      if (!more) break;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = l == 0.0f ? 0.0f : x[e] * inv;
+    *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(x);
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = l == 0.0f ? 0.0f : x[e] * inv;
-  const int token = static_cast<int>(r / a.group);
-  const int h = cut.head * a.group + static_cast<int>(r - static_cast<long long>(token) * a.group);
-  *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(x);
 }
 
 long long tilesWorkspaceBytes(int head_dim) {
@@ -868,7 +880,10 @@ cudaError_t launchOne(const Args& a, cudaStream_t s) {
   prof::countLaunch(prof::kAttention, 2);
   e = launchPdl(attentionTilesKernel<T, D, kKind>, dim3(ctas), dim3(kThreads), Geo<D>::kSmem, s, a);
   if (e != cudaSuccess) return e;
-  return launchPdl(joinTilesKernel<T, D, kKind>, dim3(ctas, D / 8), dim3(kTileRows), 0, s, a, ctas);
+  // Many tiles are cut into two or three pieces each, few into many: those
+  // are joined by more CTAs.
+  const long long tiles = (static_cast<long long>(a.q_rows) * a.group / kTileRows + 1) * a.kv_heads;
+  return launchPdl(joinTilesKernel<T, D, kKind>, dim3(ctas, tiles >= ctas ? 2 : D / 8), dim3(kTileRows), 0, s, a, ctas);
 }
 
 template <typename T, int D>
