@@ -14,21 +14,21 @@
 //                   fp32, P = 2^(s - m) rounded to the element type over the
 //                   scores' own TMEM columns. O is rescaled only when a row's
 //                   maximum grows by more than 2^8. After the last block, O / l.
-//   warps 8-11      loads: Q, K and V records into no-swizzle core-matrix
-//                   tiles [group of 8 channels][row][16 B], K and V in four
-//                   stages of 128 rows. 16-bit rows by cp.async, which takes any
-//                   strides, pages that end inside a block and zero fill of
-//                   keys that nobody sees, and arrives on the stage's barrier by
-//                   itself; e4m3 rows through registers, where they become the
-//                   element type (exact in bf16). A group's rows are padded by
-//                   16 bytes so that row-major sources write without bank
-//                   conflicts.
+//   warps 8-11      loads: Q, K and V rows into 128-byte swizzled tiles of 64
+//                   channels [row][64], which lanes that take rows (planar
+//                   sources, pages) and lanes that take groups of channels
+//                   (row-major sources) both fill without bank conflicts; K and
+//                   V in four stages of 128 rows. 16-bit rows by cp.async, which
+//                   takes any strides, pages that end inside a block and zero
+//                   fill of keys that nobody sees, and arrives on the stage's
+//                   barrier by itself; e4m3 rows through registers, where they
+//                   become the element type (exact in bf16).
 //   warp 12         MMA issue: S_t = Q_t K^T, O_t += P_t V, in the order
 //                   PV_0(n) S_0(n+1) PV_1(n) S_1(n+1), across tiles too: the
 //                   next tile's first scores do not wait for this tile's output.
 //   warp 13         the walk: the next pieces of work for the others.
 // Registers go to the softmax warps, which hold a row of scores each
-// (setmaxnreg: 2 x 128 x 168 + 128 x 96 + 128 x 80 = 65,536).
+// (setmaxnreg: 2 x 128 x 184 + 128 x 80 + 128 x 64 = 65,536).
 // TMEM: S_0 S_1 (128 columns each) O_0 O_1 (d each), one CTA per SM.
 //
 // The work of all tiles is laid on one line (a tile's length: the keys that it
@@ -39,6 +39,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "fp_attention_seq.cuh"
 #include "fp_launch.hpp"
@@ -58,10 +59,9 @@ constexpr int kStages = 4;       // K 0, V 0, K 1, V 1
 constexpr int kItems = 4;        // work items in flight between the roles
 constexpr int kLoadWarps = 4;
 constexpr int kThreads = 512;
-constexpr uint32_t kPlane = kKeys * 16 + 16;  // a group's rows, padded
+constexpr uint32_t kChunk = kKeys * 128;      // 128 rows of 64 channels
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
-constexpr uint32_t kPCol = 64;   // P among a half's 128 score columns
 constexpr float kGrowLog2 = 8.0f;
 constexpr int kTileCost = 384;   // a tile's work beside its keys, in keys
 constexpr int kMinShare = 256;   // keys
@@ -99,8 +99,8 @@ struct Smem {
 template <int D>
 struct Geo {
   static constexpr int kPlanes = D / 8;
-  static constexpr uint32_t kTileBytes = kPlanes * kPlane;  // 128 rows
-  static constexpr size_t kSmem = 1024 + (2 + kStages) * static_cast<size_t>(kTileBytes) + 128;
+  static constexpr uint32_t kTileBytes = D / 64 * kChunk;  // 128 rows
+  static constexpr size_t kSmem = 1024 + (2 + kStages) * static_cast<size_t>(kTileBytes) + 1024;
 };
 static_assert(sizeof(Smem) <= 1024, "barrier block");
 
@@ -158,10 +158,11 @@ __device__ __forceinline__ int tileLimit(const Args& a, const Sequence& q, int t
   return visible(a, q, (min(q.nq * a.group, (tile + 1) * kTileRows) - 1) / a.group);
 }
 
-// Key block at which place y of a tile of length w cuts it.
-__device__ __forceinline__ int cutBlock(long long y, long long w, int blocks, long long share) {
-  if (w * kSnap <= share) return 2 * y < w ? 0 : blocks;
-  return static_cast<int>(blocks * y / w);
+// Key block at which place y of a tile of length w cuts it. The two CTAs on
+// either side of a cut compute it alike, and it grows with y: fp32 will do.
+__device__ __forceinline__ int cutBlock(int y, int w, int blocks, int snap) {
+  if (w <= snap) return y < w - y ? 0 : blocks;
+  return min(static_cast<int>(__fdividef(static_cast<float>(y), static_cast<float>(w)) * static_cast<float>(blocks)), blocks);
 }
 
 // ---- waits ----
@@ -192,10 +193,96 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t fmt, int n, bool b_mn_majo
          (static_cast<uint32_t>(kHalf >> 4) << 24);
 }
 
+// One K step is 16 channels or keys. Q and K are K-major: rows of 128 bytes in
+// groups of 8 (1,024 bytes apart), a step 32 bytes on, 64 channels to a chunk.
+// V is MN-major: a step is two groups of 8 keys 1,024 bytes apart, 64 channels
+// of the output to a chunk. Descriptors are put together beside their
+// instruction: kept in registers they would take 128 of them.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (kLayoutSw128 << 29);
+
+__device__ __forceinline__ uint32_t descLow(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
+
+template <uint32_t kOffset>
+__device__ __forceinline__ void mmaScores(uint32_t d, uint32_t q, uint32_t k, uint32_t id) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 a, b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "add.u32 x, %1, %4;\n\tadd.u32 y, %2, %4;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(q), "r"(k), "r"(id), "n"(kOffset >> 4), "n"(kDescHigh)
+      : "memory");
+}
+
+template <uint32_t kStep>
+__device__ __forceinline__ void mmaValues(uint32_t d, uint32_t p, uint32_t v, uint32_t id, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "add.u32 x, %1, %5;\n\tadd.u32 y, %2, %6;\n\tmov.b64 b, {y, %7};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, p;\n\t}" ::"r"(d),
+      "r"(p), "r"(v), "r"(id), "r"(add), "n"(kStep * 8), "n"(kStep * 2048 >> 4), "n"(kDescHigh)
+      : "memory");
+}
+
+// The first step (offset 0) overwrites the scores, the others add.
+template <int D>
+__device__ __forceinline__ void issueScores(uint32_t d, uint32_t q, uint32_t k, uint32_t id) {
+  mmaScores<0>(d, q, k, id);
+  mmaScores<32>(d, q, k, id);
+  mmaScores<64>(d, q, k, id);
+  mmaScores<96>(d, q, k, id);
+  if constexpr (D == 128) {
+    mmaScores<kChunk>(d, q, k, id);
+    mmaScores<kChunk + 32>(d, q, k, id);
+    mmaScores<kChunk + 64>(d, q, k, id);
+    mmaScores<kChunk + 96>(d, q, k, id);
+  }
+}
+
+__device__ __forceinline__ void issueValues(uint32_t d, uint32_t p, uint32_t v, uint32_t id, int steps, bool add) {
+  mmaValues<0>(d, p, v, id, add ? 1u : 0u);
+  if (steps > 1) mmaValues<1>(d, p, v, id, 1u);
+  if (steps > 2) mmaValues<2>(d, p, v, id, 1u);
+  if (steps > 3) mmaValues<3>(d, p, v, id, 1u);
+  if (steps > 4) mmaValues<4>(d, p, v, id, 1u);
+  if (steps > 5) mmaValues<5>(d, p, v, id, 1u);
+  if (steps > 6) mmaValues<6>(d, p, v, id, 1u);
+  if (steps > 7) mmaValues<7>(d, p, v, id, 1u);
+}
+
 __device__ __forceinline__ float exp2Approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
 }
 
 __device__ __forceinline__ void copyAsync16(uint32_t dst, const void* src, bool in) {
@@ -227,8 +314,8 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   using G = Geo<D>;
   constexpr int kPlanes = G::kPlanes;
   constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-  extern __shared__ __align__(128) unsigned char smem_raw[];
-  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   Smem& sm = *reinterpret_cast<Smem*>(base);
   const uint32_t q_s = smemU32(base + 1024);
   const uint32_t kv_s = q_s + 2 * G::kTileBytes;
@@ -311,30 +398,35 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   tcFenceBefore();
   __syncthreads();
   tcFenceAfter();
-  const uint32_t tmem = sm.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   int* err = a.error_flag;
 
   if (warp >= 12) {
-    fewerRegisters<80>();
+    fewerRegisters<64>();
     if (warp == 12) {
       // ---------------- MMA issue ----------------
       const uint32_t idesc_o = idesc(kFmt, D, true);
       bool ok = true;
-      Item cur{}, nxt{};
+      struct Piece {
+        int halves, jb, je, lim;
+      };
+      Piece cur{}, nxt{};
       int i_next = 0;                 // items read so far
-      auto readItem = [&](Item& it) -> bool {
+      auto readItem = [&](Piece& it) -> bool {
         const int slot = i_next % kItems;
         if (!wait(&sm.item_full[slot], (i_next / kItems) & 1, sm, err, 55)) return false;
-        it = sm.items[slot];
+        const Item& from = sm.items[slot];
+        it = Piece{from.halves, from.jb, from.je, from.lim};
         __syncwarp();
         if (lane == 0) mbarArrive(&sm.item_empty[slot]);
         ++i_next;
         return true;
       };
       int n = 0;                                  // key blocks before the current one
-      int s_count[2] = {0, 0}, q_count[2] = {0, 0};  // score blocks issued, tiles begun
-      int pv_count[2] = {0, 0}, o_count[2] = {0, 0};
-      auto issueS = [&](const Item& it, int t, int j, int block) -> bool {
+      int q_count[2] = {0, 0}, pv_count[2] = {0, 0}, o_count[2] = {0, 0};  // tiles begun, blocks done, outputs begun
+      const uint32_t q_low = descLow(q_s, 16), k_low = descLow(kv_s, 16), v_low = descLow(kv_s, kChunk);
+      auto issueS = [&](const Piece& it, auto half, int j, int block) -> bool {
+        constexpr int t = decltype(half)::value;
         if (j == it.jb) {
           if (!wait(&sm.q_full[t], q_count[t] & 1, sm, err, 56)) return false;
           ++q_count[t];
@@ -345,53 +437,49 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         tcFenceAfter();
         const int keys = min(kKeys, max(it.lim - j * kKeys, 1));
         const uint32_t id = idesc(kFmt, (keys + 15) & ~15, false);
-        const uint32_t d = tmem + t * kKeys;
-        const uint32_t qa = q_s + t * G::kTileBytes, ka = kv_s + stage * G::kTileBytes;
-  #pragma unroll
-        for (int ks = 0; ks < kPlanes / 2; ++ks) {
-          tcMmaElect(d, smemDesc(qa + ks * 2 * kPlane, kPlane, 128, kLayoutNone), smemDesc(ka + ks * 2 * kPlane, kPlane, 128, kLayoutNone), id,
-                     ks > 0 ? 1u : 0u);
-        }
+        issueScores<D>(tmem + t * kKeys, q_low + t * (G::kTileBytes >> 4), k_low + stage * (G::kTileBytes >> 4), id);
         tcCommitElect(&sm.s_full[t]);
         if (t == it.halves - 1) tcCommitElect(&sm.kv_empty[stage]);
         if (j == it.je - 1) tcCommitElect(&sm.q_empty[t]);
-        ++s_count[t];
         return true;
       };
-      auto issuePV = [&](const Item& it, int t, int j, int block) -> bool {
-        if (!wait(&sm.p_full[t], pv_count[t] & 1, sm, err, 58)) return false;
+      auto issuePV = [&](const Piece& it, auto half, int j, int block) -> bool {
+        constexpr int t = decltype(half)::value;
         const int stage = (block & 1) * 2 + 1;
         if (t == 0 && !wait(&sm.kv_full[stage], (block >> 1) & 1, sm, err, 57)) return false;
         if (j == it.jb) {
           if (o_count[t] > 0 && !wait(&sm.o_free[t], (o_count[t] - 1) & 1, sm, err, 59)) return false;
           ++o_count[t];
         }
-        fenceProxyAsyncSmem();  // what the loading warps' copies wrote
+        if (t == 0) fenceProxyAsyncSmem();
+        if (!wait(&sm.p_full[t], pv_count[t] & 1, sm, err, 58)) return false;
         tcFenceAfter();
         const int keys = min(kKeys, max(it.lim - j * kKeys, 1));
         const int steps = (keys + 15) >> 4;
-        const uint32_t va = kv_s + stage * G::kTileBytes;
-        for (int ks = 0; ks < steps; ++ks) {
-          tcMmaTmemAElect(tmem + kOCol + t * D, tmem + t * kKeys + kPCol + ks * 8, smemDesc(va + ks * 256, 128, kPlane, kLayoutNone), idesc_o,
-                          (j > it.jb || ks > 0) ? 1u : 0u);
-        }
+        issueValues(tmem + kOCol + t * D, tmem + t * kKeys, v_low + stage * (G::kTileBytes >> 4), idesc_o, steps, j > it.jb);
         tcCommitElect(&sm.pv_done[t]);
         if (t == it.halves - 1) tcCommitElect(&sm.kv_empty[stage]);
         ++pv_count[t];
         return true;
       };
+      constexpr std::integral_constant<int, 0> kFirst{};
+      constexpr std::integral_constant<int, 1> kSecond{};
       ok = readItem(cur);
       if (ok && cur.halves > 0) {
-        for (int t = 0; t < cur.halves && ok; ++t) ok = issueS(cur, t, cur.jb, 0);
+        ok = issueS(cur, kFirst, cur.jb, 0);
+        if (ok && cur.halves > 1) ok = issueS(cur, kSecond, cur.jb, 0);
         while (ok && cur.halves > 0) {
           for (int j = cur.jb; j < cur.je && ok; ++j, ++n) {
             const bool last = j + 1 == cur.je;
             if (last) ok = readItem(nxt);
             const int halves_next = last ? nxt.halves : cur.halves;
-            for (int t = 0; t < 2 && ok; ++t) {
-              if (t < cur.halves) ok = issuePV(cur, t, j, n);
-              if (ok && t < halves_next) ok = last ? issueS(nxt, t, nxt.jb, n + 1) : issueS(cur, t, j + 1, n + 1);
-            }
+            auto turn = [&](auto half) {
+              constexpr int t = decltype(half)::value;
+              if (ok && t < cur.halves) ok = issuePV(cur, half, j, n);
+              if (ok && t < halves_next) ok = last ? issueS(nxt, half, nxt.jb, n + 1) : issueS(cur, half, j + 1, n + 1);
+            };
+            turn(kFirst);
+            turn(kSecond);
           }
           cur = nxt;
         }
@@ -410,13 +498,17 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         q = sequence<kKind>(a, seq);
         line = lineOf(a, q);
         const long long head_length = lengthBefore(line, line.tiles);
-        const long long inside = begin - sm.found[1];
-        head = static_cast<int>(inside / head_length);
-        tile = tileAt(line, inside - head * head_length);
-        at = sm.found[1] + head * head_length + lengthBefore(line, tile);
+        at = sm.found[1];
+        while (begin - at >= head_length) {
+          at += head_length;
+          ++head;
+        }
+        tile = tileAt(line, begin - at);
+        at += lengthBefore(line, tile);
       } else if (lane == 0) {
         cuts[blockIdx.x].tile_at = -1;
       }
+      const int snap = static_cast<int>(min(share / kSnap, 0x7fffffffLL));
       bool first = true;
       auto nextItem = [&](Item& it) {
         it.halves = 0;
@@ -439,8 +531,8 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           const int length = tileLength(line, tile);
           it.lim = tileLimit(a, q, tile);
           const int blocks = blocksOf(it.lim);
-          it.jb = begin <= at ? 0 : cutBlock(begin - at, length, blocks, share);
-          it.je = end >= at + length ? blocks : cutBlock(end - at, length, blocks, share);
+          it.jb = begin <= at ? 0 : cutBlock(static_cast<int>(begin - at), length, blocks, snap);
+          it.je = end >= at + length ? blocks : cutBlock(static_cast<int>(end - at), length, blocks, snap);
           if (first && lane == 0) {
             Cut cut{};
             cut.tile_at = it.jb > 0 && it.jb < blocks ? at : -1;
@@ -480,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       }
     }
   } else if (warp >= 8) {
-    fewerRegisters<96>();
+    fewerRegisters<80>();
     // ---------------- loads ----------------
     constexpr int kWarpPlanes = kPlanes / kLoadWarps;  // planes of a warp where lanes take rows
     constexpr int kRowsAtOnce = 32 / kPlanes;          // rows of a warp's copy where lanes take planes
@@ -488,6 +580,15 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
     const int w = warp - 8;
     const int p_lane = lane % kPlanes;
     const int r_lane = w * kRowsAtOnce + lane / kPlanes;
+    static_assert(kRowStep % 8 == 0, "a lane's rows have one place in the swizzle");
+    // Byte of group p of row r in a tile: chunk p/8, row r, 16-byte column p%8 ^ r%8.
+    uint32_t put[kWarpPlanes];
+#pragma unroll
+    for (int p = 0; p < kWarpPlanes; ++p) {
+      const int plane = w * kWarpPlanes + p;
+      put[p] = (plane >> 3) * kChunk + lane * 128 + (((plane & 7) ^ (lane & 7)) << 4);
+    }
+    const uint32_t put_rows = (p_lane >> 3) * kChunk + r_lane * 128 + (((p_lane & 7) ^ (r_lane & 7)) << 4);
     bool ok = true;
     int n = 0;             // key blocks so far
     int used[2] = {0, 0};  // times that Q's halves were loaded
@@ -525,21 +626,21 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           ++used[t];
           const uint32_t dst = q_s + t * G::kTileBytes;
           if (a.q.row_stride == 16) {
-  #pragma unroll
+#pragma unroll
             for (int rr = 0; rr < kHalf; rr += 32) {
               const bool in = t * kHalf + rr + lane < rows;
               const unsigned char* src = rowOf(in ? t * kHalf + rr + lane : 0, w * kWarpPlanes);
-  #pragma unroll
+#pragma unroll
               for (int p = 0; p < kWarpPlanes; ++p) {
-                copyAsync16(dst + (w * kWarpPlanes + p) * kPlane + (rr + lane) * 16, src, in);
+                copyAsync16(dst + put[p] + rr * 128, src, in);
                 src += a.q.plane_stride;
               }
             }
           } else {
-  #pragma unroll 4
+#pragma unroll 4
             for (int rr = r_lane; rr < kHalf; rr += kRowStep) {
               const bool in = t * kHalf + rr < rows;
-              copyAsync16(dst + p_lane * kPlane + rr * 16, rowOf(in ? t * kHalf + rr : 0, p_lane), in);
+              copyAsync16(dst + put_rows + (rr - r_lane) * 128, rowOf(in ? t * kHalf + rr : 0, p_lane), in);
             }
           }
           copyArrive(&sm.q_full[t]);
@@ -598,9 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
               for (int p = 0; p < kWarpRecords; ++p) {
                 uint4 out[2];
                 dequantise16<T>(codes[c][p], sc[c], out);
-                const uint32_t at = dst + 2 * (w * kWarpRecords + p) * kPlane + (c * 32 + lane) * 16;
-                storeShared16(at, out[0]);
-                storeShared16(at + kPlane, out[1]);
+                storeShared16(dst + put[2 * p] + c * 4096, out[0]);
+                storeShared16(dst + put[2 * p + 1] + c * 4096, out[1]);
               }
             }
             mbarArrive(&sm.kv_full[stage]);
@@ -608,7 +708,6 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             if (n >= 2) ok = wait(&sm.kv_empty[stage], ((n >> 1) - 1) & 1, sm, err, 54);
             if (!ok) break;
             if (kKind == kPaged16 || v.row_stride == 16) {
-              const uint32_t to = dst + w * kWarpPlanes * kPlane + lane * 16;
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 bool yes;
@@ -622,18 +721,17 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
                 }
 #pragma unroll
                 for (int p = 0; p < kWarpPlanes; ++p) {
-                  copyAsync16(to + p * kPlane + c * 512, src, yes);
+                  copyAsync16(dst + put[p] + c * 4096, src, yes);
                   if (yes) src += v.plane_stride;
                 }
               }
             } else {
               const long long step = kRowStep * v.row_stride;
               const unsigned char* src = record(v, it.head, static_cast<long long>(it.k0) + j * kKeys + r_lane, p_lane);
-              const uint32_t to = dst + p_lane * kPlane + r_lane * 16;
 #pragma unroll
               for (int x = 0; x < kKeys / kRowStep; ++x) {
                 const bool yes = r_lane + x * kRowStep < lim;
-                copyAsync16(to + x * kRowStep * 16, yes ? src : data, yes);
+                copyAsync16(dst + put_rows + x * kRowStep * 128, yes ? src : data, yes);
                 src += step;
               }
             }
@@ -644,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
     }
     copyDrain();
   } else {
-    moreRegisters<168>();
+    moreRegisters<184>();
     // ---------------- softmax and output ----------------
     const int t = warp >> 2;
     const int rr = (warp & 3) * 32 + lane;
@@ -683,36 +781,29 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         ok = wait(&sm.s_full[t], count & 1, sm, err, 58);
         if (!ok) break;
         tcFenceAfter();
-        // The maximum over both halves of the row, the second of which stays in
-        // registers; the first is read again once the maximum is known.
-        const bool edge = (j + 1) * kKeys > min_vis || bad != 0;  // the causal edge, the last keys, bad pages
-        const int lim = vis - j * kKeys;
-        uint32_t sv[64];
-        auto load = [&](int c) {
-          FPB_TMEM_LD32(s_base + 64 * c, sv);
-          FPB_TMEM_LD32(s_base + 64 * c + 32, (sv + 32));
-          tmemWaitLd();
-          if (edge) {
+        uint32_t sv[kKeys];
+        FPB_TMEM_LD32(s_base, sv);
+        FPB_TMEM_LD32(s_base + 32, (sv + 32));
+        FPB_TMEM_LD32(s_base + 64, (sv + 64));
+        FPB_TMEM_LD32(s_base + 96, (sv + 96));
+        tmemWaitLd();
+        if ((j + 1) * kKeys > min_vis || bad != 0) {  // the causal edge, the last keys, bad pages
+          const int lim = vis - j * kKeys;
 #pragma unroll
-            for (int e = 0; e < 64; ++e) {
-              if (64 * c + e >= lim) sv[e] = __float_as_uint(-INFINITY);
-            }
-            if (bad != 0) {
+          for (int e = 0; e < kKeys; ++e) {
+            if (e >= lim) sv[e] = __float_as_uint(-INFINITY);
+          }
+          if (bad != 0) {
 #pragma unroll
-              for (int e = 0; e < 64; ++e) {
-                if (((bad >> (4 * c + (e >> 4))) & 1u) != 0) sv[e] = __float_as_uint(-INFINITY);
-              }
+            for (int e = 0; e < kKeys; ++e) {
+              if (((bad >> (e >> 4)) & 1u) != 0) sv[e] = __float_as_uint(-INFINITY);
             }
           }
-        };
+        }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          load(c);
-#pragma unroll
-          for (int e = 0; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(sv[e]));
-        }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+        for (int e = 0; e < kKeys; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+        const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
         if (j == it.jb) {
           m = top;
         } else if (__any_sync(0xffffffffu, top > m + kGrowLog2)) {
@@ -734,25 +825,23 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           l *= f;
           m = m_new;
         }
-        // P over the second half's columns: keys 64 .. 127 go to the last 32,
-        // keys 0 .. 63 to the 32 before.
         const float neg = m == -INFINITY ? 0.0f : -m;  // a row that has seen no key yet
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), neg2 = pair(neg, neg);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int c = 1; c >= 0; --c) {
-          if (c == 0) load(0);
+        for (int c = 0; c < 2; ++c) {
           uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float p0 = exp2Approx(fmaf(__uint_as_float(sv[2 * e]), a.scale_log2, neg));
-            const float p1 = exp2Approx(fmaf(__uint_as_float(sv[2 * e + 1]), a.scale_log2, neg));
-            part[(e & 1) * 2] += p0;
-            part[(e & 1) * 2 + 1] += p1;
+            const float2 x = unpair(fma2(pair(__uint_as_float(sv[64 * c + 2 * e]), __uint_as_float(sv[64 * c + 2 * e + 1])), scale2, neg2));
+            const float p0 = exp2Approx(x.x), p1 = exp2Approx(x.y);
+            sum[e & 1] = add2(sum[e & 1], pair(p0, p1));
             pk[e] = pack2<T>(p0, p1);
           }
-          FPB_TMEM_ST32(s_base + kPCol + 32 * c, pk);
+          FPB_TMEM_ST32(s_base + 32 * c, pk);
         }
-        l += (part[0] + part[1]) + (part[2] + part[3]);
+        const float2 part = unpair(add2(sum[0], sum[1]));
+        l += part.x + part.y;
         tmemStoreWait();
         tcFenceBefore();
         __syncwarp();
