@@ -23,10 +23,13 @@
 //                   fill of keys that nobody sees, and arrives on the stage's
 //                   barrier by itself; e4m3 rows through registers, where they
 //                   become the element type (exact in bf16).
-//   warp 12         MMA issue: S_t = Q_t K^T, O_t += P_t V, in the order
-//                   PV_0(n) S_0(n+1) PV_1(n) S_1(n+1), across tiles too: the
-//                   next tile's first scores do not wait for this tile's output.
+//   warps 12, 15    MMA issue for half 0 and 1: S = Q K^T, then for each block
+//                   O += P V (its first 64 keys as soon as they are there) and
+//                   the next block's scores, across tiles too. One warp for
+//                   both would be bound by its own instructions.
 //   warp 13         the walk: the next pieces of work for the others.
+//   warp 14         the proxy fence between a load's arrival and the MMAs that
+//                   read it, which would cost the issuing warp 300-600 cycles.
 // Registers go to the softmax warps, which hold a row of scores each
 // (setmaxnreg: 2 x 128 x 184 + 128 x 80 + 128 x 64 = 65,536).
 // TMEM: S_0 S_1 (128 columns each) O_0 O_1 (d each), one CTA per SM.
@@ -87,8 +90,9 @@ struct Smem {
   uint64_t item_full[kItems], item_empty[kItems];
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[kStages], kv_empty[kStages];
-  uint64_t s_full[2], p_full[2], pv_done[2], o_free[2];
-  uint64_t drained;
+  uint64_t q_ready[2], kv_ready[kStages];  // full, and fenced for the tensor core
+  uint64_t s_full[2], p_half[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t drained[2];
   Item items[kItems];
   long long scan[kThreads / 32 + 1];
   long long found[2];
@@ -182,10 +186,11 @@ __device__ __forceinline__ bool waitSlow(uint64_t* bar, uint32_t parity, volatil
   }
 }
 
-// By a whole (converged) warp; lane 0's outcome is the warp's.
+// By a whole (converged) warp. The vote also tells the compiler that the warp
+// stays together, which keeps the MMA issue on the uniform datapath.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Smem& sm, int* err, int code) {
-  const bool ok = mbarTryWait(bar, parity) || waitSlow(bar, parity, &sm.stop, err, code);
-  return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+  if (__all_sync(0xffffffffu, mbarTryWait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, waitSlow(bar, parity, &sm.stop, err, code));
 }
 
 __host__ __device__ constexpr uint32_t idesc(uint32_t fmt, int n, bool b_mn_major) {
@@ -241,15 +246,13 @@ __device__ __forceinline__ void issueScores(uint32_t d, uint32_t q, uint32_t k, 
   }
 }
 
+// Steps kFirst .. kFirst + 3 of a block's 8, as far as it has keys.
+template <int kFirst>
 __device__ __forceinline__ void issueValues(uint32_t d, uint32_t p, uint32_t v, uint32_t id, int steps, bool add) {
-  mmaValues<0>(d, p, v, id, add ? 1u : 0u);
-  if (steps > 1) mmaValues<1>(d, p, v, id, 1u);
-  if (steps > 2) mmaValues<2>(d, p, v, id, 1u);
-  if (steps > 3) mmaValues<3>(d, p, v, id, 1u);
-  if (steps > 4) mmaValues<4>(d, p, v, id, 1u);
-  if (steps > 5) mmaValues<5>(d, p, v, id, 1u);
-  if (steps > 6) mmaValues<6>(d, p, v, id, 1u);
-  if (steps > 7) mmaValues<7>(d, p, v, id, 1u);
+  if (steps > kFirst) mmaValues<kFirst>(d, p, v, id, add ? 1u : 0u);
+  if (steps > kFirst + 1) mmaValues<kFirst + 1>(d, p, v, id, 1u);
+  if (steps > kFirst + 2) mmaValues<kFirst + 2>(d, p, v, id, 1u);
+  if (steps > kFirst + 3) mmaValues<kFirst + 3>(d, p, v, id, 1u);
 }
 
 __device__ __forceinline__ float exp2Approx(float x) {
@@ -325,21 +328,24 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   if (tid == 0) {
     for (int i = 0; i < kItems; ++i) {
       mbarInit(&sm.item_full[i], 1);
-      mbarInit(&sm.item_empty[i], 8 + 1 + kLoadWarps);
+      mbarInit(&sm.item_empty[i], 8 + 3 + kLoadWarps);
     }
     for (int i = 0; i < 2; ++i) {
       mbarInit(&sm.q_full[i], kLoadWarps * 32);
       mbarInit(&sm.q_empty[i], 1);
+      mbarInit(&sm.q_ready[i], 1);
       mbarInit(&sm.s_full[i], 1);
+      mbarInit(&sm.p_half[i], 4);
       mbarInit(&sm.p_full[i], 4);
       mbarInit(&sm.pv_done[i], 1);
       mbarInit(&sm.o_free[i], 4);
+      mbarInit(&sm.drained[i], 1);
     }
     for (int i = 0; i < kStages; ++i) {
       mbarInit(&sm.kv_full[i], kLoadWarps * 32);
-      mbarInit(&sm.kv_empty[i], 1);
+      mbarInit(&sm.kv_empty[i], 2);
+      mbarInit(&sm.kv_ready[i], 1);
     }
-    mbarInit(&sm.drained, 1);
     sm.stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -403,90 +409,102 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
 
   if (warp >= 12) {
     fewerRegisters<64>();
-    if (warp == 12) {
-      // ---------------- MMA issue ----------------
+    if (warp == 12 || warp == 15) {
+      // ---------------- MMA issue, a warp to each half ----------------
+      auto uniform = [](int x) { return __reduce_max_sync(0xffffffffu, x); };  // the same in every lane, and known to be
+      const int t = uniform(warp == 12 ? 0 : 1);
       const uint32_t idesc_o = idesc(kFmt, D, true);
-      bool ok = true;
+      const uint32_t q_low = descLow(q_s, 16) + t * (G::kTileBytes >> 4), k_low = descLow(kv_s, 16), v_low = descLow(kv_s, kChunk);
+      const uint32_t s_at = uniform(tmem) + t * kKeys, o_at = uniform(tmem) + kOCol + t * D;
       struct Piece {
         int halves, jb, je, lim;
       };
-      Piece cur{}, nxt{};
-      int i_next = 0;                 // items read so far
-      auto readItem = [&](Piece& it) -> bool {
-        const int slot = i_next % kItems;
-        if (!wait(&sm.item_full[slot], (i_next / kItems) & 1, sm, err, 55)) return false;
+      bool ok = true;
+      int items = 0, n = 0;              // items read, key blocks before the current one
+      int tiles = 0, outputs = 0, blocks = 0;  // of this half: begun, begun, done
+      auto readItem = [&]() -> Piece {
+        const int slot = items % kItems;
+        Piece it{0, 0, 0, 0};
+        ok = wait(&sm.item_full[slot], (items / kItems) & 1, sm, err, 55);
+        if (!ok) return it;
         const Item& from = sm.items[slot];
-        it = Piece{from.halves, from.jb, from.je, from.lim};
-        __syncwarp();
+        it = Piece{uniform(from.halves), uniform(from.jb), uniform(from.je), uniform(from.lim)};
         if (lane == 0) mbarArrive(&sm.item_empty[slot]);
-        ++i_next;
-        return true;
+        __syncwarp();
+        ++items;
+        return it;
       };
-      int n = 0;                                  // key blocks before the current one
-      int q_count[2] = {0, 0}, pv_count[2] = {0, 0}, o_count[2] = {0, 0};  // tiles begun, blocks done, outputs begun
-      const uint32_t q_low = descLow(q_s, 16), k_low = descLow(kv_s, 16), v_low = descLow(kv_s, kChunk);
-      auto issueS = [&](const Piece& it, auto half, int j, int block) -> bool {
-        constexpr int t = decltype(half)::value;
+      auto issueS = [&](const Piece& it, int j, int block) {
         if (j == it.jb) {
-          if (!wait(&sm.q_full[t], q_count[t] & 1, sm, err, 56)) return false;
-          ++q_count[t];
+          ok = wait(&sm.q_ready[t], tiles & 1, sm, err, 56);
+          if (!ok) return;
+          ++tiles;
         }
         const int stage = (block & 1) * 2;
-        if (t == 0 && !wait(&sm.kv_full[stage], (block >> 1) & 1, sm, err, 57)) return false;
-        fenceProxyAsyncSmem();  // what the loading warps' copies wrote
+        ok = wait(&sm.kv_ready[stage], (block >> 1) & 1, sm, err, 57);
+        if (!ok) return;
         tcFenceAfter();
         const int keys = min(kKeys, max(it.lim - j * kKeys, 1));
-        const uint32_t id = idesc(kFmt, (keys + 15) & ~15, false);
-        issueScores<D>(tmem + t * kKeys, q_low + t * (G::kTileBytes >> 4), k_low + stage * (G::kTileBytes >> 4), id);
+        issueScores<D>(s_at, q_low, k_low + stage * (G::kTileBytes >> 4), idesc(kFmt, (keys + 15) & ~15, false));
         tcCommitElect(&sm.s_full[t]);
-        if (t == it.halves - 1) tcCommitElect(&sm.kv_empty[stage]);
+        tcCommitElect(&sm.kv_empty[stage]);
         if (j == it.je - 1) tcCommitElect(&sm.q_empty[t]);
-        return true;
       };
-      auto issuePV = [&](const Piece& it, auto half, int j, int block) -> bool {
-        constexpr int t = decltype(half)::value;
+      auto issuePV = [&](const Piece& it, int j, int block) {
         const int stage = (block & 1) * 2 + 1;
-        if (t == 0 && !wait(&sm.kv_full[stage], (block >> 1) & 1, sm, err, 57)) return false;
-        if (j == it.jb) {
-          if (o_count[t] > 0 && !wait(&sm.o_free[t], (o_count[t] - 1) & 1, sm, err, 59)) return false;
-          ++o_count[t];
+        ok = wait(&sm.kv_ready[stage], (block >> 1) & 1, sm, err, 57);
+        if (ok && j == it.jb) {
+          if (outputs > 0) ok = wait(&sm.o_free[t], (outputs - 1) & 1, sm, err, 59);
+          ++outputs;
         }
-        if (t == 0) fenceProxyAsyncSmem();
-        if (!wait(&sm.p_full[t], pv_count[t] & 1, sm, err, 58)) return false;
+        if (ok) ok = wait(&sm.p_half[t], blocks & 1, sm, err, 58);
+        if (!ok) return;
         tcFenceAfter();
-        const int keys = min(kKeys, max(it.lim - j * kKeys, 1));
-        const int steps = (keys + 15) >> 4;
-        issueValues(tmem + kOCol + t * D, tmem + t * kKeys, v_low + stage * (G::kTileBytes >> 4), idesc_o, steps, j > it.jb);
+        const int steps = (min(kKeys, max(it.lim - j * kKeys, 1)) + 15) >> 4;
+        const uint32_t v = v_low + stage * (G::kTileBytes >> 4);
+        issueValues<0>(o_at, s_at, v, idesc_o, steps, j > it.jb);
+        ok = wait(&sm.p_full[t], blocks & 1, sm, err, 58);
+        if (!ok) return;
+        tcFenceAfter();
+        issueValues<4>(o_at, s_at, v, idesc_o, steps, true);
         tcCommitElect(&sm.pv_done[t]);
-        if (t == it.halves - 1) tcCommitElect(&sm.kv_empty[stage]);
-        ++pv_count[t];
-        return true;
+        tcCommitElect(&sm.kv_empty[stage]);
+        ++blocks;
       };
-      constexpr std::integral_constant<int, 0> kFirst{};
-      constexpr std::integral_constant<int, 1> kSecond{};
-      ok = readItem(cur);
-      if (ok && cur.halves > 0) {
-        ok = issueS(cur, kFirst, cur.jb, 0);
-        if (ok && cur.halves > 1) ok = issueS(cur, kSecond, cur.jb, 0);
-        while (ok && cur.halves > 0) {
+      Piece cur = readItem();
+      bool begun = false;  // the tile's first scores are under way
+      while (ok && cur.halves > 0) {
+        if (t >= cur.halves) {  // no rows here: the keys are the other half's
           for (int j = cur.jb; j < cur.je && ok; ++j, ++n) {
-            const bool last = j + 1 == cur.je;
-            if (last) ok = readItem(nxt);
-            const int halves_next = last ? nxt.halves : cur.halves;
-            auto turn = [&](auto half) {
-              constexpr int t = decltype(half)::value;
-              if (ok && t < cur.halves) ok = issuePV(cur, half, j, n);
-              if (ok && t < halves_next) ok = last ? issueS(nxt, half, nxt.jb, n + 1) : issueS(cur, half, j + 1, n + 1);
-            };
-            turn(kFirst);
-            turn(kSecond);
+            for (int side = 0; side < 2 && ok; ++side) {
+              const int stage = (n & 1) * 2 + side;
+              ok = wait(&sm.kv_ready[stage], (n >> 1) & 1, sm, err, 57);
+              if (ok && lane == 0) mbarArrive(&sm.kv_empty[stage]);
+              __syncwarp();
+            }
           }
-          cur = nxt;
+          if (ok) cur = readItem();
+          continue;
+        }
+        if (!begun) issueS(cur, cur.jb, n);
+        begun = false;
+        for (int j = cur.jb; j < cur.je && ok; ++j, ++n) {
+          issuePV(cur, j, n);
+          if (!ok) break;
+          if (j + 1 < cur.je) {
+            issueS(cur, j + 1, n + 1);
+          } else {
+            cur = readItem();
+            begun = ok && t < cur.halves;
+            if (begun) issueS(cur, cur.jb, n + 1);
+            ++n;
+            break;
+          }
         }
       }
       // Everything issued has completed before TMEM and shared memory go.
-      tcCommitElect(&sm.drained);
-      if (lane == 0) drainBar(&sm.drained, 0);
+      tcCommitElect(&sm.drained[t]);
+      if (lane == 0) drainBar(&sm.drained[t], 0);
       __syncwarp();
     } else if (warp == 13) {
       // ---------------- the walk ----------------
@@ -569,6 +587,36 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         }
         __syncwarp();
         if (it.halves == 0) break;
+      }
+    } else if (warp == 14) {
+      // ---------------- fences ----------------
+      // What has landed becomes visible to the tensor core, in the order of the loads.
+      bool ok = true;
+      int n = 0, used[2] = {0, 0};
+      auto pass = [&](uint64_t* full, uint64_t* ready, uint32_t parity) {
+        if (!ok) return;
+        ok = wait(full, parity, sm, err, 60);
+        fenceProxyAsyncSmem();
+        __syncwarp();
+        if (ok && lane == 0) mbarArrive(ready);
+      };
+      for (int i = 0; ok; ++i) {
+        const int slot = i % kItems;
+        ok = wait(&sm.item_full[slot], (i / kItems) & 1, sm, err, 52);
+        if (!ok) break;
+        const int halves = sm.items[slot].halves, blocks = sm.items[slot].je - sm.items[slot].jb;
+        __syncwarp();
+        if (lane == 0) mbarArrive(&sm.item_empty[slot]);
+        if (halves == 0) break;
+        for (int j = 0; j < blocks; ++j, ++n) {
+          const int stage = (n & 1) * 2;
+          pass(&sm.kv_full[stage], &sm.kv_ready[stage], (n >> 1) & 1);
+          if (j == 0) {
+            pass(&sm.q_full[0], &sm.q_ready[0], used[0]++ & 1);
+            if (halves > 1) pass(&sm.q_full[1], &sm.q_ready[1], used[1]++ & 1);
+          }
+          pass(&sm.kv_full[stage + 1], &sm.kv_ready[stage + 1], (n >> 1) & 1);
+        }
       }
     }
   } else if (warp >= 8) {
@@ -790,13 +838,14 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         if ((j + 1) * kKeys > min_vis || bad != 0) {  // the causal edge, the last keys, bad pages
           const int lim = vis - j * kKeys;
 #pragma unroll
-          for (int e = 0; e < kKeys; ++e) {
-            if (e >= lim) sv[e] = __float_as_uint(-INFINITY);
-          }
-          if (bad != 0) {
+          for (int c = 0; c < 4; ++c) {
+            const int in = min(max(lim - 32 * c, 0), 32);
+            uint32_t keep = in == 32 ? 0xffffffffu : (1u << in) - 1u;
+            if ((bad >> (2 * c)) & 1u) keep &= 0xffff0000u;
+            if ((bad >> (2 * c + 1)) & 1u) keep &= 0x0000ffffu;
 #pragma unroll
-            for (int e = 0; e < kKeys; ++e) {
-              if (((bad >> (e >> 4)) & 1u) != 0) sv[e] = __float_as_uint(-INFINITY);
+            for (int e = 0; e < 32; ++e) {
+              if (((keep >> e) & 1u) == 0) sv[32 * c + e] = __float_as_uint(-INFINITY);
             }
           }
         }
@@ -839,13 +888,14 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             pk[e] = pack2<T>(p0, p1);
           }
           FPB_TMEM_ST32(s_base + 32 * c, pk);
+          // The first 64 keys go ahead to the tensor core.
+          tmemStoreWait();
+          tcFenceBefore();
+          __syncwarp();
+          if (lane == 0) mbarArrive(c == 0 ? &sm.p_half[t] : &sm.p_full[t]);
         }
         const float2 part = unpair(add2(sum[0], sum[1]));
         l += part.x + part.y;
-        tmemStoreWait();
-        tcFenceBefore();
-        __syncwarp();
-        if (lane == 0) mbarArrive(&sm.p_full[t]);
       }
       if (ok) ok = wait(&sm.pv_done[t], (count - 1) & 1, sm, err, 59);
       if (!ok) break;
