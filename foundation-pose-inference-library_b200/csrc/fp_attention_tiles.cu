@@ -9,11 +9,11 @@
 // One persistent CTA per SM, 512 threads. Its tile is 256 query rows of one
 // (sequence, key head), two halves of 128 rows that take turns: while the
 // softmax of one half runs, the tensor core works for the other.
-//   warps 0-3, 4-7  softmax of half 0 and 1, one query row per thread: 64 scores
-//                   of the row from TMEM, running maximum and sum in fp32, P =
-//                   2^(s - m) rounded to the element type over the scores' own
-//                   TMEM columns. O is rescaled only when a row's maximum grows
-//                   by more than 2^8. After the last block, O / l.
+//   warps 0-3, 4-7  softmax of half 0 and 1, one query row per thread: the
+//                   row's 128 scores from TMEM, running maximum and sum in
+//                   fp32, P = 2^(s - m) rounded to the element type over the
+//                   scores' own TMEM columns. O is rescaled only when a row's
+//                   maximum grows by more than 2^8. After the last block, O / l.
 //   warps 8-11      loads: Q, K and V rows into 128-byte swizzled tiles of 64
 //                   channels [row][64], which lanes that take rows (planar
 //                   sources, pages) and lanes that take groups of channels
@@ -23,14 +23,16 @@
 //                   fill of keys that nobody sees, and arrives on the stage's
 //                   barrier by itself; e4m3 rows through registers, where they
 //                   become the element type (exact in bf16).
-//   warps 12, 15    MMA issue for half 0 and 1: S = Q K^T in sub-blocks of 64
-//                   keys, two ahead of O += P V and across tiles too, so that
-//                   the softmax never waits for a product. One warp for both
-//                   halves would be bound by its own instructions.
+//   warps 12, 15    MMA issue for half 0 and 1: S = Q K^T, then for each block
+//                   O += P V (its first 64 keys as soon as they are there) and
+//                   the next block's scores, across tiles too. One warp for
+//                   both would be bound by its own instructions.
 //   warp 13         the walk: the next pieces of work for the others.
 //   warp 14         the proxy fence between a load's arrival and the MMAs that
 //                   read it, which would cost the issuing warp 300-600 cycles.
-// TMEM: S_0 S_1 (two buffers of 64 columns each) O_0 O_1 (d each), one CTA per SM.
+// Registers go to the softmax warps, which hold a row of scores each
+// (setmaxnreg: 2 x 128 x 184 + 128 x 80 + 128 x 64 = 65,536).
+// TMEM: S_0 S_1 (128 columns each) O_0 O_1 (d each), one CTA per SM.
 //
 // The work of all tiles is laid on one line (a tile's length: the keys that it
 // sees) and cut into one share per CTA, so that causal and ragged batches and
@@ -55,8 +57,7 @@ namespace {
 using namespace tc;
 
 constexpr int kHalf = 128;       // rows of a half tile = TMEM lanes
-constexpr int kKeys = 128;       // keys of a block, as they are loaded
-constexpr int kSub = 64;         // keys of a sub-block, as they are computed
+constexpr int kKeys = 128;       // keys of a block
 constexpr int kStages = 4;       // K 0, V 0, K 1, V 1
 constexpr int kItems = 4;        // work items in flight between the roles
 constexpr int kLoadWarps = 4;
@@ -90,9 +91,7 @@ struct Smem {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t q_ready[2], kv_ready[kStages];  // full, and fenced for the tensor core
-  // [half][buffer]: a waiter may be a whole sub-block behind, so each buffer has its own phases.
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];
-  uint64_t o_free[2];
+  uint64_t s_full[2], p_half[2], p_full[2], pv_done[2], o_free[2];
   uint64_t drained[2];
   Item items[kItems];
   long long scan[kThreads / 32 + 1];
@@ -247,16 +246,14 @@ __device__ __forceinline__ void issueScores(uint32_t d, uint32_t q, uint32_t k, 
   }
 }
 
-// The steps of a sub-block, as far as it has keys.
+// Steps kFirst .. kFirst + 3 of a block's 8, as far as it has keys.
+template <int kFirst>
 __device__ __forceinline__ void issueValues(uint32_t d, uint32_t p, uint32_t v, uint32_t id, int steps, bool add) {
-  mmaValues<0>(d, p, v, id, add ? 1u : 0u);
-  if (steps > 1) mmaValues<1>(d, p, v, id, 1u);
-  if (steps > 2) mmaValues<2>(d, p, v, id, 1u);
-  if (steps > 3) mmaValues<3>(d, p, v, id, 1u);
+  if (steps > kFirst) mmaValues<kFirst>(d, p, v, id, add ? 1u : 0u);
+  if (steps > kFirst + 1) mmaValues<kFirst + 1>(d, p, v, id, 1u);
+  if (steps > kFirst + 2) mmaValues<kFirst + 2>(d, p, v, id, 1u);
+  if (steps > kFirst + 3) mmaValues<kFirst + 3>(d, p, v, id, 1u);
 }
-
-// Sub-blocks of key blocks jb .. je-1 of a tile that sees lim keys.
-__device__ __forceinline__ int subBlocks(int jb, int je, int lim) { return 2 * (je - jb) - (lim - (je - 1) * kKeys <= kSub ? 1 : 0); }
 
 __device__ __forceinline__ float exp2Approx(float x) {
   float y;
@@ -300,6 +297,15 @@ __device__ __forceinline__ void copyArrive(uint64_t* bar) {
 }
 __device__ __forceinline__ void copyDrain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+template <int N>
+__device__ __forceinline__ void moreRegisters() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewerRegisters() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 __device__ __forceinline__ void storeShared16(uint32_t dst, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -328,11 +334,10 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       mbarInit(&sm.q_full[i], kLoadWarps * 32);
       mbarInit(&sm.q_empty[i], 1);
       mbarInit(&sm.q_ready[i], 1);
-      for (int j = 0; j < 2; ++j) {
-        mbarInit(&sm.s_full[i][j], 1);
-        mbarInit(&sm.p_full[i][j], 4);
-        mbarInit(&sm.pv_done[i][j], 1);
-      }
+      mbarInit(&sm.s_full[i], 1);
+      mbarInit(&sm.p_half[i], 4);
+      mbarInit(&sm.p_full[i], 4);
+      mbarInit(&sm.pv_done[i], 1);
       mbarInit(&sm.o_free[i], 4);
       mbarInit(&sm.drained[i], 1);
     }
@@ -403,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   int* err = a.error_flag;
 
   if (warp >= 12) {
+    fewerRegisters<64>();
     if (warp == 12 || warp == 15) {
       // ---------------- MMA issue, a warp to each half ----------------
       auto uniform = [](int x) { return __reduce_max_sync(0xffffffffu, x); };  // the same in every lane, and known to be
@@ -410,118 +416,90 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       const uint32_t idesc_o = idesc(kFmt, D, true);
       const uint32_t q_low = descLow(q_s, 16) + t * (G::kTileBytes >> 4), k_low = descLow(kv_s, 16), v_low = descLow(kv_s, kChunk);
       const uint32_t s_at = uniform(tmem) + t * kKeys, o_at = uniform(tmem) + kOCol + t * D;
-      struct Cursor {
-        int item, halves, jb, je, lim;  // the piece of work
-        int subs, sub;                  // its sub-blocks, the next of them
-        int block, count;               // key blocks before the piece, sub-blocks of this half before the next
+      struct Piece {
+        int halves, jb, je, lim;
       };
       bool ok = true;
-      auto fetch = [&](Cursor& c) {
-        const int slot = c.item % kItems;
-        ok = wait(&sm.item_full[slot], (c.item / kItems) & 1, sm, err, 55);
-        const Item& it = sm.items[slot];
-        c.halves = ok ? uniform(it.halves) : 0;
-        c.jb = uniform(it.jb);
-        c.je = uniform(it.je);
-        c.lim = uniform(it.lim);
-        c.subs = subBlocks(c.jb, c.je, c.lim);
-        c.sub = 0;
-      };
-      auto advance = [&](Cursor& c) {
-        c.block += c.je - c.jb;
-        ++c.item;
-      };
-      auto release = [&](const Cursor& c) {
+      int items = 0, n = 0;              // items read, key blocks before the current one
+      int tiles = 0, outputs = 0, blocks = 0;  // of this half: begun, begun, done
+      auto readItem = [&]() -> Piece {
+        const int slot = items % kItems;
+        Piece it{0, 0, 0, 0};
+        ok = wait(&sm.item_full[slot], (items / kItems) & 1, sm, err, 55);
+        if (!ok) return it;
+        const Item& from = sm.items[slot];
+        it = Piece{uniform(from.halves), uniform(from.jb), uniform(from.je), uniform(from.lim)};
+        if (lane == 0) mbarArrive(&sm.item_empty[slot]);
         __syncwarp();
-        if (lane == 0) mbarArrive(&sm.item_empty[c.item % kItems]);
+        ++items;
+        return it;
       };
-      int tiles = 0, outputs = 0;  // of this half: begun
-      auto issueS = [&](Cursor& c) {
-        const int u = c.sub & 1, j = c.jb + (c.sub >> 1), block = c.block + (c.sub >> 1);
-        const int stage = (block & 1) * 2;
-        if (c.sub == 0) {
+      auto issueS = [&](const Piece& it, int j, int block) {
+        if (j == it.jb) {
           ok = wait(&sm.q_ready[t], tiles & 1, sm, err, 56);
           if (!ok) return;
           ++tiles;
         }
-        if (u == 0) {
-          ok = wait(&sm.kv_ready[stage], (block >> 1) & 1, sm, err, 57);
-          if (!ok) return;
-        }
-        // The buffer holds the P of two sub-blocks before. MMAs of different
-        // shapes are not ordered among themselves: that product has to be done.
-        if (c.count >= 2) {
-          ok = wait(&sm.pv_done[t][c.count & 1], ((c.count >> 1) - 1) & 1, sm, err, 59);
-          if (!ok) return;
-        }
+        const int stage = (block & 1) * 2;
+        ok = wait(&sm.kv_ready[stage], (block >> 1) & 1, sm, err, 57);
+        if (!ok) return;
         tcFenceAfter();
-        const int keys = min(kSub, max(c.lim - j * kKeys - u * kSub, 1));
-        issueScores<D>(s_at + (c.count & 1) * kSub, q_low, k_low + stage * (G::kTileBytes >> 4) + u * (kSub * 128 >> 4),
-                       idesc(kFmt, (keys + 15) & ~15, false));
-        tcCommitElect(&sm.s_full[t][c.count & 1]);
-        ++c.sub;
-        ++c.count;
-        if (u == 1 || c.sub == c.subs) tcCommitElect(&sm.kv_empty[stage]);
-        if (c.sub == c.subs) tcCommitElect(&sm.q_empty[t]);
+        const int keys = min(kKeys, max(it.lim - j * kKeys, 1));
+        issueScores<D>(s_at, q_low, k_low + stage * (G::kTileBytes >> 4), idesc(kFmt, (keys + 15) & ~15, false));
+        tcCommitElect(&sm.s_full[t]);
+        tcCommitElect(&sm.kv_empty[stage]);
+        if (j == it.je - 1) tcCommitElect(&sm.q_empty[t]);
       };
-      auto issuePV = [&](Cursor& c) {
-        const int u = c.sub & 1, j = c.jb + (c.sub >> 1), block = c.block + (c.sub >> 1);
+      auto issuePV = [&](const Piece& it, int j, int block) {
         const int stage = (block & 1) * 2 + 1;
-        if (u == 0) {
-          ok = wait(&sm.kv_ready[stage], (block >> 1) & 1, sm, err, 57);
-          if (!ok) return;
-        }
-        if (c.sub == 0) {
+        ok = wait(&sm.kv_ready[stage], (block >> 1) & 1, sm, err, 57);
+        if (ok && j == it.jb) {
           if (outputs > 0) ok = wait(&sm.o_free[t], (outputs - 1) & 1, sm, err, 59);
           ++outputs;
         }
-        if (ok) ok = wait(&sm.p_full[t][c.count & 1], (c.count >> 1) & 1, sm, err, 58);
+        if (ok) ok = wait(&sm.p_half[t], blocks & 1, sm, err, 58);
         if (!ok) return;
         tcFenceAfter();
-        const int steps = (min(kSub, max(c.lim - j * kKeys - u * kSub, 1)) + 15) >> 4;
-        issueValues(o_at, s_at + (c.count & 1) * kSub, v_low + stage * (G::kTileBytes >> 4) + u * (kSub * 128 >> 4), idesc_o, steps, c.sub > 0);
-        tcCommitElect(&sm.pv_done[t][c.count & 1]);
-        ++c.sub;
-        ++c.count;
-        if (u == 1 || c.sub == c.subs) tcCommitElect(&sm.kv_empty[stage]);
+        const int steps = (min(kKeys, max(it.lim - j * kKeys, 1)) + 15) >> 4;
+        const uint32_t v = v_low + stage * (G::kTileBytes >> 4);
+        issueValues<0>(o_at, s_at, v, idesc_o, steps, j > it.jb);
+        ok = wait(&sm.p_full[t], blocks & 1, sm, err, 58);
+        if (!ok) return;
+        tcFenceAfter();
+        issueValues<4>(o_at, s_at, v, idesc_o, steps, true);
+        tcCommitElect(&sm.pv_done[t]);
+        tcCommitElect(&sm.kv_empty[stage]);
+        ++blocks;
       };
-      // Scores run two sub-blocks ahead of the products with V.
-      Cursor sc{}, pv{};
-      fetch(sc);
-      pv = sc;
-      int ahead = 0;
-      while (ok) {
-        if (ahead < 2 && t < sc.halves) {
-          issueS(sc);
-          ++ahead;
-          if (ok && sc.sub == sc.subs) {
-            advance(sc);
-            fetch(sc);
-          }
-        } else if (ahead > 0) {
-          issuePV(pv);
-          --ahead;
-          if (ok && pv.sub == pv.subs) {
-            release(pv);
-            advance(pv);
-            fetch(pv);
-          }
-        } else if (sc.halves > 0) {  // no rows here: the keys are the other half's
-          for (int n = sc.block; n < sc.block + sc.je - sc.jb && ok; ++n) {
+      Piece cur = readItem();
+      bool begun = false;  // the tile's first scores are under way
+      while (ok && cur.halves > 0) {
+        if (t >= cur.halves) {  // no rows here: the keys are the other half's
+          for (int j = cur.jb; j < cur.je && ok; ++j, ++n) {
             for (int side = 0; side < 2 && ok; ++side) {
               const int stage = (n & 1) * 2 + side;
               ok = wait(&sm.kv_ready[stage], (n >> 1) & 1, sm, err, 57);
-              __syncwarp();
               if (ok && lane == 0) mbarArrive(&sm.kv_empty[stage]);
+              __syncwarp();
             }
           }
-          release(sc);
-          advance(sc);
-          advance(pv);
-          if (ok) fetch(sc);
-          if (ok) fetch(pv);
-        } else {
-          break;
+          if (ok) cur = readItem();
+          continue;
+        }
+        if (!begun) issueS(cur, cur.jb, n);
+        begun = false;
+        for (int j = cur.jb; j < cur.je && ok; ++j, ++n) {
+          issuePV(cur, j, n);
+          if (!ok) break;
+          if (j + 1 < cur.je) {
+            issueS(cur, j + 1, n + 1);
+          } else {
+            cur = readItem();
+            begun = ok && t < cur.halves;
+            if (begun) issueS(cur, cur.jb, n + 1);
+            ++n;
+            break;
+          }
         }
       }
       // Everything issued has completed before TMEM and shared memory go.
@@ -642,6 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       }
     }
   } else if (warp >= 8) {
+    fewerRegisters<80>();
     // ---------------- loads ----------------
     constexpr int kWarpPlanes = kPlanes / kLoadWarps;  // planes of a warp where lanes take rows
     constexpr int kRowsAtOnce = 32 / kPlanes;          // rows of a warp's copy where lanes take planes
@@ -811,6 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
     }
     copyDrain();
   } else {
+    moreRegisters<184>();
     // ---------------- softmax and output ----------------
     const int t = warp >> 2;
     const int rr = (warp & 3) * 32 + lane;
@@ -843,31 +823,22 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         return lane < kKeys / 16 && key < it.lim ? pageOf(a, it.seq, key) : 0;
       };
       page_next = pagesOf(it.jb);
-      const int subs = subBlocks(it.jb, it.je, it.lim);
-      uint32_t bad = 0;
-      for (int sub = 0; sub < subs && ok; ++sub, ++count) {
-        const int first = it.jb * kKeys + sub * kSub;  // key
-        const int buffer = count & 1;
-        const uint32_t s_now = s_base + buffer * kSub;
-        if constexpr (kKind != kPacked16) {
-          if ((sub & 1) == 0) {
-            bad = __ballot_sync(0xffffffffu, page_next < 0);
-            if (sub + 2 < subs) page_next = pagesOf(it.jb + (sub >> 1) + 1);
-          } else {
-            bad >>= 4;
-          }
-        }
-        ok = wait(&sm.s_full[t][buffer], (count >> 1) & 1, sm, err, 58);
+      for (int j = it.jb; j < it.je && ok; ++j, ++count) {
+        const uint32_t bad = kKind == kPacked16 ? 0u : __ballot_sync(0xffffffffu, page_next < 0);
+        if (j + 1 < it.je) page_next = pagesOf(j + 1);
+        ok = wait(&sm.s_full[t], count & 1, sm, err, 58);
         if (!ok) break;
         tcFenceAfter();
-        uint32_t sv[kSub];
-        FPB_TMEM_LD32(s_now, sv);
-        FPB_TMEM_LD32(s_now + 32, (sv + 32));
+        uint32_t sv[kKeys];
+        FPB_TMEM_LD32(s_base, sv);
+        FPB_TMEM_LD32(s_base + 32, (sv + 32));
+        FPB_TMEM_LD32(s_base + 64, (sv + 64));
+        FPB_TMEM_LD32(s_base + 96, (sv + 96));
         tmemWaitLd();
-        if (first + kSub > min_vis || (bad & 15u) != 0) {  // the causal edge, the last keys, bad pages
-          const int lim = vis - first;
+        if ((j + 1) * kKeys > min_vis || bad != 0) {  // the causal edge, the last keys, bad pages
+          const int lim = vis - j * kKeys;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 4; ++c) {
             const int in = min(max(lim - 32 * c, 0), 32);
             uint32_t keep = in == 32 ? 0xffffffffu : (1u << in) - 1u;
             if ((bad >> (2 * c)) & 1u) keep &= 0xffff0000u;
@@ -880,14 +851,14 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < kSub; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+        for (int e = 0; e < kKeys; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
         const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
-        if (sub == 0) {
+        if (j == it.jb) {
           m = top;
         } else if (__any_sync(0xffffffffu, top > m + kGrowLog2)) {
           const float m_new = top > m + kGrowLog2 ? top : m;
           const float f = m_new == m ? 1.0f : exp2Approx(m - m_new);
-          ok = wait(&sm.pv_done[t][(count - 1) & 1], ((count - 1) >> 1) & 1, sm, err, 59);
+          ok = wait(&sm.pv_done[t], (count - 1) & 1, sm, err, 59);
           if (!ok) break;
           tcFenceAfter();
 #pragma unroll 1
@@ -906,23 +877,27 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         const float neg = m == -INFINITY ? 0.0f : -m;  // a row that has seen no key yet
         const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), neg2 = pair(neg, neg);
         uint64_t sum[2] = {0, 0};
-        uint32_t pk[kSub / 2];
 #pragma unroll
-        for (int e = 0; e < kSub / 2; ++e) {
-          const float2 x = unpair(fma2(pair(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), scale2, neg2));
-          const float p0 = exp2Approx(x.x), p1 = exp2Approx(x.y);
-          sum[e & 1] = add2(sum[e & 1], pair(p0, p1));
-          pk[e] = pack2<T>(p0, p1);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float2 x = unpair(fma2(pair(__uint_as_float(sv[64 * c + 2 * e]), __uint_as_float(sv[64 * c + 2 * e + 1])), scale2, neg2));
+            const float p0 = exp2Approx(x.x), p1 = exp2Approx(x.y);
+            sum[e & 1] = add2(sum[e & 1], pair(p0, p1));
+            pk[e] = pack2<T>(p0, p1);
+          }
+          FPB_TMEM_ST32(s_base + 32 * c, pk);
+          // The first 64 keys go ahead to the tensor core.
+          tmemStoreWait();
+          tcFenceBefore();
+          __syncwarp();
+          if (lane == 0) mbarArrive(c == 0 ? &sm.p_half[t] : &sm.p_full[t]);
         }
-        FPB_TMEM_ST32(s_now, pk);
-        tmemStoreWait();
-        tcFenceBefore();
-        __syncwarp();
-        if (lane == 0) mbarArrive(&sm.p_full[t][buffer]);
         const float2 part = unpair(add2(sum[0], sum[1]));
         l += part.x + part.y;
       }
-      if (ok) ok = wait(&sm.pv_done[t][(count - 1) & 1], ((count - 1) >> 1) & 1, sm, err, 59);
+      if (ok) ok = wait(&sm.pv_done[t], (count - 1) & 1, sm, err, 59);
       if (!ok) break;
       tcFenceAfter();
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
