@@ -30,8 +30,6 @@
 //   warp 13         the walk: the next pieces of work for the others.
 //   warp 14         the proxy fence between a load's arrival and the MMAs that
 //                   read it, which would cost the issuing warp 300-600 cycles.
-// Registers go to the softmax warps, which hold a row of scores each
-// (setmaxnreg: 2 x 128 x 184 + 128 x 80 + 128 x 64 = 65,536).
 // TMEM: S_0 S_1 (128 columns each) O_0 O_1 (d each), one CTA per SM.
 //
 // The work of all tiles is laid on one line (a tile's length: the keys that it
@@ -92,6 +90,7 @@ struct Smem {
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t q_ready[2], kv_ready[kStages];  // full, and fenced for the tensor core
   uint64_t s_full[2], p_half[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t turn[2][4];         // a half's warp has finished its exponentials: the other half's may begin
   uint64_t drained[2];
   Item items[kItems];
   long long scan[kThreads / 32 + 1];
@@ -171,7 +170,7 @@ __device__ __forceinline__ int cutBlock(int y, int w, int blocks, int snap) {
 
 // ---- waits ----
 
-__device__ __forceinline__ bool waitSlow(uint64_t* bar, uint32_t parity, volatile int* stop, int* err, int code) {
+__device__ __noinline__ bool waitSlow(uint64_t* bar, uint32_t parity, volatile int* stop, int* err, int code) {
   const long long start = clock64();
   for (uint32_t i = 0;; ++i) {
     if (mbarTryWait(bar, parity)) return true;
@@ -198,61 +197,54 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t fmt, int n, bool b_mn_majo
          (static_cast<uint32_t>(kHalf >> 4) << 24);
 }
 
-// One K step is 16 channels or keys. Q and K are K-major: rows of 128 bytes in
-// groups of 8 (1,024 bytes apart), a step 32 bytes on, 64 channels to a chunk.
-// V is MN-major: a step is two groups of 8 keys 1,024 bytes apart, 64 channels
-// of the output to a chunk. Descriptors are put together beside their
-// instruction: kept in registers they would take 128 of them.
-constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (kLayoutSw128 << 29);
-
-__device__ __forceinline__ uint32_t descLow(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
-
-template <uint32_t kOffset>
-__device__ __forceinline__ void mmaScores(uint32_t d, uint32_t q, uint32_t k, uint32_t id) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 a, b;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "add.u32 x, %1, %4;\n\tadd.u32 y, %2, %4;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
-      "r"(q), "r"(k), "r"(id), "n"(kOffset >> 4), "n"(kDescHigh)
-      : "memory");
+// One lane of a converged warp, always the same.
+__device__ __forceinline__ bool electOne() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
-template <uint32_t kStep>
-__device__ __forceinline__ void mmaValues(uint32_t d, uint32_t p, uint32_t v, uint32_t id, uint32_t add) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 b;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "add.u32 x, %1, %5;\n\tadd.u32 y, %2, %6;\n\tmov.b64 b, {y, %7};\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, p;\n\t}" ::"r"(d),
-      "r"(p), "r"(v), "r"(id), "r"(add), "n"(kStep * 8), "n"(kStep * 2048 >> 4), "n"(kDescHigh)
-      : "memory");
+// MMAs and commits of one thread, in a branch of their own: guarded one by one
+// they take twice the instructions.
+template <int kAdd>
+__device__ __forceinline__ void mmaScores(uint32_t d, uint64_t q, uint64_t k, uint32_t id) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(q),
+               "l"(k), "r"(id), "n"(kAdd)
+               : "memory");
+}
+__device__ __forceinline__ void mmaValues(uint32_t d, uint32_t p, uint64_t v, uint32_t id, uint32_t add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(p),
+               "l"(v), "r"(id), "r"(add)
+               : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smemU32(bar)) : "memory");
 }
 
-// The first step (offset 0) overwrites the scores, the others add.
+// Operand descriptors. One K step is 16 channels or keys. Q and K are K-major:
+// rows of 128 bytes in groups of 8 (1,024 bytes apart), a step 32 bytes on, 64
+// channels to a chunk. V is MN-major: a step is two groups of 8 keys 1,024
+// bytes apart, 64 channels of the output to a chunk.
+__device__ __forceinline__ uint64_t keyDesc(uint32_t addr) { return smemDesc(addr, 16, 1024, kLayoutSw128); }
+__device__ __forceinline__ uint64_t valueDesc(uint32_t addr) { return smemDesc(addr, kChunk, 1024, kLayoutSw128); }
+
 template <int D>
-__device__ __forceinline__ void issueScores(uint32_t d, uint32_t q, uint32_t k, uint32_t id) {
+__device__ __forceinline__ void issueScores(uint32_t d, uint64_t q, uint64_t k, uint32_t id) {
   mmaScores<0>(d, q, k, id);
-  mmaScores<32>(d, q, k, id);
-  mmaScores<64>(d, q, k, id);
-  mmaScores<96>(d, q, k, id);
-  if constexpr (D == 128) {
-    mmaScores<kChunk>(d, q, k, id);
-    mmaScores<kChunk + 32>(d, q, k, id);
-    mmaScores<kChunk + 64>(d, q, k, id);
-    mmaScores<kChunk + 96>(d, q, k, id);
+#pragma unroll
+  for (int ks = 1; ks < D / 16; ++ks) {
+    const uint32_t at = ((ks / 4) * kChunk + (ks % 4) * 32) >> 4;
+    mmaScores<1>(d, q + at, k + at, id);
   }
 }
 
 // Steps kFirst .. kFirst + 3 of a block's 8, as far as it has keys.
 template <int kFirst>
-__device__ __forceinline__ void issueValues(uint32_t d, uint32_t p, uint32_t v, uint32_t id, int steps, bool add) {
-  if (steps > kFirst) mmaValues<kFirst>(d, p, v, id, add ? 1u : 0u);
-  if (steps > kFirst + 1) mmaValues<kFirst + 1>(d, p, v, id, 1u);
-  if (steps > kFirst + 2) mmaValues<kFirst + 2>(d, p, v, id, 1u);
-  if (steps > kFirst + 3) mmaValues<kFirst + 3>(d, p, v, id, 1u);
+__device__ __forceinline__ void issueValues(uint32_t d, uint32_t p, uint64_t v, uint32_t id, int steps, bool add) {
+#pragma unroll
+  for (int ks = kFirst; ks < kFirst + 4; ++ks) {
+    if (ks < steps) mmaValues(d, p + ks * 8, v + ks * (2048 >> 4), id, ks > kFirst || add ? 1u : 0u);
+  }
 }
 
 __device__ __forceinline__ float exp2Approx(float x) {
@@ -288,6 +280,26 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   return r;
 }
 
+// Masks 64 scores: those from lim on, and groups of 16 whose bit in bad is set.
+__device__ __noinline__ uint2 keepMask(int lim, uint32_t bad) {
+  uint32_t keep[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int in = min(max(lim - 32 * c, 0), 32);
+    keep[c] = in == 32 ? 0xffffffffu : (1u << in) - 1u;
+    if ((bad >> (2 * c)) & 1u) keep[c] &= 0xffff0000u;
+    if ((bad >> (2 * c + 1)) & 1u) keep[c] &= 0x0000ffffu;
+  }
+  return make_uint2(keep[0], keep[1]);
+}
+__device__ __forceinline__ void hide(uint32_t (&s)[64], int lim, uint32_t bad) {
+  const uint2 keep = keepMask(lim, bad);
+#pragma unroll
+  for (int e = 0; e < 64; ++e) {
+    if ((((e < 32 ? keep.x : keep.y) >> (e & 31)) & 1u) == 0) s[e] = __float_as_uint(-INFINITY);
+  }
+}
+
 __device__ __forceinline__ void copyAsync16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
@@ -296,15 +308,6 @@ __device__ __forceinline__ void copyArrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smemU32(bar)) : "memory");
 }
 __device__ __forceinline__ void copyDrain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
-template <int N>
-__device__ __forceinline__ void moreRegisters() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewerRegisters() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
 
 __device__ __forceinline__ void storeShared16(uint32_t dst, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -340,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       mbarInit(&sm.pv_done[i], 1);
       mbarInit(&sm.o_free[i], 4);
       mbarInit(&sm.drained[i], 1);
+      for (int j = 0; j < 4; ++j) mbarInit(&sm.turn[i][j], 1);
     }
     for (int i = 0; i < kStages; ++i) {
       mbarInit(&sm.kv_full[i], kLoadWarps * 32);
@@ -378,6 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
     __syncthreads();
     long long all = 0;
     at = upto - mine;
+#pragma unroll 1
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) at += sm.scan[w];
       all += sm.scan[w];
@@ -408,102 +413,114 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   int* err = a.error_flag;
 
   if (warp >= 12) {
-    fewerRegisters<64>();
     if (warp == 12 || warp == 15) {
       // ---------------- MMA issue, a warp to each half ----------------
       auto uniform = [](int x) { return __reduce_max_sync(0xffffffffu, x); };  // the same in every lane, and known to be
       const int t = uniform(warp == 12 ? 0 : 1);
       const uint32_t idesc_o = idesc(kFmt, D, true);
-      const uint32_t q_low = descLow(q_s, 16) + t * (G::kTileBytes >> 4), k_low = descLow(kv_s, 16), v_low = descLow(kv_s, kChunk);
+      const uint64_t q_desc = keyDesc(q_s + t * G::kTileBytes), k_desc = keyDesc(kv_s), v_desc = valueDesc(kv_s);
       const uint32_t s_at = uniform(tmem) + t * kKeys, o_at = uniform(tmem) + kOCol + t * D;
-      struct Piece {
-        int halves, jb, je, lim;
+      struct Cursor {
+        int item, halves, jb, je, lim;  // the piece of work
+        int j, block;                   // its next key block, that block's number in all
       };
       bool ok = true;
-      int items = 0, n = 0;              // items read, key blocks before the current one
-      int tiles = 0, outputs = 0, blocks = 0;  // of this half: begun, begun, done
-      auto readItem = [&]() -> Piece {
-        const int slot = items % kItems;
-        Piece it{0, 0, 0, 0};
-        ok = wait(&sm.item_full[slot], (items / kItems) & 1, sm, err, 55);
-        if (!ok) return it;
-        const Item& from = sm.items[slot];
-        it = Piece{uniform(from.halves), uniform(from.jb), uniform(from.je), uniform(from.lim)};
-        if (lane == 0) mbarArrive(&sm.item_empty[slot]);
+      auto release = [&](const Cursor& c) {
         __syncwarp();
-        ++items;
-        return it;
+        if (lane == 0) mbarArrive(&sm.item_empty[c.item % kItems]);
       };
-      auto issueS = [&](const Piece& it, int j, int block) {
-        if (j == it.jb) {
-          ok = wait(&sm.q_ready[t], tiles & 1, sm, err, 56);
-          if (!ok) return;
-          ++tiles;
+      int tiles = 0, outputs = 0, done = 0;  // of this half: tiles begun, outputs begun, blocks done
+      // Scores run one block ahead of the products with V, across pieces too.
+      Cursor sc{}, pv{};
+      bool ahead = false, fetch = true;
+      for (;;) {
+        if (fetch) {
+          fetch = false;
+          const int slot = sc.item % kItems;
+          ok = wait(&sm.item_full[slot], (sc.item / kItems) & 1, sm, err, 55);
+          if (!ok) break;
+          const Item& it = sm.items[slot];
+          sc.halves = uniform(it.halves);
+          sc.jb = sc.j = uniform(it.jb);
+          sc.je = uniform(it.je);
+          sc.lim = uniform(it.lim);
+          if (!ahead) pv = sc;
         }
-        const int stage = (block & 1) * 2;
-        ok = wait(&sm.kv_ready[stage], (block >> 1) & 1, sm, err, 57);
-        if (!ok) return;
-        tcFenceAfter();
-        const int keys = min(kKeys, max(it.lim - j * kKeys, 1));
-        issueScores<D>(s_at, q_low, k_low + stage * (G::kTileBytes >> 4), idesc(kFmt, (keys + 15) & ~15, false));
-        tcCommitElect(&sm.s_full[t]);
-        tcCommitElect(&sm.kv_empty[stage]);
-        if (j == it.je - 1) tcCommitElect(&sm.q_empty[t]);
-      };
-      auto issuePV = [&](const Piece& it, int j, int block) {
-        const int stage = (block & 1) * 2 + 1;
-        ok = wait(&sm.kv_ready[stage], (block >> 1) & 1, sm, err, 57);
-        if (ok && j == it.jb) {
-          if (outputs > 0) ok = wait(&sm.o_free[t], (outputs - 1) & 1, sm, err, 59);
-          ++outputs;
-        }
-        if (ok) ok = wait(&sm.p_half[t], blocks & 1, sm, err, 58);
-        if (!ok) return;
-        tcFenceAfter();
-        const int steps = (min(kKeys, max(it.lim - j * kKeys, 1)) + 15) >> 4;
-        const uint32_t v = v_low + stage * (G::kTileBytes >> 4);
-        issueValues<0>(o_at, s_at, v, idesc_o, steps, j > it.jb);
-        ok = wait(&sm.p_full[t], blocks & 1, sm, err, 58);
-        if (!ok) return;
-        tcFenceAfter();
-        issueValues<4>(o_at, s_at, v, idesc_o, steps, true);
-        tcCommitElect(&sm.pv_done[t]);
-        tcCommitElect(&sm.kv_empty[stage]);
-        ++blocks;
-      };
-      Piece cur = readItem();
-      bool begun = false;  // the tile's first scores are under way
-      while (ok && cur.halves > 0) {
-        if (t >= cur.halves) {  // no rows here: the keys are the other half's
-          for (int j = cur.jb; j < cur.je && ok; ++j, ++n) {
+        if (!ahead && t < sc.halves) {
+          if (sc.j == sc.jb) {
+            ok = wait(&sm.q_ready[t], tiles & 1, sm, err, 56);
+            ++tiles;
+          }
+          const int stage = (sc.block & 1) * 2;
+          if (ok) ok = wait(&sm.kv_ready[stage], (sc.block >> 1) & 1, sm, err, 57);
+          if (!ok) break;
+          tcFenceAfter();
+          const int keys = min(kKeys, max(sc.lim - sc.j * kKeys, 1));
+          ++sc.block;
+          ++sc.j;
+          if (electOne()) {
+            issueScores<D>(s_at, q_desc, k_desc + stage * (G::kTileBytes >> 4), idesc(kFmt, (keys + 15) & ~15, false));
+            commit(&sm.s_full[t]);
+            commit(&sm.kv_empty[stage]);
+            if (sc.j == sc.je) commit(&sm.q_empty[t]);
+          }
+          __syncwarp();
+          ahead = true;
+          if (sc.j == sc.je) {
+            ++sc.item;
+            fetch = true;
+          }
+        } else if (ahead) {
+          const int stage = (pv.block & 1) * 2 + 1;
+          ok = wait(&sm.kv_ready[stage], (pv.block >> 1) & 1, sm, err, 57);
+          if (ok && pv.j == pv.jb) {
+            if (outputs > 0) ok = wait(&sm.o_free[t], (outputs - 1) & 1, sm, err, 59);
+            ++outputs;
+          }
+          if (ok) ok = wait(&sm.p_half[t], done & 1, sm, err, 58);
+          if (!ok) break;
+          tcFenceAfter();
+          const int steps = (min(kKeys, max(pv.lim - pv.j * kKeys, 1)) + 15) >> 4;
+          const uint64_t v = v_desc + stage * (G::kTileBytes >> 4);
+          if (electOne()) issueValues<0>(o_at, s_at, v, idesc_o, steps, pv.j > pv.jb);
+          __syncwarp();
+          ok = wait(&sm.p_full[t], done & 1, sm, err, 58);
+          if (!ok) break;
+          tcFenceAfter();
+          if (electOne()) {
+            issueValues<4>(o_at, s_at, v, idesc_o, steps, true);
+            commit(&sm.pv_done[t]);
+            commit(&sm.kv_empty[stage]);
+          }
+          __syncwarp();
+          ahead = false;
+          ++done;
+          ++pv.block;
+          if (++pv.j == pv.je) {
+            release(pv);
+            pv = sc;  // the next piece, already fetched and not begun
+          }
+        } else if (sc.halves > 0) {  // no rows here: the keys are the other half's
+          for (; sc.j < sc.je && ok; ++sc.j, ++sc.block) {
             for (int side = 0; side < 2 && ok; ++side) {
-              const int stage = (n & 1) * 2 + side;
-              ok = wait(&sm.kv_ready[stage], (n >> 1) & 1, sm, err, 57);
-              if (ok && lane == 0) mbarArrive(&sm.kv_empty[stage]);
+              const int stage = (sc.block & 1) * 2 + side;
+              ok = wait(&sm.kv_ready[stage], (sc.block >> 1) & 1, sm, err, 57);
               __syncwarp();
+              if (ok && lane == 0) mbarArrive(&sm.kv_empty[stage]);
             }
           }
-          if (ok) cur = readItem();
-          continue;
-        }
-        if (!begun) issueS(cur, cur.jb, n);
-        begun = false;
-        for (int j = cur.jb; j < cur.je && ok; ++j, ++n) {
-          issuePV(cur, j, n);
           if (!ok) break;
-          if (j + 1 < cur.je) {
-            issueS(cur, j + 1, n + 1);
-          } else {
-            cur = readItem();
-            begun = ok && t < cur.halves;
-            if (begun) issueS(cur, cur.jb, n + 1);
-            ++n;
-            break;
-          }
+          release(sc);
+          ++sc.item;
+          fetch = true;
+        } else {
+          break;
         }
       }
       // Everything issued has completed before TMEM and shared memory go.
-      tcCommitElect(&sm.drained[t]);
+      __syncwarp();
+      if (electOne()) commit(&sm.drained[t]);
+      __syncwarp();
       if (lane == 0) drainBar(&sm.drained[t], 0);
       __syncwarp();
     } else if (warp == 13) {
@@ -592,14 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       // ---------------- fences ----------------
       // What has landed becomes visible to the tensor core, in the order of the loads.
       bool ok = true;
-      int n = 0, used[2] = {0, 0};
-      auto pass = [&](uint64_t* full, uint64_t* ready, uint32_t parity) {
-        if (!ok) return;
-        ok = wait(full, parity, sm, err, 60);
-        fenceProxyAsyncSmem();
-        __syncwarp();
-        if (ok && lane == 0) mbarArrive(ready);
-      };
+      int n = 0, used0 = 0, used1 = 0;  // key blocks, loads of Q's halves
       for (int i = 0; ok; ++i) {
         const int slot = i % kItems;
         ok = wait(&sm.item_full[slot], (i / kItems) & 1, sm, err, 52);
@@ -608,19 +618,22 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         __syncwarp();
         if (lane == 0) mbarArrive(&sm.item_empty[slot]);
         if (halves == 0) break;
-        for (int j = 0; j < blocks; ++j, ++n) {
-          const int stage = (n & 1) * 2;
-          pass(&sm.kv_full[stage], &sm.kv_ready[stage], (n >> 1) & 1);
-          if (j == 0) {
-            pass(&sm.q_full[0], &sm.q_ready[0], used[0]++ & 1);
-            if (halves > 1) pass(&sm.q_full[1], &sm.q_ready[1], used[1]++ & 1);
-          }
-          pass(&sm.kv_full[stage + 1], &sm.kv_ready[stage + 1], (n >> 1) & 1);
+        // K, Q's halves, V, then K and V of each block.
+        for (int x = 0; x < 2 * blocks + halves && ok; ++x) {
+          const bool is_q = x >= 1 && x <= halves;
+          const int t = x - 1, y = is_q ? 0 : x > halves ? x - halves : x;  // y: 2 * block + side
+          const int m = n + (y >> 1), stage = (m & 1) * 2 + (y & 1);
+          ok = wait(is_q ? &sm.q_full[t] : &sm.kv_full[stage], (is_q ? (t == 0 ? used0 : used1) : m >> 1) & 1, sm, err, 60);
+          fenceProxyAsyncSmem();
+          __syncwarp();
+          if (ok && lane == 0) mbarArrive(is_q ? &sm.q_ready[t] : &sm.kv_ready[stage]);
         }
+        n += blocks;
+        ++used0;
+        if (halves > 1) ++used1;
       }
     }
   } else if (warp >= 8) {
-    fewerRegisters<80>();
     // ---------------- loads ----------------
     constexpr int kWarpPlanes = kPlanes / kLoadWarps;  // planes of a warp where lanes take rows
     constexpr int kRowsAtOnce = 32 / kPlanes;          // rows of a warp's copy where lanes take planes
@@ -674,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           ++used[t];
           const uint32_t dst = q_s + t * G::kTileBytes;
           if (a.q.row_stride == 16) {
-#pragma unroll
+#pragma unroll 1
             for (int rr = 0; rr < kHalf; rr += 32) {
               const bool in = t * kHalf + rr + lane < rows;
               const unsigned char* src = rowOf(in ? t * kHalf + rr + lane : 0, w * kWarpPlanes);
@@ -685,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
               }
             }
           } else {
-#pragma unroll 4
+#pragma unroll 1
             for (int rr = r_lane; rr < kHalf; rr += kRowStep) {
               const bool in = t * kHalf + rr < rows;
               copyAsync16(dst + put_rows + (rr - r_lane) * 128, rowOf(in ? t * kHalf + rr : 0, p_lane), in);
@@ -776,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             } else {
               const long long step = kRowStep * v.row_stride;
               const unsigned char* src = record(v, it.head, static_cast<long long>(it.k0) + j * kKeys + r_lane, p_lane);
-#pragma unroll
+#pragma unroll 4
               for (int x = 0; x < kKeys / kRowStep; ++x) {
                 const bool yes = r_lane + x * kRowStep < lim;
                 copyAsync16(dst + put_rows + x * kRowStep * 128, yes ? src : data, yes);
@@ -790,7 +803,6 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
     }
     copyDrain();
   } else {
-    moreRegisters<184>();
     // ---------------- softmax and output ----------------
     const int t = warp >> 2;
     const int rr = (warp & 3) * 32 + lane;
@@ -799,6 +811,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
     const uint32_t o_base = lane_base + kOCol + t * D;
     bool ok = true;
     int count = 0;  // blocks of this half
+    int turns = 0;  // blocks that both halves have
     for (int i = 0; ok; ++i) {
       const int slot = i % kItems;
       ok = wait(&sm.item_full[slot], (i / kItems) & 1, sm, err, 55);
@@ -829,29 +842,24 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         ok = wait(&sm.s_full[t], count & 1, sm, err, 58);
         if (!ok) break;
         tcFenceAfter();
-        uint32_t sv[kKeys];
-        FPB_TMEM_LD32(s_base, sv);
-        FPB_TMEM_LD32(s_base + 32, (sv + 32));
-        FPB_TMEM_LD32(s_base + 64, (sv + 64));
-        FPB_TMEM_LD32(s_base + 96, (sv + 96));
-        tmemWaitLd();
-        if ((j + 1) * kKeys > min_vis || bad != 0) {  // the causal edge, the last keys, bad pages
-          const int lim = vis - j * kKeys;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int in = min(max(lim - 32 * c, 0), 32);
-            uint32_t keep = in == 32 ? 0xffffffffu : (1u << in) - 1u;
-            if ((bad >> (2 * c)) & 1u) keep &= 0xffff0000u;
-            if ((bad >> (2 * c + 1)) & 1u) keep &= 0x0000ffffu;
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              if (((keep >> e) & 1u) == 0) sv[32 * c + e] = __float_as_uint(-INFINITY);
-            }
-          }
-        }
+        // Twice over the row's scores, 64 at a time: reading them again from
+        // TMEM is cheap, keeping 128 in registers is not.
+        const bool edge = (j + 1) * kKeys > min_vis || bad != 0;  // the causal edge, the last keys, bad pages
+        const int lim = vis - j * kKeys;
+        uint32_t sv[64];
+        auto load = [&](int c) {
+          FPB_TMEM_LD32(s_base + 64 * c, sv);
+          FPB_TMEM_LD32(s_base + 64 * c + 32, (sv + 32));
+          tmemWaitLd();
+          if (edge) hide(sv, lim - 64 * c, bad >> (4 * c));
+        };
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          load(c);
 #pragma unroll
-        for (int e = 0; e < kKeys; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+          for (int e = 0; e < 64; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+        }
         const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
         if (j == it.jb) {
           m = top;
@@ -874,15 +882,27 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           l *= f;
           m = m_new;
         }
+        // The exponential unit goes from half to half: while one computes, the
+        // other's scores and products run. Left to themselves the halves fall
+        // into step and take turns at everything else, too.
+        if (it.halves == 2) {
+          if (t == 1) {
+            ok = wait(&sm.turn[0][warp & 3], turns & 1, sm, err, 61);
+          } else if (turns > 0) {
+            ok = wait(&sm.turn[1][warp & 3], (turns - 1) & 1, sm, err, 61);
+          }
+          if (!ok) break;
+        }
         const float neg = m == -INFINITY ? 0.0f : -m;  // a row that has seen no key yet
         const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), neg2 = pair(neg, neg);
         uint64_t sum[2] = {0, 0};
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
+          load(c);
           uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float2 x = unpair(fma2(pair(__uint_as_float(sv[64 * c + 2 * e]), __uint_as_float(sv[64 * c + 2 * e + 1])), scale2, neg2));
+            const float2 x = unpair(fma2(pair(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), scale2, neg2));
             const float p0 = exp2Approx(x.x), p1 = exp2Approx(x.y);
             sum[e & 1] = add2(sum[e & 1], pair(p0, p1));
             pk[e] = pack2<T>(p0, p1);
@@ -893,6 +913,10 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           tcFenceBefore();
           __syncwarp();
           if (lane == 0) mbarArrive(c == 0 ? &sm.p_half[t] : &sm.p_full[t]);
+        }
+        if (it.halves == 2) {
+          if (lane == 0) mbarArrive(&sm.turn[t][warp & 3]);
+          ++turns;
         }
         const float2 part = unpair(add2(sum[0], sum[1]));
         l += part.x + part.y;
