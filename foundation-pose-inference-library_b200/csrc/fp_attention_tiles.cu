@@ -972,8 +972,11 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   }
 }
 
+constexpr int kJoinGroups = 2;  // groups of 8 channels of a joining thread
+
 // Joins the pieces of a tile: CTA c looks after the tile that share c begins
-// inside, if it is the first share to. A thread joins 8 channels of a row.
+// inside, if it is the first share to. A thread joins kJoinGroups x 8 channels
+// of a row; the pieces lie [channel][row], so a warp reads whole lines.
 template <typename T, int D, KvKind kKind>
 __global__ void __launch_bounds__(kTileRows) joinTilesKernel(const Args a, int n_cta) {
   tc::pdlTrigger();
@@ -984,40 +987,48 @@ __global__ void __launch_bounds__(kTileRows) joinTilesKernel(const Args a, int n
   const Cut cut = cuts[c];
   if (cut.tile_at < 0 || (c > 0 && cuts[c - 1].tile_at == cut.tile_at)) return;
   const Sequence q = sequence<kKind>(a, cut.seq);
-  const int row = threadIdx.x;
+  const int row = threadIdx.x, grp = blockIdx.y * kJoinGroups;
   const int r = cut.tile * kTileRows + row;
   if (r >= q.nq * a.group) return;
+  // The first piece is the last of CTA c - 1, the others are first pieces.
+  float m = -INFINITY, l = 0.0f, x[kJoinGroups][8] = {};
+  auto add = [&](int part) {
+    const float* p = partials + static_cast<size_t>(part) * partialFloats(D);
+    float4 y[kJoinGroups][2];
+#pragma unroll
+    for (int g = 0; g < kJoinGroups; ++g) {
+      y[g][0] = __ldcg(reinterpret_cast<const float4*>(p) + (2 * (grp + g)) * kTileRows + row);
+      y[g][1] = __ldcg(reinterpret_cast<const float4*>(p) + (2 * (grp + g) + 1) * kTileRows + row);
+    }
+    const float pm = __ldcg(p + kTileRows * D + row), pl = __ldcg(p + kTileRows * D + kTileRows + row);
+    const float m_new = fmaxf(m, pm);
+    const float f = m == m_new ? 1.0f : exp2Approx(m - m_new), w = pm == m_new ? 1.0f : exp2Approx(pm - m_new);
+    m = m_new;
+    l = l * f + pl * w;
+#pragma unroll
+    for (int g = 0; g < kJoinGroups; ++g) {
+      const float z[8] = {y[g][0].x, y[g][0].y, y[g][0].z, y[g][0].w, y[g][1].x, y[g][1].y, y[g][1].z, y[g][1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[g][e] = x[g][e] * f + z[e] * w;
+    }
+  };
+  add(2 * (c - 1) + 1);
+  int from = cut.jb;
+  for (int d = c; d < n_cta; ++d) {
+    const bool more = d + 1 < n_cta && cuts[d + 1].tile_at == cut.tile_at;
+    const int to = more ? cuts[d + 1].jb : cut.blocks;
+    if (to > from) add(2 * d);
+    from = to;
+    if (!more) break;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int token = r / a.group;
   const int h = cut.head * a.group + r - token * a.group;
-  for (int grp = blockIdx.y; grp < D / 8; grp += gridDim.y) {
-    // The first piece is the last of CTA c - 1, the others are first pieces.
-    float m = -INFINITY, l = 0.0f, x[8] = {};
-    auto add = [&](int part) {
-      const float* p = partials + static_cast<size_t>(part) * partialFloats(D);
-      const float pm = p[kTileRows * D + row], pl = p[kTileRows * D + kTileRows + row];
-      const float4 u = reinterpret_cast<const float4*>(p)[(2 * grp) * kTileRows + row];
-      const float4 v = reinterpret_cast<const float4*>(p)[(2 * grp + 1) * kTileRows + row];
-      const float m_new = fmaxf(m, pm);
-      const float f = m == m_new ? 1.0f : exp2Approx(m - m_new), g = pm == m_new ? 1.0f : exp2Approx(pm - m_new);
-      m = m_new;
-      l = l * f + pl * g;
-      const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] * f + y[e] * g;
-    };
-    add(2 * (c - 1) + 1);
-    int from = cut.jb;
-    for (int d = c; d < n_cta; ++d) {
-      const bool more = d + 1 < n_cta && cuts[d + 1].tile_at == cut.tile_at;
-      const int to = more ? cuts[d + 1].jb : cut.blocks;
-      if (to > from) add(2 * d);
-      from = to;
-      if (!more) break;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  for (int g = 0; g < kJoinGroups; ++g) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = l == 0.0f ? 0.0f : x[e] * inv;
-    *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(x);
+    for (int e = 0; e < 8; ++e) x[g][e] = l == 0.0f ? 0.0f : x[g][e] * inv;
+    *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp + g)) = pack8<T>(x[g]);
   }
 }
 
@@ -1043,10 +1054,7 @@ cudaError_t launchOne(const Args& a, cudaStream_t s) {
   prof::countLaunch(prof::kAttention, 2);
   e = launchPdl(attentionTilesKernel<T, D, kKind>, dim3(ctas), dim3(kThreads), Geo<D>::kSmem, s, a);
   if (e != cudaSuccess) return e;
-  // Many tiles are cut into two or three pieces each, few into many: those
-  // are joined by more CTAs.
-  const long long tiles = (static_cast<long long>(a.q_rows) * a.group / kTileRows + 1) * a.kv_heads;
-  return launchPdl(joinTilesKernel<T, D, kKind>, dim3(ctas, tiles >= ctas ? 2 : D / 8), dim3(kTileRows), 0, s, a, ctas);
+  return launchPdl(joinTilesKernel<T, D, kKind>, dim3(ctas, D / 8 / kJoinGroups), dim3(kTileRows), 0, s, a, ctas);
 }
 
 template <typename T, int D>
