@@ -14,15 +14,17 @@
 //                   fp32, P = 2^(s - m) rounded to the element type over the
 //                   scores' own TMEM columns. O is rescaled only when a row's
 //                   maximum grows by more than 2^8. After the last block, O / l.
-//   warps 8-11      loads: Q, K and V rows into 128-byte swizzled tiles of 64
-//                   channels [row][64], which lanes that take rows (planar
-//                   sources, pages) and lanes that take groups of channels
-//                   (row-major sources) both fill without bank conflicts; K and
-//                   V in four stages of 128 rows. 16-bit rows by cp.async, which
-//                   takes any strides, pages that end inside a block and zero
-//                   fill of keys that nobody sees, and arrives on the stage's
-//                   barrier by itself; e4m3 rows through registers, where they
-//                   become the element type (exact in bf16).
+//   warps 8-11      loads of Q, K and V rows, K and V in four stages of 128 rows.
+//                   Two layouts in shared memory, each the one that its source
+//                   fills line by line (the other way round the copies take
+//                   eight times the shared-memory cycles and hold up the
+//                   softmax): planar sources and pages as [group of 8
+//                   channels][row][16 B], K and V by bulk copies of whole
+//                   groups; row-major sources as rows of 64 channels with the
+//                   128-byte swizzle, by cp.async, which takes any strides. e4m3
+//                   rows pass through registers, where they become the element
+//                   type (exact in bf16). Values of keys that nobody sees are
+//                   zeroed; their scores are masked.
 //   warps 12, 15    MMA issue for half 0 and 1: S = Q K^T, then for each block
 //                   O += P V (its first 64 keys as soon as they are there) and
 //                   the next block's scores, across tiles too. One warp for
@@ -61,6 +63,7 @@ constexpr int kItems = 4;        // work items in flight between the roles
 constexpr int kLoadWarps = 4;
 constexpr int kThreads = 512;
 constexpr uint32_t kChunk = kKeys * 128;      // 128 rows of 64 channels
+constexpr uint32_t kPlane = kKeys * 16;       // 128 rows of 8 channels
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
 constexpr float kGrowLog2 = 8.0f;
@@ -221,29 +224,40 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smemU32(bar)) : "memory");
 }
 
-// Operand descriptors. One K step is 16 channels or keys. Q and K are K-major:
-// rows of 128 bytes in groups of 8 (1,024 bytes apart), a step 32 bytes on, 64
-// channels to a chunk. V is MN-major: a step is two groups of 8 keys 1,024
-// bytes apart, 64 channels of the output to a chunk.
-__device__ __forceinline__ uint64_t keyDesc(uint32_t addr) { return smemDesc(addr, 16, 1024, kLayoutSw128); }
-__device__ __forceinline__ uint64_t valueDesc(uint32_t addr) { return smemDesc(addr, kChunk, 1024, kLayoutSw128); }
+// Operand descriptors and the distance of K steps (16 channels or keys) in
+// them. Either layout holds 64 channels of 128 rows in 16 KB.
+//   Q, K (K-major)   planar: groups of 8 rows 128 B apart, groups of channels
+//                    2 KB, a step 4 KB; swizzled: rows of 128 B, a step 32 B.
+//   V (MN-major)     planar: groups of 8 keys 128 B apart, of channels 2 KB, a
+//                    step 256 B; swizzled: groups of 8 keys 1 KB apart, a step
+//                    2 KB, 64 channels to a chunk.
+struct Operand {
+  uint64_t desc;
+  uint32_t step;
+};
+__device__ __forceinline__ Operand keyOperand(uint32_t addr, bool planar) {
+  return planar ? Operand{smemDesc(addr, kPlane, 128, kLayoutNone), 2 * kPlane >> 4} : Operand{smemDesc(addr, 16, 1024, kLayoutSw128), 32 >> 4};
+}
+__device__ __forceinline__ Operand valueOperand(uint32_t addr, bool planar) {
+  return planar ? Operand{smemDesc(addr, 128, kPlane, kLayoutNone), 256 >> 4} : Operand{smemDesc(addr, kChunk, 1024, kLayoutSw128), 2048 >> 4};
+}
 
 template <int D>
-__device__ __forceinline__ void issueScores(uint32_t d, uint64_t q, uint64_t k, uint32_t id) {
-  mmaScores<0>(d, q, k, id);
+__device__ __forceinline__ void issueScores(uint32_t d, const Operand& q, uint64_t k, uint32_t k_step, uint32_t id) {
+  mmaScores<0>(d, q.desc, k, id);
 #pragma unroll
   for (int ks = 1; ks < D / 16; ++ks) {
-    const uint32_t at = ((ks / 4) * kChunk + (ks % 4) * 32) >> 4;
-    mmaScores<1>(d, q + at, k + at, id);
+    const uint32_t chunk = (ks / 4) * (kChunk >> 4);
+    mmaScores<1>(d, q.desc + (chunk + (ks % 4) * q.step), k + (chunk + (ks % 4) * k_step), id);
   }
 }
 
 // Steps kFirst .. kFirst + 3 of a block's 8, as far as it has keys.
 template <int kFirst>
-__device__ __forceinline__ void issueValues(uint32_t d, uint32_t p, uint64_t v, uint32_t id, int steps, bool add) {
+__device__ __forceinline__ void issueValues(uint32_t d, uint32_t p, uint64_t v, uint32_t v_step, uint32_t id, int steps, bool add) {
 #pragma unroll
   for (int ks = kFirst; ks < kFirst + 4; ++ks) {
-    if (ks < steps) mmaValues(d, p + ks * 8, v + ks * (2048 >> 4), id, ks > kFirst || add ? 1u : 0u);
+    if (ks < steps) mmaValues(d, p + ks * 8, v + ks * v_step, id, ks > kFirst || add ? 1u : 0u);
   }
 }
 
@@ -302,6 +316,13 @@ __device__ __forceinline__ void hide(uint32_t (&s)[64], int lim, uint32_t bad) {
 
 __device__ __forceinline__ void copyAsync16(uint32_t dst, const void* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+// `bytes` of a bulk copy, and one arrival of this thread that waits for them.
+__device__ __forceinline__ void copyBulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  mbarExpectTx(bar, bytes);
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(smemU32(bar))
+               : "memory");
 }
 // One arrival of this thread on `bar` once its earlier copyAsync16 have landed.
 __device__ __forceinline__ void copyArrive(uint64_t* bar) {
@@ -411,6 +432,9 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   tcFenceAfter();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   int* err = a.error_flag;
+  // Layouts in shared memory.
+  const bool q_planar = a.q.row_stride == 16;
+  const bool k_planar = kKind != kPacked16 || a.k.row_stride == 16, v_planar = kKind != kPacked16 || a.v.row_stride == 16;
 
   if (warp >= 12) {
     if (warp == 12 || warp == 15) {
@@ -418,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       auto uniform = [](int x) { return __reduce_max_sync(0xffffffffu, x); };  // the same in every lane, and known to be
       const int t = uniform(warp == 12 ? 0 : 1);
       const uint32_t idesc_o = idesc(kFmt, D, true);
-      const uint64_t q_desc = keyDesc(q_s + t * G::kTileBytes), k_desc = keyDesc(kv_s), v_desc = valueDesc(kv_s);
+      const Operand q_op = keyOperand(q_s + t * G::kTileBytes, q_planar), k_op = keyOperand(kv_s, k_planar), v_op = valueOperand(kv_s, v_planar);
       const uint32_t s_at = uniform(tmem) + t * kKeys, o_at = uniform(tmem) + kOCol + t * D;
       struct Cursor {
         int item, halves, jb, je, lim;  // the piece of work
@@ -459,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           ++sc.block;
           ++sc.j;
           if (electOne()) {
-            issueScores<D>(s_at, q_desc, k_desc + stage * (G::kTileBytes >> 4), idesc(kFmt, (keys + 15) & ~15, false));
+            issueScores<D>(s_at, q_op, k_op.desc + stage * (G::kTileBytes >> 4), k_op.step, idesc(kFmt, (keys + 15) & ~15, false));
             commit(&sm.s_full[t]);
             commit(&sm.kv_empty[stage]);
             if (sc.j == sc.je) commit(&sm.q_empty[t]);
@@ -481,14 +505,14 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           if (!ok) break;
           tcFenceAfter();
           const int steps = (min(kKeys, max(pv.lim - pv.j * kKeys, 1)) + 15) >> 4;
-          const uint64_t v = v_desc + stage * (G::kTileBytes >> 4);
-          if (electOne()) issueValues<0>(o_at, s_at, v, idesc_o, steps, pv.j > pv.jb);
+          const uint64_t v = v_op.desc + stage * (G::kTileBytes >> 4);
+          if (electOne()) issueValues<0>(o_at, s_at, v, v_op.step, idesc_o, steps, pv.j > pv.jb);
           __syncwarp();
           ok = wait(&sm.p_full[t], done & 1, sm, err, 58);
           if (!ok) break;
           tcFenceAfter();
           if (electOne()) {
-            issueValues<4>(o_at, s_at, v, idesc_o, steps, true);
+            issueValues<4>(o_at, s_at, v, v_op.step, idesc_o, steps, true);
             commit(&sm.pv_done[t]);
             commit(&sm.kv_empty[stage]);
           }
@@ -642,17 +666,13 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
     const int p_lane = lane % kPlanes;
     const int r_lane = w * kRowsAtOnce + lane / kPlanes;
     static_assert(kRowStep % 8 == 0, "a lane's rows have one place in the swizzle");
-    // Byte of group p of row r in a tile: chunk p/8, row r, 16-byte column p%8 ^ r%8.
-    uint32_t put[kWarpPlanes];
-#pragma unroll
-    for (int p = 0; p < kWarpPlanes; ++p) {
-      const int plane = w * kWarpPlanes + p;
-      put[p] = (plane >> 3) * kChunk + lane * 128 + (((plane & 7) ^ (lane & 7)) << 4);
-    }
+    // A lane's place in the swizzled layout: chunk p/8, row r, 16-byte column p%8 ^ r%8.
     const uint32_t put_rows = (p_lane >> 3) * kChunk + r_lane * 128 + (((p_lane & 7) ^ (r_lane & 7)) << 4);
+    const int thread = w * 32 + lane;
     bool ok = true;
     int n = 0;             // key blocks so far
     int used[2] = {0, 0};  // times that Q's halves were loaded
+    uint32_t in_flight = 0;  // by stage: this thread's last bulk copy, and the parity of its phase
     for (int i = 0; ok; ++i) {
       const int slot = i % kItems;
       ok = wait(&sm.item_full[slot], (i / kItems) & 1, sm, err, 52);
@@ -693,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
               const unsigned char* src = rowOf(in ? t * kHalf + rr + lane : 0, w * kWarpPlanes);
 #pragma unroll
               for (int p = 0; p < kWarpPlanes; ++p) {
-                copyAsync16(dst + put[p] + rr * 128, src, in);
+                copyAsync16(dst + (w * kWarpPlanes + p) * kPlane + (rr + lane) * 16, src, in);
                 src += a.q.plane_stride;
               }
             }
@@ -713,18 +733,12 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         if (j + 1 < it.je) page_next = pagesOf(j + 1);
         if (kKind != kPacked16 && page < 0) reportIndex(err, FPK_ERROR_PAGE);
         const int lim = it.lim - j * kKeys;  // rows of the block that somebody sees
-        // Paged: offsets of this lane's four rows, the same in keys and values.
-        long long off[4];
-        bool in[4];
-        if constexpr (kKind != kPacked16) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int rr = c * 32 + lane;
-            const int pg = __shfl_sync(0xffffffffu, page, rr >> 4);
-            in[c] = rr < lim && pg >= 0;
-            off[c] = in[c] ? it.head * a.k.head_stride + pg * a.page_stride + ((j * kKeys + rr) & ((1 << a.page_shift) - 1)) * 16LL : 0;
-          }
-        }
+        // Paged: rows of a page in the block, and the page of this thread's copy
+        // (group `plane` of piece `piece`) and of its row.
+        const int piece_rows = kKind == kPacked16 ? kKeys : min(1 << a.page_shift, kKeys);
+        const int plane = thread % kPlanes, piece = thread / kPlanes;
+        const int page_copy = __shfl_sync(0xffffffffu, page, min(piece * piece_rows >> 4, 7));
+        const int page_row = __shfl_sync(0xffffffffu, page, thread >> 4);
         for (int side = 0; side < 2 && ok; ++side) {
           // Q after the first keys: its room is free only after the last tile's last scores.
           if (side == 1 && j == it.jb) loadQ();
@@ -734,57 +748,46 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           const fpk_heads_t& v = side == 0 ? a.k : a.v;
           const unsigned char* data = static_cast<const unsigned char*>(v.data);
           if constexpr (kKind == kPagedE4m3) {
-            // Records in flight before there is room for them.
-            constexpr int kWarpRecords = kPlanes / 2 / kLoadWarps;  // of a row: 2 or 1
+            // A thread to a row: its records are in flight before there is room.
             const float* scales = side == 0 ? a.k_scale : a.v_scale;
-            uint4 codes[4][kWarpRecords];
-            float sc[4];
+            const int r = (j * kKeys + thread) & ((1 << a.page_shift) - 1);
+            const bool in = thread < lim && page_row >= 0;
+            const unsigned char* src = data + (in ? it.head * v.head_stride + page_row * a.page_stride + r * 16LL : 0);
+            uint4 codes[kPlanes / 2];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int rr = c * 32 + lane;
-              const int pg = __shfl_sync(0xffffffffu, page, rr >> 4);
-              sc[c] = in[c] ? __ldg(scales + (((static_cast<long long>(pg) * a.kv_heads + it.head) << a.page_shift) +
-                                              ((j * kKeys + rr) & ((1 << a.page_shift) - 1))))
-                            : 0.0f;
-#pragma unroll
-              for (int p = 0; p < kWarpRecords; ++p) {
-                codes[c][p] = in[c] ? __ldg(reinterpret_cast<const uint4*>(data + off[c] + (w * kWarpRecords + p) * v.plane_stride))
-                                    : make_uint4(0, 0, 0, 0);
-              }
-            }
+            for (int p = 0; p < kPlanes / 2; ++p) codes[p] = in ? __ldg(reinterpret_cast<const uint4*>(src + p * v.plane_stride)) : make_uint4(0, 0, 0, 0);
+            const float scale = in ? __ldg(scales + (((static_cast<long long>(page_row) * a.kv_heads + it.head) << a.page_shift) + r)) : 0.0f;
             if (n >= 2) ok = wait(&sm.kv_empty[stage], ((n >> 1) - 1) & 1, sm, err, 54);
             if (!ok) break;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-#pragma unroll
-              for (int p = 0; p < kWarpRecords; ++p) {
-                uint4 out[2];
-                dequantise16<T>(codes[c][p], sc[c], out);
-                storeShared16(dst + put[2 * p] + c * 4096, out[0]);
-                storeShared16(dst + put[2 * p + 1] + c * 4096, out[1]);
-              }
+            for (int p = 0; p < kPlanes / 2; ++p) {
+              uint4 out[2];
+              dequantise16<T>(codes[p], scale, out);
+              storeShared16(dst + 2 * p * kPlane + thread * 16, out[0]);
+              storeShared16(dst + (2 * p + 1) * kPlane + thread * 16, out[1]);
             }
             mbarArrive(&sm.kv_full[stage]);
           } else {
             if (n >= 2) ok = wait(&sm.kv_empty[stage], ((n >> 1) - 1) & 1, sm, err, 54);
             if (!ok) break;
-            if (kKind == kPaged16 || v.row_stride == 16) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                bool yes;
+            if (side == 0 ? k_planar : v_planar) {
+              // Keys that nobody sees, or on no page, have no values.
+              if (side == 1 && (thread >= lim || (kKind != kPacked16 && page_row < 0))) {
+#pragma unroll 1
+                for (int p = 0; p < kPlanes; ++p) storeShared16(dst + p * kPlane + thread * 16, make_uint4(0, 0, 0, 0));
+              }
+              const int rows_in = min(lim - piece * piece_rows, piece_rows);
+              if (piece * piece_rows < kKeys && rows_in > 0 && (kKind == kPacked16 || page_copy >= 0)) {
                 const unsigned char* src;
-                if constexpr (kKind == kPaged16) {
-                  yes = in[c];
-                  src = data + off[c] + w * kWarpPlanes * v.plane_stride;
+                if constexpr (kKind == kPacked16) {
+                  src = record(v, it.head, static_cast<long long>(it.k0) + j * kKeys, plane);
                 } else {
-                  yes = c * 32 + lane < lim;
-                  src = yes ? record(v, it.head, static_cast<long long>(it.k0) + j * kKeys + c * 32 + lane, w * kWarpPlanes) : data;
+                  src = record(v, it.head, (j * kKeys + piece * piece_rows) & ((1 << a.page_shift) - 1), plane) + page_copy * a.page_stride;
                 }
-#pragma unroll
-                for (int p = 0; p < kWarpPlanes; ++p) {
-                  copyAsync16(dst + put[p] + c * 4096, src, yes);
-                  if (yes) src += v.plane_stride;
-                }
+                copyBulk(dst + plane * kPlane + piece * piece_rows * 16, src, rows_in * 16, &sm.kv_full[stage]);
+                in_flight = (in_flight & ~(17u << stage)) | (1u << stage) | (((n >> 1) & 1u) << (stage + 4));
+              } else {
+                mbarArrive(&sm.kv_full[stage]);
               }
             } else {
               const long long step = kRowStep * v.row_stride;
@@ -795,13 +798,19 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
                 copyAsync16(dst + put_rows + x * kRowStep * 128, yes ? src : data, yes);
                 src += step;
               }
+              copyArrive(&sm.kv_full[stage]);
             }
-            copyArrive(&sm.kv_full[stage]);
           }
         }
       }
     }
     copyDrain();
+    // After an error bulk copies may still be under way (otherwise all were waited for).
+    if (!ok) {
+      for (int stage = 0; stage < kStages; ++stage) {
+        if ((in_flight >> stage) & 1u) drainBar(&sm.kv_full[stage], (in_flight >> (stage + 4)) & 1u);
+      }
+    }
   } else {
     // ---------------- softmax and output ----------------
     const int t = warp >> 2;
