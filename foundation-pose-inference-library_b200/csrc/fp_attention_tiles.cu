@@ -69,6 +69,9 @@ constexpr uint32_t kOCol = 256;
 constexpr float kGrowLog2 = 8.0f;
 constexpr int kTileCost = 384;   // a tile's work beside its keys, in keys
 constexpr int kMinShare = 256;   // keys
+// Smallest piece of a page, in rows, for bulk copies: their issue takes some 70
+// cycles each whatever the size.
+constexpr int kBulkRows = 64;
 constexpr int kSnap = 8;         // a tile shorter than 1/8 share is not cut
 
 struct Item {
@@ -736,7 +739,8 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         // Paged: rows of a page in the block, and the page of this thread's copy
         // (group `plane` of piece `piece`) and of its row.
         const int piece_rows = kKind == kPacked16 ? kKeys : min(1 << a.page_shift, kKeys);
-        const int plane = thread % kPlanes, piece = thread / kPlanes;
+        const int copy = lane * kLoadWarps + w;  // copies go round the warps, which issue them one by one
+        const int plane = copy % kPlanes, piece = copy / kPlanes;
         const int page_copy = __shfl_sync(0xffffffffu, page, min(piece * piece_rows >> 4, 7));
         const int page_row = __shfl_sync(0xffffffffu, page, thread >> 4);
         for (int side = 0; side < 2 && ok; ++side) {
@@ -771,6 +775,23 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             if (n >= 2) ok = wait(&sm.kv_empty[stage], ((n >> 1) - 1) & 1, sm, err, 54);
             if (!ok) break;
             if (side == 0 ? k_planar : v_planar) {
+              if (kKind == kPaged16 && piece_rows < kBulkRows) {
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                  const int rr = c * 32 + lane;
+                  const int pg = __shfl_sync(0xffffffffu, page, rr >> 4);
+                  const bool yes = rr < lim && pg >= 0;
+                  const unsigned char* src =
+                      yes ? record(v, it.head, (j * kKeys + rr) & ((1 << a.page_shift) - 1), w * kWarpPlanes) + pg * a.page_stride : data;
+#pragma unroll
+                  for (int p = 0; p < kWarpPlanes; ++p) {
+                    copyAsync16(dst + (w * kWarpPlanes + p) * kPlane + rr * 16, src, yes);
+                    if (yes) src += v.plane_stride;
+                  }
+                }
+                copyArrive(&sm.kv_full[stage]);
+                continue;
+              }
               // Keys that nobody sees, or on no page, have no values.
               if (side == 1 && (thread >= lim || (kKind != kPacked16 && page_row < 0))) {
 #pragma unroll 1
