@@ -763,10 +763,18 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             const float scale = in ? __ldg(scales + (((static_cast<long long>(page_row) * a.kv_heads + it.head) << a.page_shift) + r)) : 0.0f;
             if (n >= 2) ok = wait(&sm.kv_empty[stage], ((n >> 1) - 1) & 1, sm, err, 54);
             if (!ok) break;
+            const FastScale<T> fast(scale);
+            const bool usual = scale >= FastScale<T>::low && scale <= FastScale<T>::high;
 #pragma unroll
             for (int p = 0; p < kPlanes / 2; ++p) {
               uint4 out[2];
-              dequantise16<T>(codes[p], scale, out);
+              if (!in || (usual && !hasNan(codes[p]))) {
+                const uint4 c = codes[p];
+                out[0] = make_uint4(fast(c.x), fast(c.x >> 16), fast(c.y), fast(c.y >> 16));
+                out[1] = make_uint4(fast(c.z), fast(c.z >> 16), fast(c.w), fast(c.w >> 16));
+              } else {
+                dequantise16<T>(codes[p], scale, out);
+              }
               storeShared16(dst + 2 * p * kPlane + thread * 16, out[0]);
               storeShared16(dst + (2 * p + 1) * kPlane + thread * 16, out[1]);
             }

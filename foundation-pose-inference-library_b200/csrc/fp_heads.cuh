@@ -78,6 +78,49 @@ __device__ __forceinline__ float largest() {
   return std::is_same<T, __half>::value ? 65504.0f : 3.3895313892515355e38f;
 }
 
+// Whether a record holds NaN: 0x7f without its sign is the one code that 1 carries into bit 7.
+__device__ __forceinline__ bool hasNan(const uint4& c) {
+  const uint32_t m = 0x7f7f7f7fu, one = 0x01010101u;
+  return ((((c.x & m) + one) | ((c.y & m) + one) | ((c.z & m) + one) | ((c.w & m) + one)) & 0x80808080u) != 0;
+}
+
+// Two e4m3 codes times a row's scale in two or five instructions, for scales
+// from `low` to `high` and records without NaN; dequantise16 below takes the
+// others. Exact but for the one rounding that T's range asks for, saturating.
+template <typename T>
+struct FastScale;
+template <>
+struct FastScale<__half> {
+  static constexpr float low = 5.9604644775390625e-8f, high = 32768.0f;  // 2^-24, 2^15: what fp16 holds
+  uint32_t factor;
+  __device__ __forceinline__ explicit FastScale(float scale) {
+    const __half2 h = __float2half2_rn(scale);
+    factor = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t two) const {
+    const uint32_t h = e4m3x2ToHalf2(two);
+    const __half2 top = __half2half2(__ushort_as_half(0x7bff)), v = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&factor));
+    const __half2 r = __hmax2_nan(__hmin2_nan(v, top), __hneg2(top));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+template <>
+struct FastScale<__nv_bfloat16> {
+  static constexpr float low = 7.888609052210118e-31f, high = 3.3230699894622897e35f;  // 2^-100, 2^118: no overflow
+  uint32_t factor;
+  __device__ __forceinline__ explicit FastScale(float scale) { factor = (__float_as_uint(scale) >> 16) * 0x10001u; }
+  __device__ __forceinline__ uint32_t operator()(uint32_t two) const {
+    // The fp16 bits, exponent field shifted into bf16's place, are the value
+    // times 2^-112 (e4m3's subnormal numbers are normal in fp16).
+    const uint32_t h = e4m3x2ToHalf2(two);
+    const uint32_t b = (h & 0x80008000u) | ((h >> 3) & 0x0fff0fffu);
+    const uint32_t back = 0x77807780u;  // 2^112
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&back));
+    const __nv_bfloat162 r = __hmul2(v, *reinterpret_cast<const __nv_bfloat162*>(&factor));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+
 // One 16-byte e4m3 record as two groups of 8 elements of T.
 template <typename T>
 __device__ __forceinline__ void dequantise16(const uint4& codes, float scale, uint4 (&out)[2]) {
