@@ -337,6 +337,15 @@ __device__ __forceinline__ void storeShared16(uint32_t dst, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+// An e4m3 record with NaN or an unusual scale, into two groups of a planar tile.
+template <typename T>
+__device__ __noinline__ void storeRecord(uint32_t dst, uint4 codes, float scale) {
+  uint4 out[2];
+  dequantise16<T>(codes, scale, out);
+  storeShared16(dst, out[0]);
+  storeShared16(dst + kPlane, out[1]);
+}
+
 }  // namespace
 
 template <typename T, int D, KvKind kKind>
@@ -764,19 +773,16 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             if (n >= 2) ok = wait(&sm.kv_empty[stage], ((n >> 1) - 1) & 1, sm, err, 54);
             if (!ok) break;
             const FastScale<T> fast(scale);
-            const bool usual = scale >= FastScale<T>::low && scale <= FastScale<T>::high;
+            const bool usual = !in || (scale >= FastScale<T>::low && scale <= FastScale<T>::high);
 #pragma unroll
             for (int p = 0; p < kPlanes / 2; ++p) {
-              uint4 out[2];
-              if (!in || (usual && !hasNan(codes[p]))) {
-                const uint4 c = codes[p];
-                out[0] = make_uint4(fast(c.x), fast(c.x >> 16), fast(c.y), fast(c.y >> 16));
-                out[1] = make_uint4(fast(c.z), fast(c.z >> 16), fast(c.w), fast(c.w >> 16));
-              } else {
-                dequantise16<T>(codes[p], scale, out);
-              }
-              storeShared16(dst + 2 * p * kPlane + thread * 16, out[0]);
-              storeShared16(dst + (2 * p + 1) * kPlane + thread * 16, out[1]);
+              const uint2 x = fast(codes[p].x), y = fast(codes[p].y), z = fast(codes[p].z), w4 = fast(codes[p].w);
+              storeShared16(dst + 2 * p * kPlane + thread * 16, make_uint4(x.x, x.y, y.x, y.y));
+              storeShared16(dst + (2 * p + 1) * kPlane + thread * 16, make_uint4(z.x, z.y, w4.x, w4.y));
+            }
+#pragma unroll
+            for (int p = 0; p < kPlanes / 2; ++p) {
+              if (!usual || hasNan(codes[p])) storeRecord<T>(dst + 2 * p * kPlane + thread * 16, codes[p], scale);
             }
             mbarArrive(&sm.kv_full[stage]);
           } else {

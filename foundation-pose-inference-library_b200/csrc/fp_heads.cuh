@@ -84,40 +84,40 @@ __device__ __forceinline__ bool hasNan(const uint4& c) {
   return ((((c.x & m) + one) | ((c.y & m) + one) | ((c.z & m) + one) | ((c.w & m) + one)) & 0x80808080u) != 0;
 }
 
-// Two e4m3 codes times a row's scale in two or five instructions, for scales
-// from `low` to `high` and records without NaN; dequantise16 below takes the
-// others. Exact but for the one rounding that T's range asks for, saturating.
+// The four e4m3 codes of a word times a row's scale, as two pairs of T, for
+// scales from `low` to `high` (products within T's range) and words without
+// NaN; dequantise16 below takes the others. One rounding at most.
 template <typename T>
 struct FastScale;
 template <>
 struct FastScale<__half> {
-  static constexpr float low = 5.9604644775390625e-8f, high = 32768.0f;  // 2^-24, 2^15: what fp16 holds
+  static constexpr float low = 5.9604644775390625e-8f, high = 128.0f;  // 2^-24: what fp16 holds; 448 * 2^7 < 65504
   uint32_t factor;
   __device__ __forceinline__ explicit FastScale(float scale) {
     const __half2 h = __float2half2_rn(scale);
     factor = *reinterpret_cast<const uint32_t*>(&h);
   }
-  __device__ __forceinline__ uint32_t operator()(uint32_t two) const {
+  __device__ __forceinline__ uint32_t pair(uint32_t two) const {
     const uint32_t h = e4m3x2ToHalf2(two);
-    const __half2 top = __half2half2(__ushort_as_half(0x7bff)), v = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&factor));
-    const __half2 r = __hmax2_nan(__hmin2_nan(v, top), __hneg2(top));
-    return *reinterpret_cast<const uint32_t*>(&r);
+    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&factor));
+    return *reinterpret_cast<const uint32_t*>(&v);
   }
+  __device__ __forceinline__ uint2 operator()(uint32_t four) const { return make_uint2(pair(four), pair(four >> 16)); }
 };
 template <>
 struct FastScale<__nv_bfloat16> {
-  static constexpr float low = 7.888609052210118e-31f, high = 3.3230699894622897e35f;  // 2^-100, 2^118: no overflow
+  static constexpr float low = 7.888609052210118e-31f, high = 128.0f;  // 2^-100, 2^7: scale * 2^120 is a normal number
   uint32_t factor;
-  __device__ __forceinline__ explicit FastScale(float scale) { factor = (__float_as_uint(scale) >> 16) * 0x10001u; }
-  __device__ __forceinline__ uint32_t operator()(uint32_t two) const {
-    // The fp16 bits, exponent field shifted into bf16's place, are the value
-    // times 2^-112 (e4m3's subnormal numbers are normal in fp16).
-    const uint32_t h = e4m3x2ToHalf2(two);
-    const uint32_t b = (h & 0x80008000u) | ((h >> 3) & 0x0fff0fffu);
-    const uint32_t back = 0x77807780u;  // 2^112
-    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&back));
-    const __nv_bfloat162 r = __hmul2(v, *reinterpret_cast<const __nv_bfloat162*>(&factor));
-    return *reinterpret_cast<const uint32_t*>(&r);
+  __device__ __forceinline__ explicit FastScale(float scale) { factor = (__float_as_uint(scale * 1.329227995784916e36f) >> 16) * 0x10001u; }
+  // Sign, exponent and mantissa moved to bf16's places are the value times
+  // 2^-120 (subnormal numbers too); the factor holds the 2^120.
+  __device__ __forceinline__ uint32_t pair(uint32_t codes_high) const {
+    const uint32_t b = ((codes_high >> 4) & 0x07f007f0u) | (codes_high & 0x80008000u);
+    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&factor));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  __device__ __forceinline__ uint2 operator()(uint32_t four) const {
+    return make_uint2(pair(__byte_perm(four, 0, 0x1404)), pair(__byte_perm(four, 0, 0x3424)));
   }
 };
 
