@@ -740,6 +740,24 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         }
       };
 
+      // e4m3: this thread's row of a tile, records and scale.
+      uint4 next_codes[kPlanes / 2];
+      float next_scale = 0.0f;
+      bool next_in = false;
+      auto fetch = [&](int j, int side, int page) {
+        const fpk_heads_t& v = side == 0 ? a.k : a.v;
+        const int r = (j * kKeys + thread) & ((1 << a.page_shift) - 1);
+        next_in = j * kKeys + thread < it.lim && page >= 0;
+        const unsigned char* src = static_cast<const unsigned char*>(v.data) + (next_in ? it.head * v.head_stride + page * a.page_stride + r * 16LL : 0);
+#pragma unroll
+        for (int p = 0; p < kPlanes / 2; ++p) {
+          next_codes[p] = next_in ? __ldg(reinterpret_cast<const uint4*>(src + p * v.plane_stride)) : make_uint4(0, 0, 0, 0);
+        }
+        const float* scales = side == 0 ? a.k_scale : a.v_scale;
+        next_scale = next_in ? __ldg(scales + (((static_cast<long long>(page) * a.kv_heads + it.head) << a.page_shift) + r)) : 0.0f;
+      };
+      if constexpr (kKind == kPagedE4m3) fetch(it.jb, 0, __shfl_sync(0xffffffffu, page_next, thread >> 4));
+
       for (int j = it.jb; j < it.je && ok; ++j, ++n) {
         const int page = page_next;
         if (j + 1 < it.je) page_next = pagesOf(j + 1);
@@ -761,15 +779,15 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           const fpk_heads_t& v = side == 0 ? a.k : a.v;
           const unsigned char* data = static_cast<const unsigned char*>(v.data);
           if constexpr (kKind == kPagedE4m3) {
-            // A thread to a row: its records are in flight before there is room.
-            const float* scales = side == 0 ? a.k_scale : a.v_scale;
-            const int r = (j * kKeys + thread) & ((1 << a.page_shift) - 1);
-            const bool in = thread < lim && page_row >= 0;
-            const unsigned char* src = data + (in ? it.head * v.head_stride + page_row * a.page_stride + r * 16LL : 0);
+            // A thread to a row. The next tile's records are on their way while
+            // this one's are converted.
             uint4 codes[kPlanes / 2];
+            const float scale = next_scale;
+            const bool in = next_in;
 #pragma unroll
-            for (int p = 0; p < kPlanes / 2; ++p) codes[p] = in ? __ldg(reinterpret_cast<const uint4*>(src + p * v.plane_stride)) : make_uint4(0, 0, 0, 0);
-            const float scale = in ? __ldg(scales + (((static_cast<long long>(page_row) * a.kv_heads + it.head) << a.page_shift) + r)) : 0.0f;
+            for (int p = 0; p < kPlanes / 2; ++p) codes[p] = next_codes[p];
+            const int page_after = __shfl_sync(0xffffffffu, side == 0 ? page : page_next, thread >> 4);
+            if (side == 0 || j + 1 < it.je) fetch(j + side, 1 - side, page_after);
             if (n >= 2) ok = wait(&sm.kv_empty[stage], ((n >> 1) - 1) & 1, sm, err, 54);
             if (!ok) break;
             const FastScale<T> fast(scale);
