@@ -8,9 +8,9 @@
 // operations), so the pass is bound by memory. Two mappings of lanes, by the
 // layout, because a warp must touch whole 128-byte lines:
 //   rows    16-byte groups of a head lie side by side (row-major): lanes take
-//           the groups, a warp takes one token and walks its heads with the
-//           token's angles in registers; the norm is a sum over the head's
-//           lanes, the partner half of a pair comes by shuffle.
+//           two groups each, a warp takes one token and walks its heads with
+//           the token's angles in registers; the norm is a sum over the head's
+//           lanes.
 //   planar  rows of a group lie side by side (row_stride 16): lanes take 32
 //           rows, a thread owns its row's whole head and reads it twice (the
 //           second time from L1) instead of holding it; the angles of the 32
@@ -54,6 +54,10 @@ __device__ __forceinline__ float2 turn(int position, float inv_freq, float scale
 constexpr int kRowsWarps = 4;
 constexpr int kBatch = 4;  // heads in flight per lane group
 
+// A lane holds two groups of a head: the two that a pair of channels lies in
+// (half layout), so that nothing is exchanged, or two neighbours. The norm's
+// weight is folded into the angles once per token: with u = w c and v = w' s a
+// pair costs a product, an fma and the product with r.
 template <typename T>
 __global__ void __launch_bounds__(kRowsWarps * 32) rotaryRowsKernel(const Args a, int lanes) {
   tc::pdlTrigger();
@@ -63,41 +67,29 @@ __global__ void __launch_bounds__(kRowsWarps * 32) rotaryRowsKernel(const Args a
   if (row >= a.rows) return;
   const int slots = 32 / lanes;  // heads that a warp holds side by side
   const int slot = lane / lanes;
-  const int g = lane - slot * lanes;
-  const bool active = g < a.groups;
+  const int k = lane - slot * lanes;  // pair of groups
   const int half_groups = a.rotary_dim >> 4;  // groups of half the rotated part
-  const bool rotated = g < 2 * half_groups;
+  const bool rotated = k < half_groups;
+  const bool halves = !a.interleaved && rotated;
+  const int ga = halves ? k : 2 * k;
+  const int gb = halves ? k + half_groups : 2 * k + 1;
+  const bool has_a = ga < a.groups, has_b = gb < a.groups;
 
-  // Angles of this lane's 8 channels: [4] pairs if interleaved; otherwise lanes
-  // g and g + half_groups need the same 8, compute 4 each and exchange them.
+  // cos and sin of channel i of the pair's groups (half layout: the same in
+  // both), or of the four pairs of each.
   float c[8], s[8];
-  int partner = lane;
-  if (a.rotary_dim > 0) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = 1.0f;
+    s[i] = 0.0f;
+  }
+  if (rotated) {
     const int position = __ldg(a.positions + row);
-    if (a.interleaved) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 cs = rotated ? turn(position, __ldg(a.inv_freq + g * 4 + i), a.scale) : make_float2(1.0f, 0.0f);
-        c[i] = cs.x;
-        s[i] = cs.y;
-      }
-    } else {
-      const bool upper = g >= half_groups;
-      if (rotated) partner = upper ? lane - half_groups : lane + half_groups;
-      const int first = (upper ? g - half_groups : g) * 8;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 cs = rotated ? turn(position, __ldg(a.inv_freq + first + (upper ? 4 : 0) + i), a.scale) : make_float2(1.0f, 0.0f);
-        const float oc = __shfl_sync(0xffffffffu, cs.x, partner);
-        const float os = __shfl_sync(0xffffffffu, cs.y, partner);
-        c[i] = upper ? oc : cs.x;
-        c[4 + i] = upper ? cs.x : oc;
-        s[i] = upper ? os : cs.y;
-        s[4 + i] = upper ? cs.y : os;
-      }
-      // Lower half: a c - b s; upper half: b c + a s.
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = !rotated ? 0.0f : (upper ? s[i] : -s[i]);
+    for (int i = 0; i < 8; ++i) {
+      const float2 cs = turn(position, __ldg(a.inv_freq + k * 8 + i), a.scale);
+      c[i] = cs.x;
+      s[i] = cs.y;
     }
   }
 
@@ -107,66 +99,68 @@ __global__ void __launch_bounds__(kRowsWarps * 32) rotaryRowsKernel(const Args a
     const int n_heads = part == 0 ? a.q_heads : a.kv_heads;
     const float* weight = part == 0 ? a.q_weight : a.k_weight;
     const bool norm = weight != nullptr;
-    float w[8], wp[8];  // this lane's weights and its partner's
+    float wa[8], wb[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = wp[i] = 1.0f;
-    if (norm && active && n_heads > 0) {
-      const int pg = partner - slot * lanes;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i] = __ldg(weight + g * 8 + i);
-        wp[i] = __ldg(weight + pg * 8 + i);
-      }
+    for (int i = 0; i < 8; ++i) {
+      wa[i] = norm && has_a && n_heads > 0 ? __ldg(weight + ga * 8 + i) : 1.0f;
+      wb[i] = norm && has_b && n_heads > 0 ? __ldg(weight + gb * 8 + i) : 1.0f;
     }
     const int stride = gridDim.y * slots;
     // Uniform trip count: every lane takes part in the shuffles.
     for (int h0 = blockIdx.y * slots; h0 < n_heads; h0 += stride * kBatch) {
-      uint4 raw[kBatch];
+      uint4 raw[kBatch][2];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const int h = h0 + b * stride + slot;
-        raw[b] = make_uint4(0, 0, 0, 0);
-        if (active && h < n_heads) raw[b] = *reinterpret_cast<const uint4*>(record(in, h, row, g));
+        raw[b][0] = raw[b][1] = make_uint4(0, 0, 0, 0);
+        if (has_a && h < n_heads) raw[b][0] = *reinterpret_cast<const uint4*>(record(in, h, row, ga));
+        if (has_b && h < n_heads) raw[b][1] = *reinterpret_cast<const uint4*>(record(in, h, row, gb));
       }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         if (h0 + b * stride >= n_heads) break;  // warp-uniform
         const int h = h0 + b * stride + slot;
-        float x[8];
-        unpack8<T>(raw[b], x);
+        float x[8], y[8];
+        unpack8<T>(raw[b][0], x);
+        unpack8<T>(raw[b][1], y);
         float r = 1.0f;
         if (norm) {
-          float sum = 0.0f;
+          float sum = 0.0f, more = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+          for (int i = 0; i < 8; ++i) {
+            sum = fmaf(x[i], x[i], sum);
+            more = fmaf(y[i], y[i], more);
+          }
+          sum += more;
           for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
           r = rsqrtf(fmaf(sum, a.inv_dim, a.eps));
         }
-        float y[8];
-        if (a.rotary_dim > 0 && !a.interleaved) {
-          uint4 other;
-          other.x = __shfl_sync(0xffffffffu, raw[b].x, partner);
-          other.y = __shfl_sync(0xffffffffu, raw[b].y, partner);
-          other.z = __shfl_sync(0xffffffffu, raw[b].z, partner);
-          other.w = __shfl_sync(0xffffffffu, raw[b].w, partner);
-          float p[8];
-          unpack8<T>(other, p);
-          // A channel that is not rotated must not meet its own infinity times 0.
+        if (!rotated) {  // its own branch: an infinity must not meet 0 sin
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = rotated ? (x[i] * r * w[i]) * c[i] + (p[i] * r * wp[i]) * s[i] : x[i] * r * w[i];
+          for (int i = 0; i < 8; ++i) {
+            x[i] *= wa[i] * r;
+            y[i] *= wb[i] * r;
+          }
+        } else if (halves) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float u = x[i] * wa[i], v = y[i] * wb[i];
+            x[i] = (u * c[i] - v * s[i]) * r;
+            y[i] = (v * c[i] + u * s[i]) * r;
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = x[i] * r * w[i];
-          if (a.rotary_dim > 0 && rotated) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float u = y[2 * i], v = y[2 * i + 1];
-              y[2 * i] = u * c[i] - v * s[i];
-              y[2 * i + 1] = v * c[i] + u * s[i];
-            }
+          for (int i = 0; i < 4; ++i) {
+            const float u = x[2 * i] * wa[2 * i], v = x[2 * i + 1] * wa[2 * i + 1];
+            x[2 * i] = (u * c[i] - v * s[i]) * r;
+            x[2 * i + 1] = (v * c[i] + u * s[i]) * r;
+            const float p = y[2 * i] * wb[2 * i], q = y[2 * i + 1] * wb[2 * i + 1];
+            y[2 * i] = (p * c[4 + i] - q * s[4 + i]) * r;
+            y[2 * i + 1] = (q * c[4 + i] + p * s[4 + i]) * r;
           }
         }
-        if (active && h < n_heads) *reinterpret_cast<uint4*>(record(out, h, row, g)) = pack8<T>(y);
+        if (has_a && h < n_heads) *reinterpret_cast<uint4*>(record(out, h, row, ga)) = pack8<T>(x);
+        if (has_b && h < n_heads) *reinterpret_cast<uint4*>(record(out, h, row, gb)) = pack8<T>(y);
       }
     }
   }
@@ -277,7 +271,7 @@ cudaError_t launch(const Args& a, cudaStream_t s) {
     return launchPdl(rotaryPlanarKernel<T>, dim3(blocks, most), dim3(kPlanarWarps * 32), static_cast<size_t>(a.rotary_dim) * 128, s, a);
   }
   int lanes = 1;
-  while (lanes < a.groups) lanes *= 2;
+  while (2 * lanes < a.groups) lanes *= 2;
   const int blocks = (a.rows + kRowsWarps - 1) / kRowsWarps;
   // Few rows: the heads are split over blocks too, so that the GPU fills.
   const int per_warp = (32 / lanes) * kBatch;
