@@ -4,16 +4,16 @@
 //
 // Bound by the keys' and values' bytes, each read once from HBM, so everything
 // serves the stream of loads:
-// * Keys and values go from global memory straight into matrix fragments (mma
-//   m16n8k16, 16 query rows). A contraction does not care for the order of its
-//   index, so the order is chosen such that a thread's 16-byte record is its
-//   fragment: scores contract 8 channels of a record in two products; a
+// * Each warp streams steps of 16 keys through its own ring in shared memory
+//   (cp.async; no barrier between warps), deep enough that some 100 KB an SM are
+//   under way. From there 16-byte records become matrix fragments (mma m16n8k16,
+//   16 query rows) as they are: a contraction does not care for the order of its
+//   index, so scores contract the 8 channels of a record in two products, and a
 //   score column c of 8-column block j stands for key 8j + 4(c%2) + c/2, so that
 //   a thread's four probabilities belong to keys t, 4+t, 8+t, 12+t (t = lane%4)
-//   and its four value records, one of each key and of plane lane/4, need only a
-//   byte permute to become fragments of the second product. No shared
-//   memory and no barrier in the loop; every load instruction covers whole
-//   sectors.
+//   and its four value records, one of each key and of plane lane/4, need only
+//   a byte permute to become fragments of the second product. The planes
+//   of a step are padded so that both readings are free of bank conflicts.
 // * e4m3 records become fp16 (exact) in registers. The key's scale multiplies
 //   its scores; the value's scale v joins the exponent: P' = 2^(s + log2 v - m),
 //   O = sum P' code, l = sum P'/v, so P' is at most 2^8 whatever the scales are
@@ -85,43 +85,61 @@ __device__ __forceinline__ float exp2Approx(float x) {
   return y;
 }
 
-// Keys and values are read once: no room in L1 for them.
-__device__ __forceinline__ uint4 loadOnce16(const void* p) {
+__device__ __forceinline__ void copyAsync16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copyAsync4(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 loadShared16(uint32_t at) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
   return v;
 }
-__device__ __forceinline__ uint2 loadOnce8(const void* p) {
+__device__ __forceinline__ uint2 loadShared8(uint32_t at) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ float loadShared4(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
   return v;
 }
 
-// Shapes of one 16-key step.
+// The four e4m3 codes of a word as two fp16 pairs.
+__device__ __forceinline__ uint2 halves(uint32_t four) {
+  uint2 r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(r.x), "=r"(r.y) : "r"(four));
+  return r;
+}
+
+// Shapes of one 16-key step in a warp's ring.
 template <int D, bool kE4m3>
 struct Step {
-  static constexpr int kKRecords = kE4m3 ? D / 64 : D / 32;  // K records of a thread per 8 keys
-  static constexpr int kVCh = kE4m3 && D == 128 ? 16 : 8;    // channels of a thread's V record
-  static constexpr int kVRecords = D / (8 * kVCh);           // V records of a thread per key
-  static constexpr int kVRegs = kE4m3 ? kVCh / 4 : 4;
-};
-
-template <int D, bool kE4m3>
-struct StepData {
-  uint4 k[2][Step<D, kE4m3>::kKRecords];
-  uint32_t v[Step<D, kE4m3>::kVRecords][4][Step<D, kE4m3>::kVRegs];
-  float ks[4], vs[4];
-  int key0, lim;  // first key, valid keys of the 16
+  static constexpr int kPlanes = kE4m3 ? D / 16 : D / 8;
+  static constexpr int kKRecords = kPlanes / 4;               // K records of a thread per 8 keys
+  static constexpr int kVCh = kE4m3 && D == 128 ? 16 : 8;     // channels of a thread's V record
+  static constexpr int kVRecords = D / (8 * kVCh);            // V records of a thread per key
+  static constexpr int kKPlane = 16 * 16 + 16, kVPlane = 16 * 16 + 64;
+  static constexpr int kV = kPlanes * kKPlane;                // byte of V
+  static constexpr int kScales = kV + kPlanes * kVPlane;      // byte of the scales, keys' then values'
+  static constexpr int kBytes = kScales + (kE4m3 ? 128 : 0);
+  // Three CTAs to an SM share its 227 KB.
+  static constexpr int kDepth = 75776 / (kWarps * kBytes) < 5 ? 75776 / (kWarps * kBytes) : 5;
+  static constexpr int kRing = kWarps * kDepth * kBytes;
+  static_assert(kDepth >= 2 && kRing >= kWarps * kStreamRows * (D + 4) * 4, "the outputs' exchange lies over the ring");
 };
 
 }  // namespace
 
 template <typename T, int D, KvKind kKind>
-__global__ void __launch_bounds__(kThreads) attentionStreamKernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args a) {
   constexpr bool kE4m3 = kKind == kPagedE4m3;
   using S = Step<D, kE4m3>;
   using M = std::conditional_t<kE4m3, __half, T>;  // type of the products
-  __shared__ float o_s[kWarps][kStreamRows][D + 4];
+  extern __shared__ __align__(16) unsigned char ring_raw[];
+  auto o_s = reinterpret_cast<float(*)[kStreamRows][D + 4]>(ring_raw);  // [kWarps], once the ring is empty
   __shared__ float ml_s[kWarps][2][kStreamRows];
   __shared__ long long scan_s[kWarps + 1];
   __shared__ long long found_s[2];
@@ -279,88 +297,94 @@ __global__ void __launch_bounds__(kThreads) attentionStreamKernel(const Args a) 
 
     // Steps of 16 keys, one warp after the other, up to the last visible key.
     const int step_end = min(b1 * (kUnitKeys / 16), (last_vis + 15) >> 4);
-    StepData<D, kE4m3> d;
-    const unsigned char* vb = nullptr;
+    const int step_first = b0 * (kUnitKeys / 16) + warp;
+    const uint32_t ring = tc::smemU32(ring_raw) + warp * S::kDepth * S::kBytes;
+    // This lane copies row lane%16 of planes lane/16, 2 + lane/16, ...
+    const int copy_row = lane & 15, copy_plane = lane >> 4;
+    uint32_t bad_steps = 0;  // by ring place: the step's page does not exist
+    int page_next = 0;
     auto pageAt = [&](int step) -> int {
       if constexpr (kKind == kPacked16) return 0;
       return step < step_end ? pageOf(a, seq, step * 16) : 0;
     };
-    auto loadK = [&](int step, int page) {
-      d.key0 = step * 16;
-      d.lim = min(16, last_vis - d.key0);
-      const unsigned char* kb;
-      if constexpr (kKind == kPacked16) {
-        kb = record(a.k, head, static_cast<long long>(q.k0) + d.key0, 0);
-        vb = record(a.v, head, static_cast<long long>(q.k0) + d.key0, 0);
-      } else {
-        if (page < 0) {
-          reportIndex(a.error_flag, FPK_ERROR_PAGE);
-          d.lim = 0;
-          page = 0;
-        }
-        const int r = d.key0 & ((1 << a.page_shift) - 1);
-        kb = record(a.k, head, r, 0) + page * a.page_stride;
-        vb = record(a.v, head, r, 0) + page * a.page_stride;
-        if constexpr (kE4m3) {
-          const long long at = ((static_cast<long long>(page) * a.kv_heads + head) << a.page_shift) + r + t;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool in = 4 * i + t < d.lim;
-            d.ks[i] = in ? __ldg(a.k_scale + at + 4 * i) : 0.0f;
-            d.vs[i] = in ? __ldg(a.v_scale + at + 4 * i) : 1.0f;
+    auto copyStep = [&](int step, int place) {
+      if (step < step_end) {
+        const int key0 = step * 16;
+        bool in = key0 + copy_row < last_vis;
+        const uint32_t to = ring + place * S::kBytes;
+        long long row = 0, page_at = 0;
+        if constexpr (kKind == kPacked16) {
+          row = static_cast<long long>(q.k0) + key0 + copy_row;
+        } else {
+          int page = page_next;
+          page_next = pageAt(step + kWarps);
+          bad_steps &= ~(1u << place);
+          if (page < 0) {
+            reportIndex(a.error_flag, FPK_ERROR_PAGE);
+            bad_steps |= 1u << place;
+            page = 0;
+            in = false;
+          }
+          row = (key0 + copy_row) & ((1 << a.page_shift) - 1);
+          page_at = page * a.page_stride;
+          if constexpr (kE4m3) {
+            const float* scale = (copy_plane == 0 ? a.k_scale : a.v_scale) + (((static_cast<long long>(page) * a.kv_heads + head) << a.page_shift) + row);
+            copyAsync4(to + S::kScales + lane * 4, scale, in);
           }
         }
-      }
+        if (!in) row = 0, page_at = 0;  // an address that exists; nothing is read
+        if constexpr (kKind == kPacked16) {
+          if (!in) row = q.k0;
+        }
+        const unsigned char* ks = record(a.k, head, row, copy_plane) + page_at;
+        const unsigned char* vs = record(a.v, head, row, copy_plane) + page_at;
+        const uint32_t kd = to + copy_plane * S::kKPlane + copy_row * 16, vd = to + S::kV + copy_plane * S::kVPlane + copy_row * 16;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int key = 8 * j + 4 * (g & 1) + (g >> 1);
-#pragma unroll
-        for (int n = 0; n < S::kKRecords; ++n) {
-          d.k[j][n] = key < d.lim ? loadOnce16(kb + key * a.k.row_stride + (4 * n + t) * a.k.plane_stride) : make_uint4(0, 0, 0, 0);
+        for (int p = 0; p < S::kPlanes / 2; ++p) {
+          copyAsync16(kd + p * 2 * S::kKPlane, ks, in);
+          copyAsync16(vd + p * 2 * S::kVPlane, vs, in);
+          ks += 2 * a.k.plane_stride;
+          vs += 2 * a.v.plane_stride;
         }
       }
-    };
-    auto loadV = [&]() {
-#pragma unroll
-      for (int i = 0; i < S::kVRecords; ++i) {
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const int key = 4 * kk + t;
-          if constexpr (S::kVRegs == 4) {
-            const uint4 w = key < d.lim ? loadOnce16(vb + key * a.v.row_stride + (8 * i + g) * a.v.plane_stride) : make_uint4(0, 0, 0, 0);
-            d.v[i][kk][0] = w.x, d.v[i][kk][1] = w.y, d.v[i][kk][2] = w.z, d.v[i][kk][3] = w.w;
-          } else {
-            const uint2 w = key < d.lim ? loadOnce8(vb + key * a.v.row_stride + (g >> 1) * a.v.plane_stride + (g & 1) * 8) : make_uint2(0, 0);
-            d.v[i][kk][0] = w.x, d.v[i][kk][1] = w.y;
-          }
-        }
-      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
-    int step = b0 * (kUnitKeys / 16) + warp;
-    int page_next = 0;
-    if (step < step_end) {
-      loadK(step, pageAt(step));
-      loadV();
-      page_next = pageAt(step + kWarps);
-    }
-    for (; step < step_end; step += kWarps) {
-      const int key0 = d.key0, lim = d.lim;
+    page_next = pageAt(step_first);
+#pragma unroll
+    for (int i = 0; i < S::kDepth - 1; ++i) copyStep(step_first + i * kWarps, i);
+    int place = 0;
+    for (int step = step_first; step < step_end; step += kWarps) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kDepth - 2) : "memory");
+      __syncwarp();
+      const uint32_t from = ring + place * S::kBytes;
+      const int key0 = step * 16;
+      const int lim = (bad_steps >> place) & 1u ? 0 : min(16, last_vis - key0);
+      float ks[4] = {}, vs[4] = {};
+      if constexpr (kE4m3) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          ks[c] = loadShared4(from + S::kScales + (4 * c + t) * 4);
+          vs[c] = loadShared4(from + S::kScales + 64 + (4 * c + t) * 4);
+        }
+      }
       float sc[2][4] = {};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if constexpr (kE4m3) {
+        const uint32_t at = from + t * S::kKPlane + (8 * j + 4 * (g & 1) + (g >> 1)) * 16;
 #pragma unroll
-          for (int n = 0; n < S::kKRecords; ++n) {
-            const uint32_t w[4] = {d.k[j][n].x, d.k[j][n].y, d.k[j][n].z, d.k[j][n].w};
+        for (int n = 0; n < S::kKRecords; ++n) {
+          const uint4 k = loadShared16(at + 4 * n * S::kKPlane);
+          if constexpr (kE4m3) {
+            const uint32_t w[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mma<M>(sc[j], qf[4 * n + e], e4m3x2ToHalf2(w[e]), e4m3x2ToHalf2(w[e] >> 16));
-          }
-        } else {
-#pragma unroll
-          for (int n = 0; n < S::kKRecords; ++n) {
-            mma<M>(sc[j], qf[2 * n], d.k[j][n].x, d.k[j][n].y);
-            mma<M>(sc[j], qf[2 * n + 1], d.k[j][n].z, d.k[j][n].w);
+            for (int e = 0; e < 4; ++e) {
+              const uint2 h = halves(w[e]);
+              mma<M>(sc[j], qf[4 * n + e], h.x, h.y);
+            }
+          } else {
+            mma<M>(sc[j], qf[2 * n], k.x, k.y);
+            mma<M>(sc[j], qf[2 * n + 1], k.z, k.w);
           }
         }
       }
@@ -372,16 +396,14 @@ __global__ void __launch_bounds__(kThreads) attentionStreamKernel(const Args a) 
         for (int c = 0; c < 4; ++c) {
           const float s = sc[c >> 1][2 * i + (c & 1)];
           if constexpr (kE4m3) {
-            const int ve = (__float_as_int(d.vs[c]) >> 23) - 127;
-            x[i][c] = fmaf(s * row_scale[i], d.ks[c] * a.scale_log2, static_cast<float>(ve));
+            const int ve = (__float_as_int(vs[c]) >> 23) - 127;
+            x[i][c] = fmaf(s * row_scale[i], ks[c] * a.scale_log2, static_cast<float>(ve));
             inv_v[c] = __int_as_float((127 - ve) << 23);
           } else {
             x[i][c] = s * a.scale_log2;
           }
         }
       }
-      const int next = step + kWarps;
-      if (next < step_end) loadK(next, page_next);
       if (key0 + lim > min_vis || lim < 16) {  // the causal edge, the last keys, a bad page
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -434,28 +456,49 @@ __global__ void __launch_bounds__(kThreads) attentionStreamKernel(const Args a) 
 #pragma unroll
       for (int i = 0; i < S::kVRecords; ++i) {
         if constexpr (kE4m3) {
+          uint32_t v[4][S::kVCh / 4];
 #pragma unroll
-          for (int e = 0; e < S::kVCh; e += 2) {
-            uint32_t h[4];
+          for (int kk = 0; kk < 4; ++kk) {
+            if constexpr (S::kVCh == 16) {
+              const uint4 w = loadShared16(from + S::kV + g * S::kVPlane + (4 * kk + t) * 16);
+              v[kk][0] = w.x, v[kk][1] = w.y, v[kk][2] = w.z, v[kk][3] = w.w;
+            } else {
+              const uint2 w = loadShared8(from + S::kV + (g >> 1) * S::kVPlane + (4 * kk + t) * 16 + (g & 1) * 8);
+              v[kk][0] = w.x, v[kk][1] = w.y;
+            }
+          }
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) h[kk] = e4m3x2ToHalf2(d.v[i][kk][e >> 2] >> ((e & 2) * 8));
-            mma<M>(o[i][e], p, __byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
-            mma<M>(o[i][e + 1], p, __byte_perm(h[0], h[1], 0x7632), __byte_perm(h[2], h[3], 0x7632));
+          for (int e = 0; e < S::kVCh; e += 4) {
+            // Codes of keys 0, 1 (2, 3) side by side, then two channels to a word.
+            const uint2 a0 = halves(__byte_perm(v[0][e / 4], v[1][e / 4], 0x5140)), a1 = halves(__byte_perm(v[0][e / 4], v[1][e / 4], 0x7362));
+            const uint2 c0 = halves(__byte_perm(v[2][e / 4], v[3][e / 4], 0x5140)), c1 = halves(__byte_perm(v[2][e / 4], v[3][e / 4], 0x7362));
+            mma<M>(o[i][e], p, a0.x, c0.x);
+            mma<M>(o[i][e + 1], p, a0.y, c0.y);
+            mma<M>(o[i][e + 2], p, a1.x, c1.x);
+            mma<M>(o[i][e + 3], p, a1.y, c1.y);
           }
         } else {
+          uint32_t v[4][4];
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint4 w = loadShared16(from + S::kV + (8 * i + g) * S::kVPlane + (4 * kk + t) * 16);
+            v[kk][0] = w.x, v[kk][1] = w.y, v[kk][2] = w.z, v[kk][3] = w.w;
+          }
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
-            const uint32_t h0 = d.v[i][0][e >> 1], h1 = d.v[i][1][e >> 1], h2 = d.v[i][2][e >> 1], h3 = d.v[i][3][e >> 1];
+            const uint32_t h0 = v[0][e >> 1], h1 = v[1][e >> 1], h2 = v[2][e >> 1], h3 = v[3][e >> 1];
             mma<M>(o[i][e], p, __byte_perm(h0, h1, 0x5410), __byte_perm(h2, h3, 0x5410));
             mma<M>(o[i][e + 1], p, __byte_perm(h0, h1, 0x7632), __byte_perm(h2, h3, 0x7632));
           }
         }
       }
-      if (next < step_end) {
-        loadV();
-        page_next = pageAt(next + kWarps);
-      }
+      __syncwarp();
+      const int refill = place == 0 ? S::kDepth - 1 : place - 1;  // the place read a step before
+      copyStep(step + (S::kDepth - 1) * kWarps, refill);
+      place = place + 1 == S::kDepth ? 0 : place + 1;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the ring is free for the exchange
 
     // ---- join the warps ----
 #pragma unroll
@@ -608,16 +651,22 @@ namespace {
 
 template <typename T, int D, KvKind kKind>
 cudaError_t launchOne(const Args& a, cudaStream_t s) {
+  constexpr int kRing = Step<D, kKind == kPagedE4m3>::kRing;
+  static DeviceOnce smem_attr;
+  const cudaError_t ae = smem_attr.run([] {
+    return cudaFuncSetAttribute(attentionStreamKernel<T, D, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+  });
+  if (ae != cudaSuccess) return ae;
   // As many CTAs as stay resident, so that equal shares end together.
   static DeviceValue resident;
   const int ctas = resident.get([](int dev) {
     int sms = 148, per = 1;
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attentionStreamKernel<T, D, kKind>, kThreads, 0);
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attentionStreamKernel<T, D, kKind>, kThreads, kRing);
     return std::min(kStreamCtas, sms * std::max(per, 1));
   });
   prof::countLaunch(prof::kAttention, 2);
-  cudaError_t e = launchPdl(attentionStreamKernel<T, D, kKind>, dim3(ctas), dim3(kThreads), 0, s, a);
+  cudaError_t e = launchPdl(attentionStreamKernel<T, D, kKind>, dim3(ctas), dim3(kThreads), kRing, s, a);
   if (e != cudaSuccess) return e;
   return launchPdl(joinStreamKernel<T, D, kKind>, dim3(ctas), dim3(kJoinWarps * 32), 0, s, a);
 }
