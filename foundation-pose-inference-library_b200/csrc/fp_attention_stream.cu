@@ -55,12 +55,24 @@ struct Split {
 
 constexpr size_t partialFloats(int d) { return static_cast<size_t>(kStreamRows) * d + 2 * kStreamRows; }
 
+// Quotient of non-negative numbers. Those past 32 bits are rare, and their
+// division is long: it stays out of the code that every launch fetches.
+__device__ __noinline__ long long divideLong(long long x, long long y) { return x / y; }
+__device__ __forceinline__ long long divide(long long x, long long y) {
+  if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+  return divideLong(x, y);
+}
+
+// The first `rest` CTAs take size + 1 units, the others size.
 struct Share {
-  long long units, ctas;
+  long long size, rest;
 };
 
-__device__ __forceinline__ long long shareBegin(const Share& s, long long c) { return c * s.units / s.ctas; }
-__device__ __forceinline__ long long shareOwner(const Share& s, long long u) { return ((u + 1) * s.ctas - 1) / s.units; }
+__device__ __forceinline__ long long shareBegin(const Share& s, long long c) { return c * s.size + min(c, s.rest); }
+__device__ __forceinline__ long long shareOwner(const Share& s, long long u) {
+  const long long large = s.rest * (s.size + 1);
+  return u < large ? divide(u, s.size + 1) : s.rest + divide(u - large, s.size);
+}
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -153,32 +165,13 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
   auto unitsOf = [&](int s, Sequence* out) -> long long {
     const Sequence q = sequence<kKind>(a, s);
     if (out != nullptr) *out = q;
-    const long long tiles = (static_cast<long long>(q.nq) * a.group + kStreamRows - 1) / kStreamRows;
+    const long long tiles = (q.nq * a.group + kStreamRows - 1) / kStreamRows;
     return tiles * a.kv_heads * max((q.nk + kUnitKeys - 1) / kUnitKeys, 1);  // no keys: still zeros to write
   };
-  long long sum = 0;
-  for (int s = tid; s < a.n_seq; s += kThreads) sum += unitsOf(s, nullptr);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) scan_s[warp] = sum;
-  __syncthreads();
-  Share share;
-  share.units = 0;
-  for (int w = 0; w < kWarps; ++w) share.units += scan_s[w];
-  share.ctas = min(static_cast<long long>(gridDim.x), (share.units + kMinUnits - 1) / kMinUnits);
-  Split* splits = reinterpret_cast<Split*>(a.workspace);
-  float* partials = reinterpret_cast<float*>(a.workspace + sizeof(Split) * kStreamCtas);
-  Split* split = splits + blockIdx.x;
-  if (static_cast<long long>(blockIdx.x) >= share.ctas) {
-    if (tid == 0) split->first_unit = -1;
-    return;
-  }
-  const long long begin = shareBegin(share, blockIdx.x), end = shareBegin(share, blockIdx.x + 1LL);
-  // The sequence that holds unit `begin`.
-  long long before = 0;
-  for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) {
-    const int s = s0 + tid;
-    const long long mine = s < a.n_seq ? unitsOf(s, nullptr) : 0;
+  // Units of kThreads sequences and their sums up to each thread's.
+  long long mine = 0, at = 0, total = 0;
+  auto scan = [&](int s0) -> long long {
+    mine = s0 + tid < a.n_seq ? unitsOf(s0 + tid, nullptr) : 0;
     long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -188,17 +181,36 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
     __syncthreads();
     if (lane == 31) scan_s[warp] = upto;
     __syncthreads();
-    long long base = before, all = 0;
+    long long all = 0;
+    at = upto - mine;
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) base += scan_s[w];
+      if (w < warp) at += scan_s[w];
       all += scan_s[w];
     }
-    if (begin >= base + upto - mine && begin < base + upto) {
-      found_s[0] = s;
-      found_s[1] = base + upto - mine;
+    return all;
+  };
+  for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) total += scan(s0);
+  const long long ctas = min(static_cast<long long>(gridDim.x), (total + kMinUnits - 1) / kMinUnits);
+  Split* splits = reinterpret_cast<Split*>(a.workspace);
+  float* partials = reinterpret_cast<float*>(a.workspace + sizeof(Split) * kStreamCtas);
+  Split* split = splits + blockIdx.x;
+  if (static_cast<long long>(blockIdx.x) >= ctas) {
+    if (tid == 0) split->first_unit = -1;
+    return;
+  }
+  Share share;
+  share.size = divide(total, ctas);
+  share.rest = total - share.size * ctas;
+  const long long begin = shareBegin(share, blockIdx.x), end = shareBegin(share, blockIdx.x + 1LL);
+  // The sequence that holds unit `begin`.
+  long long before = 0;
+  for (int s0 = 0; s0 < a.n_seq && before <= begin; s0 += kThreads) {
+    const long long all = a.n_seq > kThreads ? scan(s0) : total;  // one pass: still at hand
+    if (begin >= before + at && begin < before + at + mine) {
+      found_s[0] = s0 + tid;
+      found_s[1] = before + at;
     }
     before += all;
-    if (begin < before) break;
   }
   __syncthreads();
   int seq = static_cast<int>(found_s[0]);
@@ -214,13 +226,13 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
       seq_units = unitsOf(++seq, &q);
     }
     const int blocks = max((q.nk + kUnitKeys - 1) / kUnitKeys, 1);
-    const long long tile_head = (u - seq_first) / blocks;
-    const int tile = static_cast<int>(tile_head / a.kv_heads);
+    const long long tile_head = divide(u - seq_first, blocks);
+    const int tile = static_cast<int>(divide(tile_head, a.kv_heads));
     const int head = static_cast<int>(tile_head - static_cast<long long>(tile) * a.kv_heads);
     const long long tile_first = seq_first + tile_head * blocks;
     const int b0 = static_cast<int>(u - tile_first);
     const int b1 = static_cast<int>(min(static_cast<long long>(blocks), end - tile_first));
-    const int rows = static_cast<int>(min(static_cast<long long>(kStreamRows), static_cast<long long>(q.nq) * a.group - static_cast<long long>(tile) * kStreamRows));
+    const int rows = min(kStreamRows, q.nq * a.group - tile * kStreamRows);
 
     // Rows g and g + 8 of the tile.
     int vis[2];
@@ -229,13 +241,13 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int rr = g + 8 * i;
-      const long long r = static_cast<long long>(tile) * kStreamRows + rr;
-      const int token = static_cast<int>(r / q_heads_per);
+      const int r = tile * kStreamRows + rr;  // below 2^31: checked by the host
+      const int token = r / q_heads_per;
       vis[i] = rr < rows ? visible(a, q, token) : q.nk;
-      qp[i] = rr < rows ? record(a.q, head * q_heads_per + static_cast<int>(r - static_cast<long long>(token) * q_heads_per), q.q0 + token, 0) : nullptr;
+      qp[i] = rr < rows ? record(a.q, head * q_heads_per + r - token * q_heads_per, q.q0 + token, 0) : nullptr;
       min_vis = min(min_vis, vis[i]);
     }
-    const int last_vis = visible(a, q, static_cast<int>((static_cast<long long>(tile) * kStreamRows + rows - 1) / q_heads_per));
+    const int last_vis = visible(a, q, (tile * kStreamRows + rows - 1) / q_heads_per);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) min_vis = min(min_vis, __shfl_xor_sync(0xffffffffu, min_vis, o));
 
@@ -540,9 +552,9 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] *= inv;
-        const long long r = static_cast<long long>(tile) * kStreamRows + rr;
-        const int token = static_cast<int>(r / q_heads_per);
-        const int h = head * q_heads_per + static_cast<int>(r - static_cast<long long>(token) * q_heads_per);
+        const int r = tile * kStreamRows + rr;  // below 2^31: checked by the host
+        const int token = r / q_heads_per;
+        const int h = head * q_heads_per + r - token * q_heads_per;
         *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(acc);
       } else {
         float4* dst = reinterpret_cast<float4*>(part + rr * D + grp * 8);
@@ -636,9 +648,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) joinStreamKernel(const Args a
     const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= inv;
-    const long long r = static_cast<long long>(split.tile) * kStreamRows + rr;
-    const int token = static_cast<int>(r / a.group);
-    const int h = split.head * a.group + static_cast<int>(r - static_cast<long long>(token) * a.group);
+    const int r = split.tile * kStreamRows + rr;
+    const int token = r / a.group;
+    const int h = split.head * a.group + r - token * a.group;
     *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(x);
   }
 }
