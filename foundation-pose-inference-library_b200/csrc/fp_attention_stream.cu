@@ -251,62 +251,6 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) min_vis = min(min_vis, __shfl_xor_sync(0xffffffffu, min_vis, o));
 
-    // Query fragments: the records of the channels that this thread's K records hold.
-    uint32_t qf[D / 16][4];
-    float row_scale[2] = {1.0f, 1.0f};
-    {
-      uint4 raw[2][D / 32];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int n = 0; n < D / 32; ++n) {
-          const int plane = kE4m3 ? 2 * (4 * (n / 2) + t) + n % 2 : 4 * n + t;
-          raw[i][n] = qp[i] != nullptr ? *reinterpret_cast<const uint4*>(qp[i] + plane * a.q.plane_stride) : make_uint4(0, 0, 0, 0);
-        }
-      }
-      if constexpr (kE4m3) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float m = 0.0f;
-#pragma unroll
-          for (int n = 0; n < D / 32; ++n) {
-            float x[8];
-            unpack8<T>(raw[i][n], x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
-          }
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          // 2^(exponent of m), kept where its inverse is a normal number.
-          const int e = min(max((__float_as_int(m) >> 23) & 0xff, 1), 253) - 127;
-          row_scale[i] = m > 0.0f ? __int_as_float((e + 127) << 23) : 1.0f;
-          const float inv = m > 0.0f ? __int_as_float((127 - e) << 23) : 1.0f;
-#pragma unroll
-          for (int n = 0; n < D / 32; ++n) {
-            float x[8];
-            unpack8<T>(raw[i][n], x);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) x[c] *= inv;
-            raw[i][n] = pack8<__half>(x);
-          }
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < D / 32; ++n) {
-        const uint4 lo = raw[0][n], hi = raw[1][n];
-        qf[2 * n][0] = lo.x, qf[2 * n][1] = hi.x, qf[2 * n][2] = lo.y, qf[2 * n][3] = hi.y;
-        qf[2 * n + 1][0] = lo.z, qf[2 * n + 1][1] = hi.z, qf[2 * n + 1][2] = lo.w, qf[2 * n + 1][3] = hi.w;
-      }
-    }
-
-    float o[S::kVRecords][S::kVCh][4];
-#pragma unroll
-    for (int i = 0; i < S::kVRecords; ++i) {
-#pragma unroll
-      for (int e = 0; e < S::kVCh; ++e) o[i][e][0] = o[i][e][1] = o[i][e][2] = o[i][e][3] = 0.0f;
-    }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-
     // Steps of 16 keys, one warp after the other, up to the last visible key.
     const int step_end = min(b1 * (kUnitKeys / 16), (last_vis + 15) >> 4);
     const int step_first = b0 * (kUnitKeys / 16) + warp;
@@ -365,6 +309,62 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
     page_next = pageAt(step_first);
 #pragma unroll
     for (int i = 0; i < S::kDepth - 1; ++i) copyStep(step_first + i * kWarps, i);
+    // Query fragments: the records of the channels that this thread's K records hold.
+    uint32_t qf[D / 16][4];
+    float row_scale[2] = {1.0f, 1.0f};
+    {
+      uint4 raw[2][D / 32];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+          const int plane = kE4m3 ? 2 * (4 * (n / 2) + t) + n % 2 : 4 * n + t;
+          raw[i][n] = qp[i] != nullptr ? *reinterpret_cast<const uint4*>(qp[i] + plane * a.q.plane_stride) : make_uint4(0, 0, 0, 0);
+        }
+      }
+      if constexpr (kE4m3) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float m = 0.0f;
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) {
+            float x[8];
+            unpack8<T>(raw[i][n], x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+          }
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          // 2^(exponent of m), kept where its inverse is a normal number.
+          const int e = min(max((__float_as_int(m) >> 23) & 0xff, 1), 253) - 127;
+          row_scale[i] = m > 0.0f ? __int_as_float((e + 127) << 23) : 1.0f;
+          const float inv = m > 0.0f ? __int_as_float((127 - e) << 23) : 1.0f;
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) {
+            float x[8];
+            unpack8<T>(raw[i][n], x);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[c] *= inv;
+            raw[i][n] = pack8<__half>(x);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < D / 32; ++n) {
+        const uint4 lo = raw[0][n], hi = raw[1][n];
+        qf[2 * n][0] = lo.x, qf[2 * n][1] = hi.x, qf[2 * n][2] = lo.y, qf[2 * n][3] = hi.y;
+        qf[2 * n + 1][0] = lo.z, qf[2 * n + 1][1] = hi.z, qf[2 * n + 1][2] = lo.w, qf[2 * n + 1][3] = hi.w;
+      }
+    }
+
+    float o[S::kVRecords][S::kVCh][4];
+#pragma unroll
+    for (int i = 0; i < S::kVRecords; ++i) {
+#pragma unroll
+      for (int e = 0; e < S::kVCh; ++e) o[i][e][0] = o[i][e][1] = o[i][e][2] = o[i][e][3] = 0.0f;
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
     int place = 0;
     for (int step = step_first; step < step_end; step += kWarps) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kDepth - 2) : "memory");
@@ -611,18 +611,33 @@ __global__ void __launch_bounds__(kJoinWarps * 32) joinStreamKernel(const Args a
   constexpr int kPer = D / 32;  // channels of a lane
   float acc[kPer] = {}, m = -INFINITY, l = 0.0f;
   if (row < split.rows) {
-    // Piece i of the tile is CTA c0 + i's: its last piece (1) for i = 0, its first (0) after.
-    auto piece = [&](int i) { return partials + (2 * static_cast<size_t>(c0 + i) + (i == 0 ? 1 : 0)) * partialFloats(D); };
-    for (int i = sub; i < n; i += per_row) m = fmaxf(m, __ldcg(piece(i) + kStreamRows * D + row));
-#pragma unroll 4
-    for (int i = sub; i < n; i += per_row) {
-      const float* p = piece(i);
-      const float pm = __ldcg(p + kStreamRows * D + row);
-      const float pl = __ldcg(p + kStreamRows * D + kStreamRows + row);
-      const float f = pm == m ? 1.0f : exp2Approx(pm - m);
-      l = fmaf(pl, f, l);
+    // Piece i of the tile is CTA c0 + i's: its last piece (1) for i = 0, its
+    // first (0) after. Four are read at a time.
+    for (int i0 = sub; i0 < n; i0 += 4 * per_row) {
+      float pm[4], pl[4], po[4][kPer];
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[e] = fmaf(__ldcg(p + row * D + e * 32 + lane), f, acc[e]);
+      for (int x = 0; x < 4; ++x) {
+        const int i = i0 + x * per_row;
+        const bool in = i < n;
+        const float* p = partials + (2 * static_cast<size_t>(c0 + (in ? i : i0)) + ((in ? i : i0) == 0 ? 1 : 0)) * partialFloats(D);
+        pm[x] = in ? __ldcg(p + kStreamRows * D + row) : -INFINITY;
+        pl[x] = in ? __ldcg(p + kStreamRows * D + kStreamRows + row) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) po[x][e] = in ? __ldcg(p + row * D + e * 32 + lane) : 0.0f;
+      }
+      const float top = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
+      const float keep = m == top ? 1.0f : exp2Approx(m - top);
+      m = top;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] *= keep;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float f = pm[x] == m ? 1.0f : exp2Approx(pm[x] - m);
+        l = fmaf(pl[x], f, l);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[e] = fmaf(po[x][e], f, acc[e]);
+      }
     }
     if (lane == 0) {
       ml_s[warp][0] = m;
