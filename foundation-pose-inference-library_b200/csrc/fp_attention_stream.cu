@@ -26,6 +26,8 @@
 //   keys form one line that the CTAs share out, each finding its part from the
 //   lengths on the device. A tile that crosses CTAs leaves fp32 partials that a
 //   second launch joins in order (deterministic, no atomics).
+// * Short sequences instead take a cluster of CTAs for each tile, which share its
+//   keys out evenly and join over distributed shared memory: no second launch.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -46,6 +48,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kUnitKeys = 64;     // one unit of the split: 16 keys of each warp
 constexpr int kMinUnits = 4;      // a CTA takes at least 256 keys
 constexpr float kGrowLog2 = 8.0f;
+constexpr int kClusterKeys = 512;  // a cluster's most keys to a CTA
 
 // The tile that a CTA's range begins inside, for the joining launch.
 struct Split {
@@ -119,6 +122,18 @@ __device__ __forceinline__ float loadShared4(uint32_t at) {
   return v;
 }
 
+// From another CTA of the cluster.
+__device__ __forceinline__ float4 loadCluster16(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ float loadCluster4(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+
 // The four e4m3 codes of a word as two fp16 pairs.
 __device__ __forceinline__ uint2 halves(uint32_t four) {
   uint2 r;
@@ -140,13 +155,13 @@ struct Step {
   // Three CTAs to an SM share its 227 KB.
   static constexpr int kDepth = 75776 / (kWarps * kBytes) < 5 ? 75776 / (kWarps * kBytes) : 5;
   static constexpr int kRing = kWarps * kDepth * kBytes;
-  static_assert(kDepth >= 2 && kRing >= kWarps * kStreamRows * (D + 4) * 4, "the outputs' exchange lies over the ring");
+  static_assert(kDepth >= 2 && kRing >= (kWarps * kStreamRows * (D + 4) + kStreamRows * D) * 4, "the outputs' exchange lies over the ring");
 };
 
 }  // namespace
 
-template <typename T, int D, KvKind kKind>
-__global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args a) {
+template <typename T, int D, KvKind kKind, bool kCluster>
+__global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args a, int cluster) {
   constexpr bool kE4m3 = kKind == kPagedE4m3;
   using S = Step<D, kE4m3>;
   using M = std::conditional_t<kE4m3, __half, T>;  // type of the products
@@ -155,12 +170,21 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
   __shared__ float ml_s[kWarps][2][kStreamRows];
   __shared__ long long scan_s[kWarps + 1];
   __shared__ long long found_s[2];
+  __shared__ int owner_s;                     // clusters: the sequence, the last that has this tile
+  __shared__ float joined_s[2][kStreamRows];  // clusters: this CTA's m and l
 
   tc::pdlTrigger();
   tc::pdlWait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
 
+  Split* splits = reinterpret_cast<Split*>(a.workspace);
+  float* partials = reinterpret_cast<float*>(a.workspace + sizeof(Split) * kStreamCtas);
+  Split* split = splits + blockIdx.x;
+  Share share{};
+  long long begin = 0, end = 1, seq_first = 0, seq_units = 1;
+  int seq = 0, rank = 0, cluster_tile = 0, cluster_head = 0;
+  Sequence q{};
   // ---- this CTA's part of the line ----
   auto unitsOf = [&](int s, Sequence* out) -> long long {
     const Sequence q = sequence<kKind>(a, s);
@@ -168,70 +192,98 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
     const long long tiles = (q.nq * a.group + kStreamRows - 1) / kStreamRows;
     return tiles * a.kv_heads * max((q.nk + kUnitKeys - 1) / kUnitKeys, 1);  // no keys: still zeros to write
   };
-  // Units of kThreads sequences and their sums up to each thread's.
-  long long mine = 0, at = 0, total = 0;
-  auto scan = [&](int s0) -> long long {
-    mine = s0 + tid < a.n_seq ? unitsOf(s0 + tid, nullptr) : 0;
-    long long upto = mine;
+  if constexpr (kCluster) {
+    // Tiles of sequence s have the numbers q0 * group / 16 + s + 0, 1, ...: apart
+    // from those of the next, whatever the lengths are. Starts that overlap (an
+    // error) give all CTAs of a cluster the same one: the last.
+    rank = static_cast<int>(tc::clusterCtaRank());
+    const int x = static_cast<int>(blockIdx.x) / cluster;
+    const int number = x / a.kv_heads;
+    cluster_head = x - number * a.kv_heads;
+    if (tid == 0) owner_s = -1;
+    __syncthreads();
+    if (tid < a.n_seq) {  // at most kThreads sequences: clusterOf()
+      const Sequence c = sequence<kKind>(a, tid);
+      const int tile = number - c.q0 * a.group / kStreamRows - tid;
+      if (tile >= 0 && tile < (c.nq * a.group + kStreamRows - 1) / kStreamRows) atomicMax(&owner_s, tid);
+    }
+    __syncthreads();
+    if (owner_s < 0) return;  // a number without a tile: the whole cluster leaves
+    seq = owner_s;
+    q = sequence<kKind>(a, seq);
+    cluster_tile = number - q.q0 * a.group / kStreamRows - seq;
+  } else {
+    // Units of kThreads sequences and their sums up to each thread's.
+    long long mine = 0, at = 0, total = 0;
+    auto scan = [&](int s0) -> long long {
+      mine = s0 + tid < a.n_seq ? unitsOf(s0 + tid, nullptr) : 0;
+      long long upto = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      __syncthreads();
+      if (lane == 31) scan_s[warp] = upto;
+      __syncthreads();
+      long long all = 0;
+      at = upto - mine;
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) at += scan_s[w];
+        all += scan_s[w];
+      }
+      return all;
+    };
+    for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) total += scan(s0);
+    const long long ctas = min(static_cast<long long>(gridDim.x), (total + kMinUnits - 1) / kMinUnits);
+    if (static_cast<long long>(blockIdx.x) >= ctas) {
+      if (tid == 0) split->first_unit = -1;
+      return;
+    }
+    share.size = divide(total, ctas);
+    share.rest = total - share.size * ctas;
+    begin = shareBegin(share, blockIdx.x);
+    end = shareBegin(share, blockIdx.x + 1LL);
+    // The sequence that holds unit `begin`.
+    long long before = 0;
+    for (int s0 = 0; s0 < a.n_seq && before <= begin; s0 += kThreads) {
+      const long long all = a.n_seq > kThreads ? scan(s0) : total;  // one pass: still at hand
+      if (begin >= before + at && begin < before + at + mine) {
+        found_s[0] = s0 + tid;
+        found_s[1] = before + at;
+      }
+      before += all;
     }
     __syncthreads();
-    if (lane == 31) scan_s[warp] = upto;
-    __syncthreads();
-    long long all = 0;
-    at = upto - mine;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) at += scan_s[w];
-      all += scan_s[w];
-    }
-    return all;
-  };
-  for (int s0 = 0; s0 < a.n_seq; s0 += kThreads) total += scan(s0);
-  const long long ctas = min(static_cast<long long>(gridDim.x), (total + kMinUnits - 1) / kMinUnits);
-  Split* splits = reinterpret_cast<Split*>(a.workspace);
-  float* partials = reinterpret_cast<float*>(a.workspace + sizeof(Split) * kStreamCtas);
-  Split* split = splits + blockIdx.x;
-  if (static_cast<long long>(blockIdx.x) >= ctas) {
-    if (tid == 0) split->first_unit = -1;
-    return;
+    seq = static_cast<int>(found_s[0]);
+    seq_first = found_s[1];
+    seq_units = unitsOf(seq, &q);
   }
-  Share share;
-  share.size = divide(total, ctas);
-  share.rest = total - share.size * ctas;
-  const long long begin = shareBegin(share, blockIdx.x), end = shareBegin(share, blockIdx.x + 1LL);
-  // The sequence that holds unit `begin`.
-  long long before = 0;
-  for (int s0 = 0; s0 < a.n_seq && before <= begin; s0 += kThreads) {
-    const long long all = a.n_seq > kThreads ? scan(s0) : total;  // one pass: still at hand
-    if (begin >= before + at && begin < before + at + mine) {
-      found_s[0] = s0 + tid;
-      found_s[1] = before + at;
-    }
-    before += all;
-  }
-  __syncthreads();
-  int seq = static_cast<int>(found_s[0]);
-  long long seq_first = found_s[1];
-  Sequence q;
-  long long seq_units = unitsOf(seq, &q);
 
   const int q_heads_per = a.group;
   bool first_piece = true;
   for (long long u = begin; u < end;) {
-    while (u >= seq_first + seq_units) {  // the next sequence with rows
-      seq_first += seq_units;
-      seq_units = unitsOf(++seq, &q);
+    int blocks, tile, head, b0, b1;
+    long long tile_first = 0;
+    if constexpr (kCluster) {
+      blocks = max((q.nk + kUnitKeys - 1) / kUnitKeys, 1);
+      tile = cluster_tile;
+      head = cluster_head;
+      b0 = blocks * rank / cluster;
+      b1 = blocks * (rank + 1) / cluster;
+    } else {
+      while (u >= seq_first + seq_units) {  // the next sequence with rows
+        seq_first += seq_units;
+        seq_units = unitsOf(++seq, &q);
+      }
+      blocks = max((q.nk + kUnitKeys - 1) / kUnitKeys, 1);
+      const long long tile_head = divide(u - seq_first, blocks);
+      tile = static_cast<int>(divide(tile_head, a.kv_heads));
+      head = static_cast<int>(tile_head - static_cast<long long>(tile) * a.kv_heads);
+      tile_first = seq_first + tile_head * blocks;
+      b0 = static_cast<int>(u - tile_first);
+      b1 = static_cast<int>(min(static_cast<long long>(blocks), end - tile_first));
     }
-    const int blocks = max((q.nk + kUnitKeys - 1) / kUnitKeys, 1);
-    const long long tile_head = divide(u - seq_first, blocks);
-    const int tile = static_cast<int>(divide(tile_head, a.kv_heads));
-    const int head = static_cast<int>(tile_head - static_cast<long long>(tile) * a.kv_heads);
-    const long long tile_first = seq_first + tile_head * blocks;
-    const int b0 = static_cast<int>(u - tile_first);
-    const int b1 = static_cast<int>(min(static_cast<long long>(blocks), end - tile_first));
     const int rows = min(kStreamRows, q.nq * a.group - tile * kStreamRows);
 
     // Rows g and g + 8 of the tile.
@@ -531,8 +583,14 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
       }
     }
     __syncthreads();
-    const bool whole = b0 == 0 && b1 == blocks;
-    float* part = partials + (2 * static_cast<size_t>(blockIdx.x) + (first_piece && b0 > 0 ? 0 : 1)) * partialFloats(D);
+    const bool whole = kCluster ? cluster == 1 : b0 == 0 && b1 == blocks;
+    // A partial: in this CTA's shared memory behind the exchange, or in the workspace.
+    float* part;
+    if constexpr (kCluster) {
+      part = reinterpret_cast<float*>(ring_raw) + kWarps * kStreamRows * (D + 4);
+    } else {
+      part = partials + (2 * static_cast<size_t>(blockIdx.x) + (first_piece && b0 > 0 ? 0 : 1)) * partialFloats(D);
+    }
     for (int i = tid; i < kStreamRows * (D / 8); i += kThreads) {
       const int rr = i / (D / 8), grp = i % (D / 8);
       if (rr >= rows) continue;
@@ -561,10 +619,39 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
         dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
         if (grp == 0) {
-          part[kStreamRows * D + rr] = mm;
-          part[kStreamRows * D + kStreamRows + rr] = ll;
+          (kCluster ? joined_s[0] : part + kStreamRows * D)[rr] = mm;
+          (kCluster ? joined_s[1] : part + kStreamRows * D + kStreamRows)[rr] = ll;
         }
       }
+    }
+    if constexpr (kCluster) {
+      if (cluster > 1) {
+        tc::clusterSync();
+        const uint32_t part_at = tc::smemU32(part), ml_at = tc::smemU32(&joined_s[0][0]);
+        for (int i = rank * kThreads + tid; i < rows * (D / 8); i += cluster * kThreads) {
+          const int rr = i / (D / 8), grp = i % (D / 8);
+          float m_all = -INFINITY, l_all = 0.0f, x[8] = {};
+          for (int c = 0; c < cluster; ++c) m_all = fmaxf(m_all, loadCluster4(tc::mapaShared(ml_at + rr * 4, c)));
+          for (int c = 0; c < cluster; ++c) {
+            const float mc = loadCluster4(tc::mapaShared(ml_at + rr * 4, c));
+            const float f = mc == m_all ? 1.0f : exp2Approx(mc - m_all);
+            l_all = fmaf(loadCluster4(tc::mapaShared(ml_at + (kStreamRows + rr) * 4, c)), f, l_all);
+            const uint32_t at = tc::mapaShared(part_at + (rr * D + grp * 8) * 4, c);
+            const float4 y = loadCluster16(at), z = loadCluster16(at + 16);
+            const float v[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = fmaf(v[e], f, x[e]);
+          }
+          const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= inv;
+          const int r = tile * kStreamRows + rr;
+          const int token = r / q_heads_per;
+          *reinterpret_cast<uint4*>(record(a.out, head * q_heads_per + r - token * q_heads_per, q.q0 + token, grp)) = pack8<T>(x);
+        }
+        tc::clusterSync();  // no CTA leaves while another reads its memory
+      }
+      return;
     }
     if (first_piece && tid == 0) {
       if (b0 > 0) {
@@ -676,12 +763,29 @@ long long streamWorkspaceBytes(int head_dim) {
 
 namespace {
 
+// CTAs to a tile where sequences are at most max_keys long, 0: even shares of
+// the line instead, joined by a second launch. A cluster grows while all CTAs run
+// at once and have two units or more, and is taken where none of its CTAs gets
+// more than kClusterKeys keys. Measured with 8 key heads, clusters against shares
+// (us): 4 x 64 keys 4.4 / 14.2, 4 x 1000 (128 keys to a CTA) 9.7 / 12.7, 4 x 2000
+// (256) 12.7 / 14.8, 32 x 500 (512) 15.3 / 20.9, 1 x 4000 (512) 13.2 / 13.2, 16 x
+// 2000 (1024) 29.2 / 20.0, 8 x 4000 (1024) 28.4 / 18.9.
+int clusterOf(const Args& a, int max_keys, int resident) {
+  if (a.n_seq > kThreads) return 0;  // each thread looks at one sequence
+  const long long tiles = (static_cast<long long>(a.q_rows) * a.group / kStreamRows + a.n_seq) * a.kv_heads;
+  if (tiles > 0x7fffffffLL / 8) return 0;
+  int n = 1;
+  while (n < 8 && 2 * n * tiles <= resident && 2 * n * 2 * kUnitKeys <= max_keys) n *= 2;
+  return max_keys <= n * kClusterKeys ? n : 0;
+}
+
 template <typename T, int D, KvKind kKind>
-cudaError_t launchOne(const Args& a, cudaStream_t s) {
+cudaError_t launchOne(const Args& a, int max_keys, cudaStream_t s) {
   constexpr int kRing = Step<D, kKind == kPagedE4m3>::kRing;
   static DeviceOnce smem_attr;
   const cudaError_t ae = smem_attr.run([] {
-    return cudaFuncSetAttribute(attentionStreamKernel<T, D, kKind>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+    const cudaError_t e = cudaFuncSetAttribute(attentionStreamKernel<T, D, kKind, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(attentionStreamKernel<T, D, kKind, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
   });
   if (ae != cudaSuccess) return ae;
   // As many CTAs as stay resident, so that equal shares end together.
@@ -689,31 +793,50 @@ cudaError_t launchOne(const Args& a, cudaStream_t s) {
   const int ctas = resident.get([](int dev) {
     int sms = 148, per = 1;
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attentionStreamKernel<T, D, kKind>, kThreads, kRing);
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attentionStreamKernel<T, D, kKind, false>, kThreads, kRing);
     return std::min(kStreamCtas, sms * std::max(per, 1));
   });
+  if (const int cluster = clusterOf(a, max_keys, ctas); cluster > 0) {
+    const long long tiles = (static_cast<long long>(a.q_rows) * a.group / kStreamRows + a.n_seq) * a.kv_heads;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kRing;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    prof::countLaunch(prof::kAttention);
+    return cudaLaunchKernelEx(&cfg, attentionStreamKernel<T, D, kKind, true>, a, cluster);
+  }
   prof::countLaunch(prof::kAttention, 2);
-  cudaError_t e = launchPdl(attentionStreamKernel<T, D, kKind>, dim3(ctas), dim3(kThreads), kRing, s, a);
+  cudaError_t e = launchPdl(attentionStreamKernel<T, D, kKind, false>, dim3(ctas), dim3(kThreads), kRing, s, a, 0);
   if (e != cudaSuccess) return e;
   return launchPdl(joinStreamKernel<T, D, kKind>, dim3(ctas), dim3(kJoinWarps * 32), 0, s, a);
 }
 
 template <typename T, int D>
-cudaError_t launchKind(const Args& a, KvKind kind, cudaStream_t s) {
+cudaError_t launchKind(const Args& a, KvKind kind, int max_keys, cudaStream_t s) {
   switch (kind) {
-    case kPacked16: return launchOne<T, D, kPacked16>(a, s);
-    case kPaged16: return launchOne<T, D, kPaged16>(a, s);
-    default: return launchOne<T, D, kPagedE4m3>(a, s);
+    case kPacked16: return launchOne<T, D, kPacked16>(a, max_keys, s);
+    case kPaged16: return launchOne<T, D, kPaged16>(a, max_keys, s);
+    default: return launchOne<T, D, kPagedE4m3>(a, max_keys, s);
   }
 }
 
 }  // namespace
 
 cudaError_t launchStream(const Args& a, KvKind kind, int head_dim, int dtype, cudaStream_t s) {
+  const long long most = kind == kPacked16 ? a.kv_rows : static_cast<long long>(a.table_pages) << a.page_shift;
+  const int max_keys = static_cast<int>(std::min(most, 0x7fffffffLL));
   if (dtype == FPK_DTYPE_BF16) {
-    return head_dim == 64 ? launchKind<__nv_bfloat16, 64>(a, kind, s) : launchKind<__nv_bfloat16, 128>(a, kind, s);
+    return head_dim == 64 ? launchKind<__nv_bfloat16, 64>(a, kind, max_keys, s) : launchKind<__nv_bfloat16, 128>(a, kind, max_keys, s);
   }
-  return head_dim == 64 ? launchKind<__half, 64>(a, kind, s) : launchKind<__half, 128>(a, kind, s);
+  return head_dim == 64 ? launchKind<__half, 64>(a, kind, max_keys, s) : launchKind<__half, 128>(a, kind, max_keys, s);
 }
 
 }  // namespace seqattn
