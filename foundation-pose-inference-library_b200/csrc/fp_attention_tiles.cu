@@ -7,13 +7,13 @@
 // takes 1,024 cycles of MMA and 16,384 / 16 = 1,024 cycles of ex2.
 //
 // One persistent CTA per SM, 512 threads. Its tile is 256 query rows of one
-// (sequence, key head), two halves of 128 rows that take turns: while the
-// softmax of one half runs, the tensor core works for the other.
+// (sequence, key head), two halves of 128 rows: while the softmax of one half
+// runs, the tensor core works for the other.
 //   warps 0-3, 4-7  softmax of half 0 and 1, one query row per thread: the
-//                   row's 128 scores from TMEM, running maximum and sum in
-//                   fp32, P = 2^(s - m) rounded to the element type over the
-//                   scores' own TMEM columns. O is rescaled only when a row's
-//                   maximum grows by more than 2^8. After the last block, O / l.
+//                   row's 128 scores from TMEM, 64 at a time: running maximum
+//                   and sum in fp32, P = 2^(s - m) rounded to the element type
+//                   over the scores' own TMEM columns. O is rescaled only when a
+//                   row's maximum grows by more than 2^8. After the last, O / l.
 //   warps 8-11      loads of Q, K and V rows, K and V in four stages of 128 rows.
 //                   Two layouts in shared memory, each the one that its source
 //                   fills line by line (the other way round the copies take
@@ -95,8 +95,7 @@ struct Smem {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t q_ready[2], kv_ready[kStages];  // full, and fenced for the tensor core
-  uint64_t s_full[2], p_half[2], p_full[2], pv_done[2], o_free[2];
-  uint64_t turn[2][4];         // a half's warp has finished its exponentials: the other half's may begin
+  uint64_t s_full[2], p_half[2], p_full[2], pv_half[2], pv_done[2], o_free[2];  // half: of a block's first 64 keys
   uint64_t drained[2];
   Item items[kItems];
   long long scan[kThreads / 32 + 1];
@@ -373,10 +372,10 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       mbarInit(&sm.s_full[i], 1);
       mbarInit(&sm.p_half[i], 4);
       mbarInit(&sm.p_full[i], 4);
+      mbarInit(&sm.pv_half[i], 1);
       mbarInit(&sm.pv_done[i], 1);
       mbarInit(&sm.o_free[i], 4);
       mbarInit(&sm.drained[i], 1);
-      for (int j = 0; j < 4; ++j) mbarInit(&sm.turn[i][j], 1);
     }
     for (int i = 0; i < kStages; ++i) {
       mbarInit(&sm.kv_full[i], kLoadWarps * 32);
@@ -506,7 +505,10 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           if (ok) ok = wait(&sm.p_half[t], done & 1, sm, err, 58);
           if (!ok) break;
           tcFenceAfter();
-          if (electOne()) issueValues<0>(o_at, s_at, v, v_op.step, idesc_o, steps, pv.j > pv.jb);
+          if (electOne()) {
+            issueValues<0>(o_at, s_at, v, v_op.step, idesc_o, steps, pv.j > pv.jb);
+            commit(&sm.pv_half[t]);
+          }
           __syncwarp();
           ok = wait(&sm.p_full[t], done & 1, sm, err, 58);
           if (!ok) break;
@@ -880,7 +882,6 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
     const uint32_t o_base = lane_base + kOCol + t * D;
     bool ok = true;
     int count = 0;  // blocks of this half
-    int turns = 0;  // blocks that both halves have
     for (int i = 0; ok; ++i) {
       const int slot = i % kItems;
       ok = wait(&sm.item_full[slot], (i / kItems) & 1, sm, err, 55);
@@ -911,63 +912,48 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         ok = wait(&sm.s_full[t], count & 1, sm, err, 58);
         if (!ok) break;
         tcFenceAfter();
-        // Twice over the row's scores, 64 at a time: reading them again from
-        // TMEM is cheap, keeping 128 in registers is not.
+        // 64 scores at a time, which registers hold, each read once. (A pass for
+        // the maximum of all 128 before it, with the halves taking turns at the
+        // exponentials, took 162 us for crops and 549 for planar prompts in place
+        // of 150 and 530.)
         const bool edge = (j + 1) * kKeys > min_vis || bad != 0;  // the causal edge, the last keys, bad pages
         const int lim = vis - j * kKeys;
-        uint32_t sv[64];
-        auto load = [&](int c) {
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sv[64];
           FPB_TMEM_LD32(s_base + 64 * c, sv);
           FPB_TMEM_LD32(s_base + 64 * c + 32, (sv + 32));
           tmemWaitLd();
           if (edge) hide(sv, lim - 64 * c, bad >> (4 * c));
-        };
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          load(c);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int e = 0; e < 64; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
-        }
-        const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
-        if (j == it.jb) {
-          m = top;
-        } else if (__any_sync(0xffffffffu, top > m + kGrowLog2)) {
-          const float m_new = top > m + kGrowLog2 ? top : m;
-          const float f = m_new == m ? 1.0f : exp2Approx(m - m_new);
-          ok = wait(&sm.pv_done[t], (count - 1) & 1, sm, err, 59);
-          if (!ok) break;
-          tcFenceAfter();
+          const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
+          if (j == it.jb && c == 0) {
+            m = top;
+          } else if (__any_sync(0xffffffffu, top > m + kGrowLog2)) {
+            const float m_new = top > m + kGrowLog2 ? top : m;
+            const float f = m_new == m ? 1.0f : exp2Approx(m - m_new);
+            // O takes in the products of the 64 keys before these.
+            ok = wait(c == 0 ? &sm.pv_done[t] : &sm.pv_half[t], (c == 0 ? count - 1 : count) & 1, sm, err, 59);
+            if (!ok) break;
+            tcFenceAfter();
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t ov[32];
-            FPB_TMEM_LD32(o_base + c, ov);
-            tmemWaitLd();
+            for (int d = 0; d < D; d += 16) {
+              uint32_t ov[16];
+              FPB_TMEM_LD16(o_base + d, ov);
+              tmemWaitLd();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * f);
-            FPB_TMEM_ST32(o_base + c, ov);
+              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * f);
+              FPB_TMEM_ST16(o_base + d, ov);
+            }
+            tmemStoreWait();
+            l *= f;
+            m = m_new;
           }
-          tmemStoreWait();
-          l *= f;
-          m = m_new;
-        }
-        // The exponential unit goes from half to half: while one computes, the
-        // other's scores and products run. Left to themselves the halves fall
-        // into step and take turns at everything else, too.
-        if (it.halves == 2) {
-          if (t == 1) {
-            ok = wait(&sm.turn[0][warp & 3], turns & 1, sm, err, 61);
-          } else if (turns > 0) {
-            ok = wait(&sm.turn[1][warp & 3], (turns - 1) & 1, sm, err, 61);
-          }
-          if (!ok) break;
-        }
-        const float neg = m == -INFINITY ? 0.0f : -m;  // a row that has seen no key yet
-        const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), neg2 = pair(neg, neg);
-        uint64_t sum[2] = {0, 0};
-#pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          load(c);
+          const float neg = m == -INFINITY ? 0.0f : -m;  // a row that has seen no key yet
+          const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), neg2 = pair(neg, neg);
+          uint64_t sum[2] = {0, 0};
           uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
@@ -977,18 +963,15 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             pk[e] = pack2<T>(p0, p1);
           }
           FPB_TMEM_ST32(s_base + 32 * c, pk);
+          const float2 part = unpair(add2(sum[0], sum[1]));
+          l += part.x + part.y;
           // The first 64 keys go ahead to the tensor core.
           tmemStoreWait();
           tcFenceBefore();
           __syncwarp();
           if (lane == 0) mbarArrive(c == 0 ? &sm.p_half[t] : &sm.p_full[t]);
         }
-        if (it.halves == 2) {
-          if (lane == 0) mbarArrive(&sm.turn[t][warp & 3]);
-          ++turns;
-        }
-        const float2 part = unpair(add2(sum[0], sum[1]));
-        l += part.x + part.y;
+        if (!ok) break;
       }
       if (ok) ok = wait(&sm.pv_done[t], (count - 1) & 1, sm, err, 59);
       if (!ok) break;

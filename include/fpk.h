@@ -303,7 +303,7 @@ FP_API int fpk_attention(const void* qkv, long long qkv_plane_stride, int qkv_la
 #define FPK_ERROR_PAGE 42   /* a page number outside the cache: its keys were treated as masked */
 #define FPK_ERROR_STARTS 43 /* starts that decrease or pass the buffer: clamped */
 #define FPK_ERROR_LENGTH 44 /* a length outside [0, table_pages*page_rows]: clamped */
-/* 51..61: a bounded wait inside the tensor-core kernel ran out; the tile was not stored. */
+/* 51..60: a bounded wait inside the tensor-core kernel ran out; the tile was not stored. */
 
 typedef struct fpk_heads {
   void* data;
