@@ -360,7 +360,8 @@ typedef struct fpk_kv_cache {
  * 448*scale, 1 for a row of zeros; elements are rounded to nearest even, and an
  * infinity or NaN is kept as NaN and does not count in the maximum. Reading
  * rounds value*scale to the rows' type, saturating at its largest finite value.
- * A slot that is written twice in one call holds a mixture of the two rows. */
+ * A slot that is written twice in one call holds a mixture of the two rows.
+ * kv_heads is at most 4096 here. */
 typedef struct fpk_cache_copy_desc {
   fpk_kv_cache_t cache;
   fpk_heads_t k, v;
@@ -410,7 +411,10 @@ FP_API int fpk_attention_packed(const fpk_attention_packed_desc_t* desc, void* s
  * fpk_attention_packed, with key j of sequence s in row j % page_rows of page
  * page_table[s*table_pages + j / page_rows] and kv_lengths[s] keys. Any number
  * of query rows per sequence: one, or a chunk. Entries of the table past a
- * sequence's last page are not read. */
+ * sequence's last page are not read. The v_scale of the keys that one query
+ * sees lie within a factor of 2^90: sums of weights are kept in their units.
+ * E4M3 elements beyond the range of FP16 rows may count as fpk_cache_read gives
+ * them. */
 typedef struct fpk_attention_paged_desc {
   fpk_heads_t q, out;
   fpk_kv_cache_t cache;

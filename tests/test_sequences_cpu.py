@@ -124,3 +124,9 @@ def test_rotary_frequencies():
     for bad in (dict(rotary_dim=3), dict(rotary_dim=4, factor=0), dict(rotary_dim=4, slow_turns=5, fast_turns=2)):
         with pytest.raises(ValueError):
             K.rotary_frequencies(**bad)
+
+
+def test_cache_copies_of_too_many_heads_are_refused(fl):
+    for call in (K.cache_write, K.cache_read):
+        with pytest.raises(K.FpkError, match="sizes"):
+            call(fl, copy(cache=cache(kv_heads=4097)))
