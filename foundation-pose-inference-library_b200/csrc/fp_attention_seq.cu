@@ -14,6 +14,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct Shape {
   int q_heads, kv_heads, head_dim, n_seq, q_rows;
+  long long keys;  // of a sequence: paged at most, packed four times the average
 };
 
 std::string shapeProblem(const Shape& n) {
@@ -36,16 +37,28 @@ float scaleLog2(float scale, int head_dim) {
   return kLog2e * (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(head_dim)));
 }
 
-// Rows (tokens x query heads to a key head) of a sequence on average, the
-// longest that the streaming kernel takes. Lengths are on the device, so the
-// choice goes by the average; either kernel is right for any lengths.
-constexpr int kStreamMostRows = 64;
+// Which kernel, by what the host knows (lengths are on the device; either kernel
+// is right for any). Rows are tokens x query heads to a key head, on average.
+// Up to 16 rows are one tile of the streaming kernel, which reads the keys at
+// the memory's rate; with more it reads them again for each 16 rows, while the
+// tile kernel takes 256 at once but begins at some 18 us. Streaming against tiles
+// (us, 8 key heads of 128, sequences x keys): 16 rows, 8 x 4000: 33 / 40, 8 x
+// 16000: 87 / 113; 48 rows, 8 x 4000: 52 / 39; 64 rows, 1 x 600: 11.8 / 19.0, 8 x
+// 600: 20.0 / 19.5, 1 x 4000: 21.2 / 31.4, 8 x 4000: 59 / 38; 128 rows, 1 x 600:
+// 12.7 / 20.3, 8 x 600: 30 / 22, 1 x 4000: 28 / 33; 1,600 rows, 4 key heads, 1 x
+// 400: 27 / 19.
+constexpr int kStreamMostRows = kStreamRows;
+constexpr int kStreamMostWork = 1 << 17;  // tiles of 16 rows x keys
 
 bool useTiles(const Shape& n) {
-  return static_cast<long long>(n.q_rows) * (n.q_heads / n.kv_heads) > static_cast<long long>(kStreamMostRows) * n.n_seq;
+  const long long rows = static_cast<long long>(n.q_rows) * (n.q_heads / n.kv_heads);  // below 2^31
+  if (n.n_seq == 0 || rows <= static_cast<long long>(kStreamMostRows) * n.n_seq) return false;
+  const double tiles = std::ceil(static_cast<double>(rows) / (static_cast<double>(kStreamRows) * n.n_seq)) * n.n_seq * n.kv_heads;
+  return tiles * static_cast<double>(n.keys) > kStreamMostWork;
 }
 
-long long workspaceBytes(const Shape& n) { return useTiles(n) ? tilesWorkspaceBytes(n.head_dim) : streamWorkspaceBytes(n.head_dim); }
+// Enough for either kernel: a workspace for one batch does for any other.
+long long workspaceBytes(const Shape& n) { return std::max(tilesWorkspaceBytes(n.head_dim), streamWorkspaceBytes(n.head_dim)); }
 
 int launch(const std::string& name, const Args& a, KvKind kind, const Shape& n, int dtype, void* stream) {
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -60,8 +73,8 @@ std::string workspaceProblem(const void* p, long long have, long long need) {
   return std::string();
 }
 
-Shape shapeOf(const fpk_attention_packed_desc_t& d) { return {d.q_heads, d.kv_heads, d.head_dim, d.n_seq, d.q_rows}; }
-Shape shapeOf(const fpk_attention_paged_desc_t& d) { return {d.q_heads, d.cache.kv_heads, d.cache.head_dim, d.n_seq, d.q_rows}; }
+Shape shapeOf(const fpk_attention_packed_desc_t& d) { return {d.q_heads, d.kv_heads, d.head_dim, d.n_seq, d.q_rows, d.n_seq > 0 ? std::min<long long>(d.kv_rows, 4LL * d.kv_rows / d.n_seq) : 0}; }
+Shape shapeOf(const fpk_attention_paged_desc_t& d) { return {d.q_heads, d.cache.kv_heads, d.cache.head_dim, d.n_seq, d.q_rows, static_cast<long long>(d.table_pages) * d.cache.page_rows}; }
 
 }  // namespace
 

@@ -46,7 +46,9 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnitKeys = 64;     // one unit of the split: 16 keys of each warp
-constexpr int kMinUnits = 4;      // a CTA takes at least 256 keys
+// Shares of 128 keys or more. One token over 6,000 keys: 16.9 us with 64, 14.4
+// with 128, 15.0 with 256, 17.2 with 512.
+constexpr int kMinUnits = 2;
 constexpr float kGrowLog2 = 8.0f;
 constexpr int kClusterKeys = 512;  // a cluster's most keys to a CTA
 
@@ -765,17 +767,18 @@ namespace {
 
 // CTAs to a tile where sequences are at most max_keys long, 0: even shares of
 // the line instead, joined by a second launch. A cluster grows while all CTAs run
-// at once and have two units or more, and is taken where none of its CTAs gets
-// more than kClusterKeys keys. Measured with 8 key heads, clusters against shares
-// (us): 4 x 64 keys 4.4 / 14.2, 4 x 1000 (128 keys to a CTA) 9.7 / 12.7, 4 x 2000
-// (256) 12.7 / 14.8, 32 x 500 (512) 15.3 / 20.9, 1 x 4000 (512) 13.2 / 13.2, 16 x
-// 2000 (1024) 29.2 / 20.0, 8 x 4000 (1024) 28.4 / 18.9.
+// at once and have two units or more, but up to 256 keys stay one CTA's (4 x 256
+// keys 7.0 us, with two CTAs 7.6), and is taken where none of its CTAs gets more
+// than kClusterKeys keys. Measured with 8 key heads, clusters against shares (us):
+// 4 x 64 keys 4.4 / 14.2, 4 x 1000 (128 keys to a CTA) 9.7 / 12.7, 4 x 2000 (256)
+// 12.7 / 14.8, 32 x 500 (512) 15.3 / 20.9, 1 x 4000 (512) 13.2 / 13.2, 16 x 2000
+// (1024) 29.2 / 20.0, 8 x 4000 (1024) 28.4 / 18.9.
 int clusterOf(const Args& a, int max_keys, int resident) {
   if (a.n_seq > kThreads) return 0;  // each thread looks at one sequence
   const long long tiles = (static_cast<long long>(a.q_rows) * a.group / kStreamRows + a.n_seq) * a.kv_heads;
   if (tiles > 0x7fffffffLL / 8) return 0;
   int n = 1;
-  while (n < 8 && 2 * n * tiles <= resident && 2 * n * 2 * kUnitKeys <= max_keys) n *= 2;
+  while (n < 8 && max_keys > 4 * kUnitKeys && 2 * n * tiles <= resident && 2 * n * 2 * kUnitKeys <= max_keys) n *= 2;
   return max_keys <= n * kClusterKeys ? n : 0;
 }
 

@@ -67,12 +67,18 @@ constexpr uint32_t kPlane = kKeys * 16;       // 128 rows of 8 channels
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
 constexpr float kGrowLog2 = 8.0f;
-constexpr int kTileCost = 384;   // a tile's work beside its keys, in keys
-constexpr int kMinShare = 256;   // keys
+// A tile's work beside its keys, in keys (of 192 to 384 none is better).
+constexpr int kTileCost = 384;
+// Least share, in keys. One prompt of 100 rows: 13.6 us with 256, 17.6 with 512.
+constexpr int kMinShare = 256;
 // Smallest piece of a page, in rows, for bulk copies: their issue takes some 70
-// cycles each whatever the size.
-constexpr int kBulkRows = 64;
-constexpr int kSnap = 8;         // a tile shorter than 1/8 share is not cut
+// cycles each whatever the size. Four chunks over 12,000 keys, bulk against 16
+// bytes at a time (us): pages of 16 rows 259 / 196, of 32 193 / 216, of 64 205 /
+// 217, of 128 191 / 214.
+constexpr int kBulkRows = 32;
+// A tile shorter than 1/8 share is not cut. Crops (short tiles) 150 us, 155 if
+// all are cut; at 1/2 chunks over pages lose 10 % to uneven shares.
+constexpr int kSnap = 8;
 
 struct Item {
   int halves;                  // halves with rows; 0: no more work

@@ -386,9 +386,12 @@ FP_API int fpk_cache_read(const fpk_cache_copy_desc_t* desc, void* stream);
  * the tensor cores with probabilities rounded to the element type; scores,
  * softmax statistics and sums are fp32. An infinity or NaN in V reaches, besides the
  * queries that see its key, those of its tile whose causal mask hides it.
- * workspace (fpk_attention_packed_workspace_bytes, 16-byte aligned, needs no
- * initialising) holds the partial results of sequences that are split over
- * several CTAs; calls that may overlap on the GPU need one each. */
+ * How far sequences are split over the GPU follows the sizes in the descriptor,
+ * so the last bits may; for one descriptor and lengths they do not change.
+ * workspace (fpk_attention_packed_workspace_bytes, the same for every batch of
+ * one head_dim, 16-byte aligned, needs no initialising) holds the partial results
+ * of sequences that are split over several CTAs; calls that may overlap on the
+ * GPU need one each. */
 typedef struct fpk_attention_packed_desc {
   fpk_heads_t q, k, v, out;
   int q_heads, kv_heads, head_dim, n_seq;
