@@ -1,6 +1,6 @@
 // Attention of few query rows over many keys (decoding): fpk_attention_paged
-// and fpk_attention_packed where a sequence has at most a few dozen query rows
-// (tokens x query heads to a key head).
+// and fpk_attention_packed where a sequence has at most 16 query rows (tokens x
+// query heads to a key head), or there is little work in all.
 //
 // Bound by the keys' and values' bytes, each read once from HBM, so everything
 // serves the stream of loads:
@@ -17,7 +17,7 @@
 // * e4m3 records become fp16 (exact) in registers. The key's scale multiplies
 //   its scores; the value's scale v joins the exponent: P' = 2^(s + log2 v - m),
 //   O = sum P' code, l = sum P'/v, so P' is at most 2^8 whatever the scales are
-//   (rows of one sequence may differ by up to 2^126). Queries become fp16 with a
+//   (rows of one sequence may differ by up to 2^90). Queries become fp16 with a
 //   power of two taken out of each row, exact down to 2^-14 of its maximum.
 // * Softmax in one pass, statistics and sums in fp32. A row's reference m moves
 //   only when a score exceeds it by 2^8, a warp vote, so most steps need no
@@ -28,6 +28,12 @@
 //   second launch joins in order (deterministic, no atomics).
 // * Short sequences instead take a cluster of CTAs for each tile, which share its
 //   keys out evenly and join over distributed shared memory: no second launch.
+//
+// Measured (32 query heads over 8 key heads of 128, bf16): one token of each of 8
+// sequences of 8,000 to 131,072 keys 167 us over e4m3 (941 MB, 5.6 TB/s; 86 % of
+// the copy rate: unpacking the codes takes half of the issue slots) and 284 us
+// over 16 bits (1.82 GB, 6.4 TB/s: the copy rate); of each of 4 sequences of 40 to
+// 1,000 keys 9.7 us, launch and latency.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

@@ -1,6 +1,6 @@
 // Attention of many query rows (prompts, chunks over a cache) on tcgen05 tensor
 // cores: fpk_attention_packed and fpk_attention_paged where a sequence has more
-// than a few dozen query rows (tokens x query heads to a key head).
+// than 16 query rows (tokens x query heads to a key head) and there is enough work.
 //
 // Bound by the tensor cores (4 d FLOP for each query row and key) and, as
 // closely, by the exponential unit: for d = 128 a 128 x 128 block of scores
@@ -39,6 +39,15 @@
 // few long rows all end together. A tile cut inside leaves fp32 partials that a
 // second launch joins in order; where tiles are short against a share, cuts
 // move to tile ends and nothing is joined. All mbarrier waits are bounded.
+//
+// Measured: 4 causal prompts of 700 to 8,192 tokens, 16 heads over 2 of 128, bf16,
+// 555 us = 936 TFLOP/s, without a mask 970; 252 sequences of 400, 4 heads of 128,
+// fp16, 150 us = 551 TFLOP/s (a fifth of the rows of its tiles are empty). A block of 128 keys takes some 3,900 cycles
+// for the 256 rows, of 2,048 that either the tensor core or the exponentials
+// need: each half waits for its scores (1,200), then for its own 2 x 64
+// exponentials (2,400, the other half's among them). Tried and not kept: the
+// halves in turns, a quarter of the exponentials as polynomials (slower by 3 to 8
+// %), both halves of a block unrolled with loads ahead (no gain, crops 8 % slower).
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

@@ -15,6 +15,8 @@
 //           rows, a thread owns its row's whole head and reads it twice (the
 //           second time from L1) instead of holding it; the angles of the 32
 //           rows are a table in shared memory that the block's heads share.
+// Measured: 16,384 tokens of 40 heads of 128, bf16, normalised, rows: 69 us = 4.9
+// TB/s (62 % of the issue slots, 50 % of DRAM); 5,003 rows of 8 heads, planar, 8 us.
 #include <cmath>
 #include <cstdint>
 #include <string>
