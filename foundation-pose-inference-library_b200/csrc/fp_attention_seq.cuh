@@ -83,7 +83,7 @@ __device__ __forceinline__ int pageOf(const Args& a, int s, int key) {
 // Work that the launch helpers cannot see on the host (lengths live on the
 // device) is bounded by these.
 constexpr int kStreamCtas = 592;  // most CTAs of the streaming kernel: 4 on each of 148 SMs
-constexpr int kStreamRows = 16;   // query rows of its tile
+constexpr int kStreamRows = 16;   // most query rows of its tile
 
 constexpr int kTileCtas = 148;    // most CTAs of the tile kernel: one on each SM
 constexpr int kTileRows = 256;    // query rows of its tile

@@ -6,14 +6,16 @@
 // serves the stream of loads:
 // * Each warp streams steps of 16 keys through its own ring in shared memory
 //   (cp.async; no barrier between warps), deep enough that some 100 KB an SM are
-//   under way. From there 16-byte records become matrix fragments (mma m16n8k16,
-//   16 query rows) as they are: a contraction does not care for the order of its
-//   index, so scores contract the 8 channels of a record in two products, and a
-//   score column c of 8-column block j stands for key 8j + 4(c%2) + c/2, so that
-//   a thread's four probabilities belong to keys t, 4+t, 8+t, 12+t (t = lane%4)
-//   and its four value records, one of each key and of plane lane/4, need only
-//   a byte permute to become fragments of the second product. The planes
-//   of a step are padded so that both readings are free of bank conflicts.
+//   under way. From there 16-byte records become matrix fragments (mma m16n8k16)
+//   as they are, keys and values always the operand of 16 rows, so that 8 query
+//   rows fill a product: S^T = K Q^T with 16 keys, O^T = V^T P^T with 16 channels.
+//   A contraction does not care for the order of its index: scores contract the 8
+//   channels of a record in two products, and score row g of 8-key block j stands
+//   for key 8j + 4(g%2) + g/2, so that, once P is transposed (movmatrix), a
+//   thread's probabilities belong to keys t, 4+t, 8+t, 12+t (t = lane%4) and its
+//   four value records, one of each key and of plane lane/4, need only a byte
+//   permute to become fragments. The planes of a step are padded so that both
+//   readings are free of bank conflicts.
 // * e4m3 records become fp16 (exact) in registers. The key's scale multiplies
 //   its scores; the value's scale v joins the exponent: P' = 2^(s + log2 v - m),
 //   O = sum P' code, l = sum P'/v, so P' is at most 2^8 whatever the scales are
@@ -30,10 +32,9 @@
 //   keys out evenly and join over distributed shared memory: no second launch.
 //
 // Measured (32 query heads over 8 key heads of 128, bf16): one token of each of 8
-// sequences of 8,000 to 131,072 keys 167 us over e4m3 (941 MB, 5.6 TB/s; 86 % of
-// the copy rate: unpacking the codes takes half of the issue slots) and 284 us
-// over 16 bits (1.82 GB, 6.4 TB/s: the copy rate); of each of 4 sequences of 40 to
-// 1,000 keys 9.7 us, launch and latency.
+// sequences of 8,000 to 131,072 keys 151 us over e4m3 (941 MB, 6.2 TB/s, 95 % of
+// the copy rate; 164 under the power cap) and 278 us over 16 bits (1.82 GB, the
+// copy rate); of each of 4 sequences of 40 to 1,000 keys 8.9 us, launch and latency.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -130,6 +131,13 @@ __device__ __forceinline__ float loadShared4(uint32_t at) {
   return v;
 }
 
+// An 8 x 8 matrix of 16-bit elements, two of row lane/4 to a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 // From another CTA of the cluster.
 __device__ __forceinline__ float4 loadCluster16(uint32_t at) {
   float4 v;
@@ -168,9 +176,10 @@ struct Step {
 
 }  // namespace
 
-template <typename T, int D, KvKind kKind, bool kCluster>
+template <typename T, int D, KvKind kKind, int R, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args a, int cluster) {
   constexpr bool kE4m3 = kKind == kPagedE4m3;
+  constexpr int kCols = R / 8;  // blocks of 8 query rows
   using S = Step<D, kE4m3>;
   using M = std::conditional_t<kE4m3, __half, T>;  // type of the products
   extern __shared__ __align__(16) unsigned char ring_raw[];
@@ -197,11 +206,11 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
   auto unitsOf = [&](int s, Sequence* out) -> long long {
     const Sequence q = sequence<kKind>(a, s);
     if (out != nullptr) *out = q;
-    const long long tiles = (q.nq * a.group + kStreamRows - 1) / kStreamRows;
+    const long long tiles = (q.nq * a.group + R - 1) / R;
     return tiles * a.kv_heads * max((q.nk + kUnitKeys - 1) / kUnitKeys, 1);  // no keys: still zeros to write
   };
   if constexpr (kCluster) {
-    // Tiles of sequence s have the numbers q0 * group / 16 + s + 0, 1, ...: apart
+    // Tiles of sequence s have the numbers q0 * group / R + s + 0, 1, ...: apart
     // from those of the next, whatever the lengths are. Starts that overlap (an
     // error) give all CTAs of a cluster the same one: the last.
     rank = static_cast<int>(tc::clusterCtaRank());
@@ -212,14 +221,14 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
     __syncthreads();
     if (tid < a.n_seq) {  // at most kThreads sequences: clusterOf()
       const Sequence c = sequence<kKind>(a, tid);
-      const int tile = number - c.q0 * a.group / kStreamRows - tid;
-      if (tile >= 0 && tile < (c.nq * a.group + kStreamRows - 1) / kStreamRows) atomicMax(&owner_s, tid);
+      const int tile = number - c.q0 * a.group / R - tid;
+      if (tile >= 0 && tile < (c.nq * a.group + R - 1) / R) atomicMax(&owner_s, tid);
     }
     __syncthreads();
     if (owner_s < 0) return;  // a number without a tile: the whole cluster leaves
     seq = owner_s;
     q = sequence<kKind>(a, seq);
-    cluster_tile = number - q.q0 * a.group / kStreamRows - seq;
+    cluster_tile = number - q.q0 * a.group / R - seq;
   } else {
     // Units of kThreads sequences and their sums up to each thread's.
     long long mine = 0, at = 0, total = 0;
@@ -292,24 +301,23 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
       b0 = static_cast<int>(u - tile_first);
       b1 = static_cast<int>(min(static_cast<long long>(blocks), end - tile_first));
     }
-    const int rows = min(kStreamRows, q.nq * a.group - tile * kStreamRows);
+    const int rows = min(R, q.nq * a.group - tile * R);
 
-    // Rows g and g + 8 of the tile.
-    int vis[2];
-    const unsigned char* qp[2];
+    // This thread's score columns are rows 8 n + 2t and 8 n + 2t + 1 of the tile.
+    int vis[kCols][2];
     int min_vis = q.nk;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int rr = g + 8 * i;
-      const int r = tile * kStreamRows + rr;  // below 2^31: checked by the host
-      const int token = r / q_heads_per;
-      vis[i] = rr < rows ? visible(a, q, token) : q.nk;
-      qp[i] = rr < rows ? record(a.q, head * q_heads_per + r - token * q_heads_per, q.q0 + token, 0) : nullptr;
-      min_vis = min(min_vis, vis[i]);
-    }
-    const int last_vis = visible(a, q, (tile * kStreamRows + rows - 1) / q_heads_per);
+    for (int n = 0; n < kCols; ++n) {
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) min_vis = min(min_vis, __shfl_xor_sync(0xffffffffu, min_vis, o));
+      for (int i = 0; i < 2; ++i) {
+        const int rr = 8 * n + 2 * t + i;  // tile * R + rr is below 2^31: checked by the host
+        vis[n][i] = rr < rows ? visible(a, q, (tile * R + rr) / q_heads_per) : q.nk;
+        min_vis = min(min_vis, vis[n][i]);
+      }
+    }
+    const int last_vis = visible(a, q, (tile * R + rows - 1) / q_heads_per);
+    min_vis = min(min_vis, __shfl_xor_sync(0xffffffffu, min_vis, 1));
+    min_vis = min(min_vis, __shfl_xor_sync(0xffffffffu, min_vis, 2));
 
     // Steps of 16 keys, one warp after the other, up to the last visible key.
     const int step_end = min(b1 * (kUnitKeys / 16), (last_vis + 15) >> 4);
@@ -317,6 +325,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
     const uint32_t ring = tc::smemU32(ring_raw) + warp * S::kDepth * S::kBytes;
     // This lane copies row lane%16 of planes lane/16, 2 + lane/16, ...
     const int copy_row = lane & 15, copy_plane = lane >> 4;
+    const int row_key = 4 * (g & 1) + (g >> 1);
     uint32_t bad_steps = 0;  // by ring place: the step's page does not exist
     int page_next = 0;
     auto pageAt = [&](int step) -> int {
@@ -369,61 +378,65 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
     page_next = pageAt(step_first);
 #pragma unroll
     for (int i = 0; i < S::kDepth - 1; ++i) copyStep(step_first + i * kWarps, i);
-    // Query fragments: the records of the channels that this thread's K records hold.
-    uint32_t qf[D / 16][4];
-    float row_scale[2] = {1.0f, 1.0f};
-    {
-      uint4 raw[2][D / 32];
+    // Query fragments: of row g of each block the channels that this thread's K records hold.
+    uint32_t qf[kCols][D / 16][2];
+    float row_scale[kCols][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+    for (int c = 0; c < kCols; ++c) {
+      const int r = tile * R + 8 * c + g;
+      const int token = r / q_heads_per;
+      const unsigned char* qp = 8 * c + g < rows ? record(a.q, head * q_heads_per + r - token * q_heads_per, q.q0 + token, 0) : nullptr;
+      uint4 raw[D / 32];
 #pragma unroll
-        for (int n = 0; n < D / 32; ++n) {
-          const int plane = kE4m3 ? 2 * (4 * (n / 2) + t) + n % 2 : 4 * n + t;
-          raw[i][n] = qp[i] != nullptr ? *reinterpret_cast<const uint4*>(qp[i] + plane * a.q.plane_stride) : make_uint4(0, 0, 0, 0);
-        }
+      for (int n = 0; n < D / 32; ++n) {
+        const int plane = kE4m3 ? 2 * (4 * (n / 2) + t) + n % 2 : 4 * n + t;
+        raw[n] = qp != nullptr ? *reinterpret_cast<const uint4*>(qp + plane * a.q.plane_stride) : make_uint4(0, 0, 0, 0);
       }
       if constexpr (kE4m3) {
+        float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float m = 0.0f;
+        for (int n = 0; n < D / 32; ++n) {
+          float x[8];
+          unpack8<T>(raw[n], x);
 #pragma unroll
-          for (int n = 0; n < D / 32; ++n) {
-            float x[8];
-            unpack8<T>(raw[i][n], x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
-          }
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          // 2^(exponent of m), kept where its inverse is a normal number.
-          const int e = min(max((__float_as_int(m) >> 23) & 0xff, 1), 253) - 127;
-          row_scale[i] = m > 0.0f ? __int_as_float((e + 127) << 23) : 1.0f;
-          const float inv = m > 0.0f ? __int_as_float((127 - e) << 23) : 1.0f;
-#pragma unroll
-          for (int n = 0; n < D / 32; ++n) {
-            float x[8];
-            unpack8<T>(raw[i][n], x);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) x[c] *= inv;
-            raw[i][n] = pack8<__half>(x);
-          }
+          for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
         }
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        // 2^(exponent of m), kept where its inverse is a normal number.
+        const int e = min(max((__float_as_int(m) >> 23) & 0xff, 1), 253) - 127;
+        const float mine = m > 0.0f ? __int_as_float((e + 127) << 23) : 1.0f;
+        const float inv = m > 0.0f ? __int_as_float((127 - e) << 23) : 1.0f;
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+          float x[8];
+          unpack8<T>(raw[n], x);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] *= inv;
+          raw[n] = pack8<__half>(x);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) row_scale[c][i] = __shfl_sync(0xffffffffu, mine, (2 * t + i) * 4) * a.scale_log2;
       }
 #pragma unroll
       for (int n = 0; n < D / 32; ++n) {
-        const uint4 lo = raw[0][n], hi = raw[1][n];
-        qf[2 * n][0] = lo.x, qf[2 * n][1] = hi.x, qf[2 * n][2] = lo.y, qf[2 * n][3] = hi.y;
-        qf[2 * n + 1][0] = lo.z, qf[2 * n + 1][1] = hi.z, qf[2 * n + 1][2] = lo.w, qf[2 * n + 1][3] = hi.w;
+        qf[c][2 * n][0] = raw[n].x, qf[c][2 * n][1] = raw[n].y;
+        qf[c][2 * n + 1][0] = raw[n].z, qf[c][2 * n + 1][1] = raw[n].w;
       }
     }
 
-    float o[S::kVRecords][S::kVCh][4];
+    float o[kCols][S::kVRecords][S::kVCh / 2][4];
 #pragma unroll
-    for (int i = 0; i < S::kVRecords; ++i) {
+    for (int c = 0; c < kCols; ++c) {
 #pragma unroll
-      for (int e = 0; e < S::kVCh; ++e) o[i][e][0] = o[i][e][1] = o[i][e][2] = o[i][e][3] = 0.0f;
+      for (int i = 0; i < S::kVRecords; ++i) {
+#pragma unroll
+        for (int e = 0; e < S::kVCh / 2; ++e) o[c][i][e][0] = o[c][i][e][1] = o[c][i][e][2] = o[c][i][e][3] = 0.0f;
+      }
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float m[kCols][2], l[kCols][2];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) m[c][0] = m[c][1] = -INFINITY, l[c][0] = l[c][1] = 0.0f;
 
     int place = 0;
     for (int step = step_first; step < step_end; step += kWarps) {
@@ -432,99 +445,109 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
       const uint32_t from = ring + place * S::kBytes;
       const int key0 = step * 16;
       const int lim = (bad_steps >> place) & 1u ? 0 : min(16, last_vis - key0);
-      float ks[4] = {}, vs[4] = {};
+      // Keys row_key and 8 + row_key of the step: rows g and g + 8 of its scores.
+      float ks[2] = {}, vs[2] = {};
       if constexpr (kE4m3) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          ks[c] = loadShared4(from + S::kScales + (4 * c + t) * 4);
-          vs[c] = loadShared4(from + S::kScales + 64 + (4 * c + t) * 4);
+        for (int j = 0; j < 2; ++j) {
+          ks[j] = loadShared4(from + S::kScales + (8 * j + row_key) * 4);
+          vs[j] = loadShared4(from + S::kScales + 64 + (8 * j + row_key) * 4);
         }
       }
-      float sc[2][4] = {};
+      float sc[kCols][4] = {};
+      const uint32_t k_at = from + t * S::kKPlane + row_key * 16;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t at = from + t * S::kKPlane + (8 * j + 4 * (g & 1) + (g >> 1)) * 16;
+      for (int n = 0; n < S::kKRecords; ++n) {
+        const uint4 k0 = loadShared16(k_at + 4 * n * S::kKPlane), k1 = loadShared16(k_at + 4 * n * S::kKPlane + 128);
+        if constexpr (kE4m3) {
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-        for (int n = 0; n < S::kKRecords; ++n) {
-          const uint4 k = loadShared16(at + 4 * n * S::kKPlane);
-          if constexpr (kE4m3) {
-            const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+          for (int e = 0; e < 4; ++e) {
+            const uint2 h0 = halves(w0[e]), h1 = halves(w1[e]);
+            const uint32_t f[4] = {h0.x, h1.x, h0.y, h1.y};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint2 h = halves(w[e]);
-              mma<M>(sc[j], qf[4 * n + e], h.x, h.y);
-            }
-          } else {
-            mma<M>(sc[j], qf[2 * n], k.x, k.y);
-            mma<M>(sc[j], qf[2 * n + 1], k.z, k.w);
+            for (int c = 0; c < kCols; ++c) mma<M>(sc[c], f, qf[c][4 * n + e][0], qf[c][4 * n + e][1]);
+          }
+        } else {
+          const uint32_t f0[4] = {k0.x, k1.x, k0.y, k1.y}, f1[4] = {k0.z, k1.z, k0.w, k1.w};
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            mma<M>(sc[c], f0, qf[c][2 * n][0], qf[c][2 * n][1]);
+            mma<M>(sc[c], f1, qf[c][2 * n + 1][0], qf[c][2 * n + 1][1]);
           }
         }
       }
-      float x[2][4];  // [row][key t, 4+t, 8+t, 12+t], log2 domain
-      float inv_v[4];
+      float x[kCols][2][2];  // [block][key j][row i], log2 domain
+      float inv_v[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int j = 0; j < 2; ++j) {
+        const int ve = (__float_as_int(vs[j]) >> 23) - 127;
+        inv_v[j] = __int_as_float((127 - ve) << 23);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float s = sc[c >> 1][2 * i + (c & 1)];
-          if constexpr (kE4m3) {
-            const int ve = (__float_as_int(vs[c]) >> 23) - 127;
-            x[i][c] = fmaf(s * row_scale[i], ks[c] * a.scale_log2, static_cast<float>(ve));
-            inv_v[c] = __int_as_float((127 - ve) << 23);
-          } else {
-            x[i][c] = s * a.scale_log2;
+        for (int c = 0; c < kCols; ++c) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float s = sc[c][2 * j + i];
+            x[c][j][i] = kE4m3 ? fmaf(s * row_scale[c][i], ks[j], static_cast<float>(ve)) : s * a.scale_log2;
           }
         }
       }
       if (key0 + lim > min_vis || lim < 16) {  // the causal edge, the last keys, a bad page
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int j = 0; j < 2; ++j) {
+          const int key = 8 * j + row_key;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (4 * c + t >= lim || key0 + 4 * c + t >= vis[i]) x[i][c] = -INFINITY;
-          }
-        }
-      }
-      bool grow = false;
-      float mx[2];
+          for (int c = 0; c < kCols; ++c) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mx[i] = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
-        grow |= mx[i] > m[i] + kGrowLog2;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-          const float m_new = fmaxf(m[i], mx[i]);
-          const float f = m[i] == m_new ? 1.0f : exp2Approx(m[i] - m_new);  // -inf stays: nothing to scale
-          m[i] = m_new;
-          l[i] *= f;
-#pragma unroll
-          for (int r = 0; r < S::kVRecords; ++r) {
-#pragma unroll
-            for (int e = 0; e < S::kVCh; ++e) {
-              o[r][e][2 * i] *= f;
-              o[r][e][2 * i + 1] *= f;
+            for (int i = 0; i < 2; ++i) {
+              if (key >= lim || key0 + key >= vis[c][i]) x[c][j][i] = -INFINITY;
             }
           }
         }
       }
-      uint32_t p[4];
+      bool grow = false;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float neg = m[i] == -INFINITY ? 0.0f : -m[i];  // a row that has seen no key yet
-        float e[4];
+      for (int c = 0; c < kCols; ++c) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          e[c] = exp2Approx(x[i][c] + neg);
-          l[i] = kE4m3 ? fmaf(e[c], inv_v[c], l[i]) : l[i] + e[c];
-        }
-        p[i] = pack2<M>(e[0], e[1]);
-        p[2 + i] = pack2<M>(e[2], e[3]);
+        for (int i = 0; i < 2; ++i) grow |= fmaxf(x[c][0][i], x[c][1][i]) > m[c][i] + kGrowLog2;
       }
-      // O += P V. Byte permutes bring two keys of one channel together.
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float m_new = fmaxf(m[c][i], fmaxf(x[c][0][i], x[c][1][i]));
+#pragma unroll
+            for (int z = 4; z < 32; z <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, z));
+            const float f = m[c][i] == m_new ? 1.0f : exp2Approx(m[c][i] - m_new);  // -inf stays: nothing to scale
+            m[c][i] = m_new;
+            l[c][i] *= f;
+#pragma unroll
+            for (int r = 0; r < S::kVRecords; ++r) {
+#pragma unroll
+              for (int e = 0; e < S::kVCh / 2; ++e) {
+                o[c][r][e][i] *= f;
+                o[c][r][e][2 + i] *= f;
+              }
+            }
+          }
+        }
+      }
+      uint32_t p[kCols][2];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        float neg[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) neg[i] = m[c][i] == -INFINITY ? 0.0f : -m[c][i];  // a row that has seen no key yet
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float e0 = exp2Approx(x[c][j][0] + neg[0]), e1 = exp2Approx(x[c][j][1] + neg[1]);
+          l[c][0] = kE4m3 ? fmaf(e0, inv_v[j], l[c][0]) : l[c][0] + e0;
+          l[c][1] = kE4m3 ? fmaf(e1, inv_v[j], l[c][1]) : l[c][1] + e1;
+          p[c][j] = transpose8x8(pack2<M>(e0, e1));  // from keys x rows to rows x keys
+        }
+      }
+      // O^T += V^T P^T. Byte permutes bring two keys of one channel together.
 #pragma unroll
       for (int i = 0; i < S::kVRecords; ++i) {
         if constexpr (kE4m3) {
@@ -544,10 +567,12 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
             // Codes of keys 0, 1 (2, 3) side by side, then two channels to a word.
             const uint2 a0 = halves(__byte_perm(v[0][e / 4], v[1][e / 4], 0x5140)), a1 = halves(__byte_perm(v[0][e / 4], v[1][e / 4], 0x7362));
             const uint2 c0 = halves(__byte_perm(v[2][e / 4], v[3][e / 4], 0x5140)), c1 = halves(__byte_perm(v[2][e / 4], v[3][e / 4], 0x7362));
-            mma<M>(o[i][e], p, a0.x, c0.x);
-            mma<M>(o[i][e + 1], p, a0.y, c0.y);
-            mma<M>(o[i][e + 2], p, a1.x, c1.x);
-            mma<M>(o[i][e + 3], p, a1.y, c1.y);
+            const uint32_t f0[4] = {a0.x, a0.y, c0.x, c0.y}, f1[4] = {a1.x, a1.y, c1.x, c1.y};
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              mma<M>(o[c][i][e / 2], f0, p[c][0], p[c][1]);
+              mma<M>(o[c][i][e / 2 + 1], f1, p[c][0], p[c][1]);
+            }
           }
         } else {
           uint32_t v[4][4];
@@ -557,10 +582,11 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
             v[kk][0] = w.x, v[kk][1] = w.y, v[kk][2] = w.z, v[kk][3] = w.w;
           }
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const uint32_t h0 = v[0][e >> 1], h1 = v[1][e >> 1], h2 = v[2][e >> 1], h3 = v[3][e >> 1];
-            mma<M>(o[i][e], p, __byte_perm(h0, h1, 0x5410), __byte_perm(h2, h3, 0x5410));
-            mma<M>(o[i][e + 1], p, __byte_perm(h0, h1, 0x7632), __byte_perm(h2, h3, 0x7632));
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t f[4] = {__byte_perm(v[0][e], v[1][e], 0x5410), __byte_perm(v[0][e], v[1][e], 0x7632),
+                                   __byte_perm(v[2][e], v[3][e], 0x5410), __byte_perm(v[2][e], v[3][e], 0x7632)};
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) mma<M>(o[c][i][e], f, p[c][0], p[c][1]);
           }
         }
       }
@@ -574,19 +600,22 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
 
     // ---- join the warps ----
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      if (t == 0) {
-        ml_s[warp][0][g + 8 * i] = m[i];
-        ml_s[warp][1][g + 8 * i] = l[i];
-      }
+    for (int c = 0; c < kCols; ++c) {
 #pragma unroll
-      for (int r = 0; r < S::kVRecords; ++r) {
+      for (int i = 0; i < 2; ++i) {
+        const int rr = 8 * c + 2 * t + i;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int z = 4; z < 32; z <<= 1) l[c][i] += __shfl_xor_sync(0xffffffffu, l[c][i], z);
+        if (g == 0) {
+          ml_s[warp][0][rr] = m[c][i];
+          ml_s[warp][1][rr] = l[c][i];
+        }
 #pragma unroll
-          for (int e = 0; e < S::kVCh; ++e) o_s[warp][g + 8 * i][(8 * r + 2 * t + n) * S::kVCh + e] = o[r][e][2 * i + n];
+        for (int r = 0; r < S::kVRecords; ++r) {
+#pragma unroll
+          for (int e = 0; e < S::kVCh / 2; ++e) {
+            *reinterpret_cast<float2*>(&o_s[warp][rr][(8 * r + g) * S::kVCh + 2 * e]) = make_float2(o[c][r][e][i], o[c][r][e][2 + i]);
+          }
         }
       }
     }
@@ -599,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
     } else {
       part = partials + (2 * static_cast<size_t>(blockIdx.x) + (first_piece && b0 > 0 ? 0 : 1)) * partialFloats(D);
     }
-    for (int i = tid; i < kStreamRows * (D / 8); i += kThreads) {
+    for (int i = tid; i < R * (D / 8); i += kThreads) {
       const int rr = i / (D / 8), grp = i % (D / 8);
       if (rr >= rows) continue;
       float mm = -INFINITY;
@@ -618,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] *= inv;
-        const int r = tile * kStreamRows + rr;  // below 2^31: checked by the host
+        const int r = tile * R + rr;  // below 2^31: checked by the host
         const int token = r / q_heads_per;
         const int h = head * q_heads_per + r - token * q_heads_per;
         *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(acc);
@@ -653,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
           const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= inv;
-          const int r = tile * kStreamRows + rr;
+          const int r = tile * R + rr;
           const int token = r / q_heads_per;
           *reinterpret_cast<uint4*>(record(a.out, head * q_heads_per + r - token * q_heads_per, q.q0 + token, grp)) = pack8<T>(x);
         }
@@ -685,7 +714,7 @@ constexpr int kJoinWarps = 16;
 
 // Joins the partials of a tile that several CTAs worked on: CTA c looks after
 // the tile in which share c begins, if it is the first share to begin there.
-template <typename T, int D, KvKind kKind>
+template <typename T, int D, KvKind kKind, int R>
 __global__ void __launch_bounds__(kJoinWarps * 32) joinStreamKernel(const Args a) {
   __shared__ float acc_s[kJoinWarps][D];
   __shared__ float ml_s[kJoinWarps][2];
@@ -758,7 +787,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) joinStreamKernel(const Args a
     const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= inv;
-    const int r = split.tile * kStreamRows + rr;
+    const int r = split.tile * R + rr;
     const int token = r / a.group;
     const int h = split.head * a.group + r - token * a.group;
     *reinterpret_cast<uint4*>(record(a.out, h, q.q0 + token, grp)) = pack8<T>(x);
@@ -779,22 +808,23 @@ namespace {
 // 4 x 64 keys 4.4 / 14.2, 4 x 1000 (128 keys to a CTA) 9.7 / 12.7, 4 x 2000 (256)
 // 12.7 / 14.8, 32 x 500 (512) 15.3 / 20.9, 1 x 4000 (512) 13.2 / 13.2, 16 x 2000
 // (1024) 29.2 / 20.0, 8 x 4000 (1024) 28.4 / 18.9.
-int clusterOf(const Args& a, int max_keys, int resident) {
+long long numbersOf(const Args& a, int rows) { return (static_cast<long long>(a.q_rows) * a.group / rows + a.n_seq) * a.kv_heads; }
+
+int clusterOf(const Args& a, long long tiles, int max_keys, int resident) {
   if (a.n_seq > kThreads) return 0;  // each thread looks at one sequence
-  const long long tiles = (static_cast<long long>(a.q_rows) * a.group / kStreamRows + a.n_seq) * a.kv_heads;
   if (tiles > 0x7fffffffLL / 8) return 0;
   int n = 1;
   while (n < 8 && max_keys > 4 * kUnitKeys && 2 * n * tiles <= resident && 2 * n * 2 * kUnitKeys <= max_keys) n *= 2;
   return max_keys <= n * kClusterKeys ? n : 0;
 }
 
-template <typename T, int D, KvKind kKind>
+template <typename T, int D, KvKind kKind, int R>
 cudaError_t launchOne(const Args& a, int max_keys, cudaStream_t s) {
   constexpr int kRing = Step<D, kKind == kPagedE4m3>::kRing;
   static DeviceOnce smem_attr;
   const cudaError_t ae = smem_attr.run([] {
-    const cudaError_t e = cudaFuncSetAttribute(attentionStreamKernel<T, D, kKind, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(attentionStreamKernel<T, D, kKind, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+    const cudaError_t e = cudaFuncSetAttribute(attentionStreamKernel<T, D, kKind, R, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(attentionStreamKernel<T, D, kKind, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing);
   });
   if (ae != cudaSuccess) return ae;
   // As many CTAs as stay resident, so that equal shares end together.
@@ -802,11 +832,11 @@ cudaError_t launchOne(const Args& a, int max_keys, cudaStream_t s) {
   const int ctas = resident.get([](int dev) {
     int sms = 148, per = 1;
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attentionStreamKernel<T, D, kKind, false>, kThreads, kRing);
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, attentionStreamKernel<T, D, kKind, R, false>, kThreads, kRing);
     return std::min(kStreamCtas, sms * std::max(per, 1));
   });
-  if (const int cluster = clusterOf(a, max_keys, ctas); cluster > 0) {
-    const long long tiles = (static_cast<long long>(a.q_rows) * a.group / kStreamRows + a.n_seq) * a.kv_heads;
+  const long long tiles = numbersOf(a, R);
+  if (const int cluster = clusterOf(a, tiles, max_keys, ctas); cluster > 0) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -820,20 +850,29 @@ cudaError_t launchOne(const Args& a, int max_keys, cudaStream_t s) {
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     prof::countLaunch(prof::kAttention);
-    return cudaLaunchKernelEx(&cfg, attentionStreamKernel<T, D, kKind, true>, a, cluster);
+    return cudaLaunchKernelEx(&cfg, attentionStreamKernel<T, D, kKind, R, true>, a, cluster);
   }
   prof::countLaunch(prof::kAttention, 2);
-  cudaError_t e = launchPdl(attentionStreamKernel<T, D, kKind, false>, dim3(ctas), dim3(kThreads), kRing, s, a, 0);
+  cudaError_t e = launchPdl(attentionStreamKernel<T, D, kKind, R, false>, dim3(ctas), dim3(kThreads), kRing, s, a, 0);
   if (e != cudaSuccess) return e;
-  return launchPdl(joinStreamKernel<T, D, kKind>, dim3(ctas), dim3(kJoinWarps * 32), 0, s, a);
+  return launchPdl(joinStreamKernel<T, D, kKind, R>, dim3(ctas), dim3(kJoinWarps * 32), 0, s, a);
+}
+
+// Rows of a tile: 8 where sequences have at most 8 on average, else 16. One row
+// over 8 x 131,072 e4m3 keys (4 rows a tile): 151 us, with tiles of 16 172; 16 rows:
+// 178 in one tile of 16.
+template <typename T, int D, KvKind kKind>
+cudaError_t launchRows(const Args& a, int max_keys, cudaStream_t s) {
+  const bool few = static_cast<long long>(a.q_rows) * a.group <= 8LL * a.n_seq;
+  return few ? launchOne<T, D, kKind, 8>(a, max_keys, s) : launchOne<T, D, kKind, 16>(a, max_keys, s);
 }
 
 template <typename T, int D>
 cudaError_t launchKind(const Args& a, KvKind kind, int max_keys, cudaStream_t s) {
   switch (kind) {
-    case kPacked16: return launchOne<T, D, kPacked16>(a, max_keys, s);
-    case kPaged16: return launchOne<T, D, kPaged16>(a, max_keys, s);
-    default: return launchOne<T, D, kPagedE4m3>(a, max_keys, s);
+    case kPacked16: return launchRows<T, D, kPacked16>(a, max_keys, s);
+    case kPaged16: return launchRows<T, D, kPaged16>(a, max_keys, s);
+    default: return launchRows<T, D, kPagedE4m3>(a, max_keys, s);
   }
 }
 
