@@ -47,7 +47,8 @@
 // need: each half waits for its scores (1,200), then for its own 2 x 64
 // exponentials (2,400, the other half's among them). Tried and not kept: the
 // halves in turns, a quarter of the exponentials as polynomials (slower by 3 to 8
-// %), both halves of a block unrolled with loads ahead (no gain, crops 8 % slower).
+// %), both halves of a block unrolled with loads ahead (no gain, crops 8 % slower),
+// two threads to a row in 16 warps of 80 registers (13 to 30 % slower).
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
