@@ -1,5 +1,6 @@
 // Host side of fpk_attention_packed and fpk_attention_paged (include/fpk.h):
 // checks and the choice of the kernel.
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -73,8 +74,14 @@ std::string workspaceProblem(const void* p, long long have, long long need) {
   return std::string();
 }
 
-Shape shapeOf(const fpk_attention_packed_desc_t& d) { return {d.q_heads, d.kv_heads, d.head_dim, d.n_seq, d.q_rows, d.n_seq > 0 ? std::min<long long>(d.kv_rows, 4LL * d.kv_rows / d.n_seq) : 0}; }
-Shape shapeOf(const fpk_attention_paged_desc_t& d) { return {d.q_heads, d.cache.kv_heads, d.cache.head_dim, d.n_seq, d.q_rows, static_cast<long long>(d.table_pages) * d.cache.page_rows}; }
+Shape shapeOf(const fpk_attention_packed_desc_t& d) {
+  const long long keys = d.n_seq > 0 ? std::min<long long>(d.kv_rows, 4LL * d.kv_rows / d.n_seq) : 0;
+  return {d.q_heads, d.kv_heads, d.head_dim, d.n_seq, d.q_rows, keys};
+}
+Shape shapeOf(const fpk_attention_paged_desc_t& d) {
+  const long long keys = static_cast<long long>(d.table_pages) * d.cache.page_rows;
+  return {d.q_heads, d.cache.kv_heads, d.cache.head_dim, d.n_seq, d.q_rows, keys};
+}
 
 }  // namespace
 
