@@ -48,7 +48,9 @@
 // exponentials (2,400, the other half's among them). Tried and not kept: the
 // halves in turns, a quarter of the exponentials as polynomials (slower by 3 to 8
 // %), both halves of a block unrolled with loads ahead (no gain, crops 8 % slower),
-// two threads to a row in 16 warps of 80 registers (13 to 30 % slower).
+// two threads to a row in 16 warps of 80 registers (13 to 30 % slower), scores of 64
+// keys two parts ahead in either half of their columns (prompts the same, crops
+// 164: a product with 64 keys takes 53 cycles for half of the 64 that 128 take).
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
