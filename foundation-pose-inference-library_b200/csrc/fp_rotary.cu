@@ -15,8 +15,9 @@
 //           rows, a thread owns its row's whole head and reads it twice (the
 //           second time from L1) instead of holding it; the angles of the 32
 //           rows are a table in shared memory that the block's heads share.
-// Measured: 16,384 tokens of 40 heads of 128, bf16, normalised, rows: 69 us = 4.9
-// TB/s (62 % of the issue slots, 50 % of DRAM); 5,003 rows of 8 heads, planar, 8 us.
+// Measured: 16,384 tokens of 40 heads of 128, bf16, normalised, rows: 63 us = 5.3
+// TB/s, 81 % of the copy rate (sharing the angles between a warp's heads changes
+// nothing: it waits for memory); 5,003 rows of 8 heads, planar, 8 us.
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -54,12 +55,12 @@ __device__ __forceinline__ float2 turn(int position, float inv_freq, float scale
 }
 
 constexpr int kRowsWarps = 4;
-constexpr int kBatch = 4;  // heads in flight per lane group
+// Heads in flight per lane group: 16,384 tokens of 40 heads take 63 us with 2, 68
+// with 4 (fewer warps fit), 66 with 2 that are loaded ahead of the angles.
+constexpr int kBatch = 2;
 
 // A lane holds two groups of a head: the two that a pair of channels lies in
-// (half layout), so that nothing is exchanged, or two neighbours. The norm's
-// weight is folded into the angles once per token: with u = w c and v = w' s a
-// pair costs a product, an fma and the product with r.
+// (half layout), so that nothing is exchanged, or two neighbours.
 template <typename T>
 __global__ void __launch_bounds__(kRowsWarps * 32) rotaryRowsKernel(const Args a, int lanes) {
   tc::pdlTrigger();
