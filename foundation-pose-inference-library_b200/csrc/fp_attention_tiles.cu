@@ -503,6 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         const int k_stage = (sc.block & 1) * 2, v_stage = (pv.block & 1) * 2 + 1;
         // All that the next scores need is waited for before P: their MMAs then
         // follow the products' at once (some 450 cycles of a block's 4,100).
+        // The tensor core takes them in this order, so the scores may overwrite P.
         if (scores) {
           if (sc.j == sc.jb) {
             ok = wait(&sm.q_ready[t], tiles & 1, sm, err, 56);
