@@ -12,6 +12,8 @@ namespace seqattn {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr long long kMostKeys = (1LL << 31) - 1024;  // key counts round up to blocks in 32 bits
+constexpr const char* kMisaligned = "starts, lengths, page_table and error_flag must be 4-byte aligned";
 
 struct Shape {
   int q_heads, kv_heads, head_dim, n_seq, q_rows;
@@ -108,6 +110,7 @@ extern "C" int fpk_attention_packed(const fpk_attention_packed_desc_t* d, void* 
   std::string p = shapeProblem(n);
   if (p.empty()) p = scaleProblem(d->scale);
   if (p.empty() && d->kv_rows < 0) p = "sizes must not be negative";
+  if (p.empty() && d->kv_rows > kMostKeys) p = "kv_rows must be at most 2^31 - 1024";
   if (!p.empty()) return fail(name + ": " + p);
   if (d->n_seq == 0 || d->q_rows == 0) return 0;
   for (const fpk_heads_t* v : {&d->q, &d->out, &d->k, &d->v}) {
@@ -115,6 +118,7 @@ extern "C" int fpk_attention_packed(const fpk_attention_packed_desc_t* d, void* 
     if (const char* q = headsProblem(*v)) return fail(name + ": " + q);
   }
   if (d->q_starts == nullptr || d->kv_starts == nullptr) return fail(name + ": q_starts and kv_starts are required");
+  if (!aligned4(d->q_starts) || !aligned4(d->kv_starts) || !aligned4(d->error_flag)) return fail(name + ": " + kMisaligned);
   p = workspaceProblem(d->workspace, d->workspace_bytes, workspaceBytes(n));
   if (p.empty()) p = deviceProblem(d->q.data);
   if (!p.empty()) return fail(name + ": " + p);
@@ -149,7 +153,7 @@ extern "C" int fpk_attention_paged(const fpk_attention_paged_desc_t* d, void* st
   if (p.empty()) p = shapeProblem(n);
   if (p.empty()) p = scaleProblem(d->scale);
   if (p.empty() && d->table_pages < 0) p = "sizes must not be negative";
-  if (p.empty() && static_cast<long long>(d->table_pages) * d->cache.page_rows >= (1LL << 31)) p = "table_pages * page_rows must be below 2^31";
+  if (p.empty() && n.keys > kMostKeys) p = "table_pages * page_rows must be at most 2^31 - 1024";
   if (!p.empty()) return fail(name + ": " + p);
   if (d->n_seq == 0 || d->q_rows == 0) return 0;
   for (const fpk_heads_t* v : {&d->q, &d->out}) {
@@ -157,6 +161,9 @@ extern "C" int fpk_attention_paged(const fpk_attention_paged_desc_t* d, void* st
   }
   if (d->q_starts == nullptr || d->kv_lengths == nullptr || (d->page_table == nullptr && d->table_pages > 0)) {
     return fail(name + ": q_starts, kv_lengths and page_table are required");
+  }
+  if (!aligned4(d->q_starts) || !aligned4(d->kv_lengths) || !aligned4(d->page_table) || !aligned4(d->error_flag)) {
+    return fail(name + ": " + kMisaligned);
   }
   p = workspaceProblem(d->workspace, d->workspace_bytes, workspaceBytes(n));
   if (p.empty()) p = deviceProblem(d->q.data);

@@ -152,6 +152,9 @@ __device__ __forceinline__ void reportIndex(int* error_flag, int code) {
 
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// Arrays of int32 or float (NULL passes): a misaligned one would fault in the kernel.
+inline bool aligned4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+
 // nullptr if the heads can be addressed, else what is wrong with them.
 inline const char* headsProblem(const fpk_heads_t& v) {
   if (v.data == nullptr) return "null pointer";
@@ -168,6 +171,7 @@ inline std::string cacheProblem(const fpk_kv_cache_t& c, int dtype) {
   if (!aligned16(c.k) || !aligned16(c.v)) return "the cache must be 16-byte aligned";
   if (c.dtype != FPK_DTYPE_E4M3 && c.dtype != dtype) return "a 16-bit cache must have the rows' type";
   if (c.dtype == FPK_DTYPE_E4M3 && (c.k_scale == nullptr || c.v_scale == nullptr)) return "an e4m3 cache needs k_scale and v_scale";
+  if (!aligned4(c.k_scale) || !aligned4(c.v_scale)) return "k_scale and v_scale must be 4-byte aligned";
   if (c.head_dim != 64 && c.head_dim != 128) return "head_dim must be 64 or 128";
   if (c.page_rows < 16 || c.page_rows > 1024 || (c.page_rows & (c.page_rows - 1)) != 0) {
     return "page_rows must be a power of two from 16 to 1024";

@@ -394,6 +394,7 @@ int copy(const char* name, const fpk_cache_copy_desc_t* d, bool write, void* str
     if (const char* q = headsProblem(*v)) return fail(std::string(name) + ": " + q);
   }
   if (d->slots == nullptr) return fail(std::string(name) + ": slots are required");
+  if (!aligned4(d->slots) || !aligned4(d->error_flag)) return fail(std::string(name) + ": slots and error_flag must be 4-byte aligned");
   const std::string where = deviceProblem(d->cache.k);
   if (!where.empty()) return fail(std::string(name) + ": " + where);
   Args a{};

@@ -308,6 +308,9 @@ extern "C" int fpk_qk_norm_rotary(const fpk_qk_rotary_desc_t* d, void* stream) {
   if (d->rotary_dim > 0 && (d->positions == nullptr || d->inv_freq == nullptr)) {
     return fail("fpk_qk_norm_rotary: positions and inv_freq are required");
   }
+  if (!heads::aligned4(d->positions) || !heads::aligned4(d->inv_freq) || !heads::aligned4(d->q_weight) || !heads::aligned4(d->k_weight)) {
+    return fail("fpk_qk_norm_rotary: positions, inv_freq and weights must be 4-byte aligned");
+  }
   if ((d->q_weight != nullptr || d->k_weight != nullptr) && !(d->eps >= 0.0f)) return fail("fpk_qk_norm_rotary: eps must not be negative");
   const std::string where = heads::deviceProblem(d->q_heads > 0 ? d->q.data : d->k.data);
   if (!where.empty()) return fail("fpk_qk_norm_rotary: " + where);

@@ -381,7 +381,7 @@ FP_API int fpk_cache_read(const fpk_cache_copy_desc_t* desc, void* stream);
  * the sequence's, or with causal != 0 keys 0 .. kv_length - q_length + i for its
  * query i (the last query sees the last key). A query that sees no key gets
  * zeros. Rows of no sequence are neither read into a result nor written, whatever they
- * hold. scale 0 means 1/sqrt(head_dim). head_dim is 64 or 128, q_heads a
+ * hold. At most 2^31 - 1024 keys. scale 0 means 1/sqrt(head_dim). head_dim is 64 or 128, q_heads a
  * multiple of kv_heads, at most 128 query heads to a key head. Products run on
  * the tensor cores with probabilities rounded to the element type; scores,
  * softmax statistics and sums are fp32. An infinity or NaN in V reaches, besides the

@@ -130,3 +130,22 @@ def test_cache_copies_of_too_many_heads_are_refused(fl):
     for call in (K.cache_write, K.cache_read):
         with pytest.raises(K.FpkError, match="sizes"):
             call(fl, copy(cache=cache(kv_heads=4097)))
+
+
+@pytest.mark.parametrize("call,make,change", [
+    (K.qk_norm_rotary, rotary, dict(positions=A + 2)), (K.qk_norm_rotary, rotary, dict(inv_freq=A + 1)), (K.qk_norm_rotary, rotary, dict(q_weight=A + 3)),
+    (K.cache_write, copy, dict(slots=A + 2)), (K.cache_read, copy, dict(error_flag=A + 1)),
+    (K.attention_packed, packed, dict(q_starts=A + 2)), (K.attention_packed, packed, dict(kv_starts=A + 1)),
+    (K.attention_packed, packed, dict(error_flag=A + 2)), (K.attention_paged, paged, dict(kv_lengths=A + 2)),
+    (K.attention_paged, paged, dict(page_table=A + 3)),
+    (K.attention_paged, paged, dict(cache=cache(dtype=E4M3, k_scale=A + 2, v_scale=A)))])
+def test_misaligned_arrays_are_refused(fl, call, make, change):
+    with pytest.raises(K.FpkError, match="4-byte aligned"):
+        call(fl, make(**change))
+
+
+def test_key_counts_that_would_overflow_are_refused(fl):
+    with pytest.raises(K.FpkError, match="2\\^31 - 1024"):
+        K.attention_packed(fl, packed(kv_rows=2 ** 31 - 1))
+    with pytest.raises(K.FpkError, match="2\\^31 - 1024"):
+        K.attention_paged(fl, paged(table_pages=(1 << 27) - 1))  # pages of 16 rows
