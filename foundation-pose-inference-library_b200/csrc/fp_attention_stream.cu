@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
           vs[j] = loadShared4(from + S::kScales + 64 + (8 * j + row_key) * 4);
         }
       }
-      float sc[kCols][4] = {};
+      float sc[kCols][4] = {}, sc1[kCols][4] = {};  // two chains, of half the latency each
       const uint32_t k_at = from + t * S::kKPlane + row_key * 16;
 #pragma unroll
       for (int n = 0; n < S::kKRecords; ++n) {
@@ -466,14 +466,14 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
             const uint2 h0 = halves(w0[e]), h1 = halves(w1[e]);
             const uint32_t f[4] = {h0.x, h1.x, h0.y, h1.y};
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) mma<M>(sc[c], f, qf[c][4 * n + e][0], qf[c][4 * n + e][1]);
+            for (int c = 0; c < kCols; ++c) mma<M>(e & 1 ? sc1[c] : sc[c], f, qf[c][4 * n + e][0], qf[c][4 * n + e][1]);
           }
         } else {
           const uint32_t f0[4] = {k0.x, k1.x, k0.y, k1.y}, f1[4] = {k0.z, k1.z, k0.w, k1.w};
 #pragma unroll
           for (int c = 0; c < kCols; ++c) {
             mma<M>(sc[c], f0, qf[c][2 * n][0], qf[c][2 * n][1]);
-            mma<M>(sc[c], f1, qf[c][2 * n + 1][0], qf[c][2 * n + 1][1]);
+            mma<M>(sc1[c], f1, qf[c][2 * n + 1][0], qf[c][2 * n + 1][1]);
           }
         }
       }
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         for (int c = 0; c < kCols; ++c) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float s = sc[c][2 * j + i];
+            const float s = sc[c][2 * j + i] + sc1[c][2 * j + i];
             x[c][j][i] = kE4m3 ? fmaf(s * row_scale[c][i], ks[j], static_cast<float>(ve)) : s * a.scale_log2;
           }
         }
