@@ -802,7 +802,8 @@ namespace {
 
 // CTAs to a tile where sequences are at most max_keys long, 0: even shares of
 // the line instead, joined by a second launch. A cluster grows while all CTAs run
-// at once and have two units or more, but up to 256 keys stay one CTA's (4 x 256
+// at once (8 hypothesis groups of 3 to 252 rows: 10.6 us with 2 CTAs to a tile,
+// 16.8 with 4 in two waves) and have two units or more, but up to 256 keys stay one CTA's (4 x 256
 // keys 7.0 us, with two CTAs 7.6), and is taken where none of its CTAs gets more
 // than kClusterKeys keys. Measured with 8 key heads, clusters against shares (us):
 // 4 x 64 keys 4.4 / 14.2, 4 x 1000 (128 keys to a CTA) 9.7 / 12.7, 4 x 2000 (256)
