@@ -45,11 +45,11 @@ float scaleLog2(float scale, int head_dim) {
 // Up to 16 rows are one tile of the streaming kernel, which reads the keys at
 // the memory's rate; with more it reads them again for each 16 rows, while the
 // tile kernel takes 256 at once but begins at some 18 us. Streaming against tiles
-// (us, 8 key heads of 128, sequences x keys): 16 rows, 8 x 4000: 33 / 40, 8 x
-// 16000: 87 / 113; 48 rows, 8 x 4000: 52 / 39; 64 rows, 1 x 600: 11.8 / 19.0, 8 x
-// 600: 20.0 / 19.5, 1 x 4000: 21.2 / 31.4, 8 x 4000: 59 / 38; 128 rows, 1 x 600:
-// 12.7 / 20.3, 8 x 600: 30 / 22, 1 x 4000: 28 / 33; 1,600 rows, 4 key heads, 1 x
-// 400: 27 / 19.
+// (us, 8 key heads of 128, sequences x keys): 16 rows, 8 x 4000: 33 / 39, 8 x
+// 16000: 86 / 113; 48 rows, 8 x 4000: 52 / 39; 64 rows, 1 x 600: 12.7 / 18.3, 8 x
+// 600: 20 / 20, 1 x 4000: 22 / 21, 8 x 4000: 59 / 38; 128 rows, 1 x 600: 13.5 /
+// 19.5, 8 x 600: 30 / 22, 1 x 4000: 28 / 22; 1,600 rows, 4 key heads, 1 x 400:
+// 27 / 20.
 constexpr int kStreamMostRows = kStreamRows;
 constexpr int kStreamMostWork = 1 << 17;  // tiles of 16 rows x keys
 
