@@ -663,6 +663,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
     }
     if constexpr (kCluster) {
       if (cluster > 1) {
+        __syncwarp();  // the barrier is one of whole warps, and lanes leave the loop apart
         tc::clusterSync();
         const uint32_t part_at = tc::smemU32(part), ml_at = tc::smemU32(&joined_s[0][0]);
         for (int i = rank * kThreads + tid; i < rows * (D / 8); i += cluster * kThreads) {
@@ -686,6 +687,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
           const int token = r / q_heads_per;
           *reinterpret_cast<uint4*>(record(a.out, head * q_heads_per + r - token * q_heads_per, q.q0 + token, grp)) = pack8<T>(x);
         }
+        __syncwarp();
         tc::clusterSync();  // no CTA leaves while another reads its memory
       }
       return;

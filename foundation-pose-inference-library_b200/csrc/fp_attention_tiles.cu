@@ -1002,10 +1002,10 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t ov[32];
+        __syncwarp();  // the load is one of a whole warp, and lanes without a row skip the stores
         FPB_TMEM_LD32(o_base + c, ov);
         tmemWaitLd();
-        if (!valid) continue;
-        if (part_at == nullptr) {
+        if (valid && part_at == nullptr) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             float x[8];
@@ -1018,7 +1018,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             }
             *reinterpret_cast<uint4*>(record(a.out, h, it.q0 + token, (c >> 3) + g)) = pack8<T>(x);
           }
-        } else {
+        } else if (valid) {
 #pragma unroll
           for (int g = 0; g < 8; ++g) {
             reinterpret_cast<uint4*>(part_at)[((c >> 2) + g) * kTileRows + tile_row] =
