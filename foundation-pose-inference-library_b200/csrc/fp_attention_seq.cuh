@@ -46,19 +46,19 @@ struct Sequence {
 template <KvKind kKind>
 __device__ __forceinline__ Sequence sequence(const Args& a, int s) {
   Sequence q;
-  const int b0 = __ldg(a.q_starts + s), b1 = __ldg(a.q_starts + s + 1);
+  const int b0 = a.q_starts[s], b1 = a.q_starts[s + 1];
   q.q0 = min(max(b0, 0), a.q_rows);
   const int q1 = min(max(b1, q.q0), a.q_rows);
   q.nq = q1 - q.q0;
   if (q.q0 != b0 || q1 != b1) reportIndex(a.error_flag, FPK_ERROR_STARTS);
   if constexpr (kKind == kPacked16) {
-    const int c0 = __ldg(a.kv_starts + s), c1 = __ldg(a.kv_starts + s + 1);
+    const int c0 = a.kv_starts[s], c1 = a.kv_starts[s + 1];
     q.k0 = min(max(c0, 0), a.kv_rows);
     const int k1 = min(max(c1, q.k0), a.kv_rows);
     q.nk = k1 - q.k0;
     if (q.k0 != c0 || k1 != c1) reportIndex(a.error_flag, FPK_ERROR_STARTS);
   } else {
-    const int n = __ldg(a.kv_lengths + s);
+    const int n = a.kv_lengths[s];
     q.k0 = 0;
     q.nk = static_cast<int>(min(static_cast<long long>(max(n, 0)), static_cast<long long>(a.table_pages) << a.page_shift));
     if (q.nk != n) reportIndex(a.error_flag, FPK_ERROR_LENGTH);
@@ -74,7 +74,7 @@ __device__ __forceinline__ int visible(const Args& a, const Sequence& q, int i) 
 
 // Page of key `key` of sequence s, or -1 if the table holds no page there.
 __device__ __forceinline__ int pageOf(const Args& a, int s, int key) {
-  const int p = __ldg(a.page_table + static_cast<long long>(s) * a.table_pages + (key >> a.page_shift));
+  const int p = a.page_table[static_cast<long long>(s) * a.table_pages + (key >> a.page_shift)];
   return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages) ? p : -1;
 }
 

@@ -746,10 +746,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) joinStreamKernel(const Args a
         const int i = i0 + x * per_row;
         const bool in = i < n;
         const float* p = partials + (2 * static_cast<size_t>(c0 + (in ? i : i0)) + ((in ? i : i0) == 0 ? 1 : 0)) * partialFloats(D);
-        pm[x] = in ? __ldcg(p + kStreamRows * D + row) : -INFINITY;
-        pl[x] = in ? __ldcg(p + kStreamRows * D + kStreamRows + row) : 0.0f;
+        pm[x] = in ? p[kStreamRows * D + row] : -INFINITY;
+        pl[x] = in ? p[kStreamRows * D + kStreamRows + row] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) po[x][e] = in ? __ldcg(p + row * D + e * 32 + lane) : 0.0f;
+        for (int e = 0; e < kPer; ++e) po[x][e] = in ? p[row * D + e * 32 + lane] : 0.0f;
       }
       const float top = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])), m);
       const float keep = m == top ? 1.0f : exp2Approx(m - top);

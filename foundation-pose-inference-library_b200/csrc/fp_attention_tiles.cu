@@ -779,10 +779,10 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         const unsigned char* src = static_cast<const unsigned char*>(v.data) + (next_in ? it.head * v.head_stride + page * a.page_stride + r * 16LL : 0);
 #pragma unroll
         for (int p = 0; p < kPlanes / 2; ++p) {
-          next_codes[p] = next_in ? __ldg(reinterpret_cast<const uint4*>(src + p * v.plane_stride)) : make_uint4(0, 0, 0, 0);
+          next_codes[p] = next_in ? *reinterpret_cast<const uint4*>(src + p * v.plane_stride) : make_uint4(0, 0, 0, 0);
         }
         const float* scales = side == 0 ? a.k_scale : a.v_scale;
-        next_scale = next_in ? __ldg(scales + (((static_cast<long long>(page) * a.kv_heads + it.head) << a.page_shift) + r)) : 0.0f;
+        next_scale = next_in ? scales[((static_cast<long long>(page) * a.kv_heads + it.head) << a.page_shift) + r] : 0.0f;
       };
       if constexpr (kKind == kPagedE4m3) fetch(it.jb, 0, __shfl_sync(0xffffffffu, page_next, thread >> 4));
 
@@ -1091,11 +1091,11 @@ __global__ void __launch_bounds__(kTileRows) joinTilesKernel(const Args a, int n
       for (int g = 0; g < kJoinGroups; ++g) {
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          y[i][g][z] = in ? __ldcg(reinterpret_cast<const float4*>(p) + (2 * (grp + g) + z) * kTileRows + row) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          y[i][g][z] = in ? reinterpret_cast<const float4*>(p)[(2 * (grp + g) + z) * kTileRows + row] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
       }
-      pm[i] = in ? __ldcg(p + kTileRows * D + row) : -INFINITY;
-      pl[i] = in ? __ldcg(p + kTileRows * D + kTileRows + row) : 0.0f;
+      pm[i] = in ? p[kTileRows * D + row] : -INFINITY;
+      pl[i] = in ? p[kTileRows * D + kTileRows + row] : 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < kJoinAhead; ++i) top = fmaxf(top, pm[i]);

@@ -2,6 +2,11 @@
 // behind fpk_qk_norm_rotary, fpk_cache_write / _read, fpk_attention_packed and
 // fpk_attention_paged share. Device addressing, 16-bit and e4m3 conversions,
 // and the host's checks of the descriptors (include/fpk.h).
+//
+// These kernels begin while the one before may still be writing what they will
+// read (fp_launch.hpp), so they read with plain loads behind the wait: a load
+// through the read-only path asks for memory that no one writes while the kernel
+// lives.
 #pragma once
 
 #include <cuda_bf16.h>

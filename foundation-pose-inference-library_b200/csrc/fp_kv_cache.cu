@@ -112,7 +112,7 @@ __device__ __forceinline__ float* cacheScale(const Args& a, int side, int slot, 
 
 // The row's slot, or -1 where it is left out.
 __device__ __forceinline__ int slotOf(const Args& a, int row) {
-  const int slot = __ldg(a.slots + row);
+  const int slot = a.slots[row];
   if (slot < 0) return -1;
   if (static_cast<uint32_t>(slot) >= a.total) {
     reportIndex(a.error_flag, FPK_ERROR_SLOT);
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) writeRowsKernel(const Args a) {
     const int row = n.row + i * n.step;
     const bool in = n.active && row < a.rows;
     slot[i] = in ? slotOf(a, row) : -1;
-    raw[i] = in ? __ldg(reinterpret_cast<const uint4*>(record(a.dense[n.side], n.head, row, n.group))) : make_uint4(0, 0, 0, 0);
+    raw[i] = in ? *reinterpret_cast<const uint4*>(record(a.dense[n.side], n.head, row, n.group)) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
@@ -242,11 +242,11 @@ __global__ void __launch_bounds__(kThreads) writePlanarKernel(const Args a) {
   if constexpr (kE4m3) {
     float m = 0.0f;
 #pragma unroll 8
-    for (int g = 0; g < kGroups; ++g) m = fmaxf(m, groupMax<T>(__ldg(reinterpret_cast<const uint4*>(src + g * step))));
+    for (int g = 0; g < kGroups; ++g) m = fmaxf(m, groupMax<T>(*reinterpret_cast<const uint4*>(src + g * step)));
     finite = m <= FLT_MAX;
     if (!finite) {
       m = 0.0f;
-      for (int g = 0; g < kGroups; ++g) m = fmaxf(m, groupFiniteMax<T>(__ldg(reinterpret_cast<const uint4*>(src + g * step))));
+      for (int g = 0; g < kGroups; ++g) m = fmaxf(m, groupFiniteMax<T>(*reinterpret_cast<const uint4*>(src + g * step)));
     }
     e = scaleExponent(m);
     *cacheScale(a, side, slot, head) = powerOfTwo(e);
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) writePlanarKernel(const Args a) {
   for (int g0 = 0; g0 < kGroups; g0 += 4) {
     uint4 raw[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) raw[g] = __ldg(reinterpret_cast<const uint4*>(src + (g0 + g) * step));
+    for (int g = 0; g < 4; ++g) raw[g] = *reinterpret_cast<const uint4*>(src + (g0 + g) * step);
     if constexpr (!kE4m3) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) *reinterpret_cast<uint4*>(dst + (g0 + g) * dst_step) = raw[g];

@@ -87,10 +87,10 @@ __global__ void __launch_bounds__(kRowsWarps * 32) rotaryRowsKernel(const Args a
     s[i] = 0.0f;
   }
   if (rotated) {
-    const int position = __ldg(a.positions + row);
+    const int position = a.positions[row];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 cs = turn(position, __ldg(a.inv_freq + k * 8 + i), a.scale);
+      const float2 cs = turn(position, a.inv_freq[k * 8 + i], a.scale);
       c[i] = cs.x;
       s[i] = cs.y;
     }
@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32) rotaryRowsKernel(const Args a
     float wa[8], wb[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      wa[i] = norm && has_a && n_heads > 0 ? __ldg(weight + ga * 8 + i) : 1.0f;
-      wb[i] = norm && has_b && n_heads > 0 ? __ldg(weight + gb * 8 + i) : 1.0f;
+      wa[i] = norm && has_a && n_heads > 0 ? weight[ga * 8 + i] : 1.0f;
+      wb[i] = norm && has_b && n_heads > 0 ? weight[gb * 8 + i] : 1.0f;
     }
     const int stride = gridDim.y * slots;
     // Uniform trip count: every lane takes part in the shuffles.
@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(kPlanarWarps * 32) rotaryPlanarKernel(const Ar
   const bool valid = row < a.rows;
   const int half = a.rotary_dim >> 1;
   if (half > 0) {
-    const int position = valid ? __ldg(a.positions + row) : 0;
-    for (int i = warp; i < half; i += kPlanarWarps) table[i * 32 + lane] = turn(position, __ldg(a.inv_freq + i), a.scale);
+    const int position = valid ? a.positions[row] : 0;
+    for (int i = warp; i < half; i += kPlanarWarps) table[i * 32 + lane] = turn(position, a.inv_freq[i], a.scale);
   }
   __syncthreads();
   if (!valid) return;
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kPlanarWarps * 32) rotaryPlanarKernel(const Ar
       unpack8<T>(*reinterpret_cast<const uint4*>(src + g * in.plane_stride), x);
       if (weight != nullptr) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * __ldg(weight + g * 8 + i);
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * weight[g * 8 + i];
       }
     };
     auto store = [&](int g, const float (&y)[8]) { *reinterpret_cast<uint4*>(dst + g * out.plane_stride) = pack8<T>(y); };
