@@ -18,9 +18,12 @@
 //   readings are free of bank conflicts.
 // * e4m3 records become fp16 (exact) in registers. The key's scale multiplies
 //   its scores; the value's scale v joins the exponent: P' = 2^(s + log2 v - m),
-//   O = sum P' code, l = sum P'/v, so P' is at most 2^8 whatever the scales are
-//   (rows of one sequence may differ by up to 2^90). Queries become fp16 with a
-//   power of two taken out of each row, exact down to 2^-14 of its maximum.
+//   O = sum P' code, l = sum P'/v, so P' is at most 2^8 whatever the scales are.
+//   A product with V keeps P' to 2^-25, so a key counts against the largest weight
+//   times value, not the largest weight. A row of zeros would set m by a scale
+//   that stands for nothing, and the others' P' would fall out of fp16: it counts
+//   as 2^-48 there, and its weight in l alone. Queries become fp16 with a power of
+//   two taken out of each row, exact down to 2^-14 of its maximum.
 // * Softmax in one pass, statistics and sums in fp32. A row's reference m moves
 //   only when a score exceeds it by 2^8, a warp vote, so most steps need no
 //   shuffle.
@@ -57,6 +60,8 @@ constexpr int kUnitKeys = 64;     // one unit of the split: 16 keys of each warp
 // with 128, 15.0 with 256, 17.2 with 512.
 constexpr int kMinUnits = 2;
 constexpr float kGrowLog2 = 8.0f;
+// e4m3: a row of zeros moves the reference only when its score is this far above.
+constexpr float kZerosLog2 = 48.0f;
 constexpr int kClusterKeys = 512;  // a cluster's most keys to a CTA
 
 // The tile that a CTA's range begins inside, for the joining launch.
@@ -512,6 +517,28 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         for (int i = 0; i < 2; ++i) grow |= fmaxf(x[c][0][i], x[c][1][i]) > m[c][i] + kGrowLog2;
       }
       if (__any_sync(0xffffffffu, grow)) {
+        // Keys whose values are all zeros (their scale says nothing): no word of
+        // theirs has a bit beside the signs. The four lanes of a score row share the planes.
+        bool zeros[2] = {false, false};
+        if constexpr (kE4m3) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int p = 0; p < S::kPlanes; p += 4) {
+              const uint4 w = loadShared16(from + S::kV + (p + t) * S::kVPlane + (8 * j + row_key) * 16);
+              any |= w.x | w.y | w.z | w.w;
+            }
+            any |= __shfl_xor_sync(0xffffffffu, any, 1);
+            any |= __shfl_xor_sync(0xffffffffu, any, 2);
+            zeros[j] = (any & 0x7f7f7f7fu) == 0;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              const float ve = static_cast<float>((__float_as_int(vs[j]) >> 23) - 127);
+              if (zeros[j]) x[c][j][0] -= ve + kZerosLog2, x[c][j][1] -= ve + kZerosLog2;
+            }
+          }
+        }
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
 #pragma unroll
@@ -528,6 +555,13 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
               for (int e = 0; e < S::kVCh / 2; ++e) {
                 o[c][r][e][i] *= f;
                 o[c][r][e][2 + i] *= f;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (kE4m3 && zeros[j] && x[c][j][i] != -INFINITY) {  // the weight alone, which may be past fp16
+                l[c][i] += exp2Approx(x[c][j][i] + kZerosLog2 - m_new);
+                x[c][j][i] = -INFINITY;
               }
             }
           }

@@ -414,10 +414,12 @@ FP_API int fpk_attention_packed(const fpk_attention_packed_desc_t* desc, void* s
  * fpk_attention_packed, with key j of sequence s in row j % page_rows of page
  * page_table[s*table_pages + j / page_rows] and kv_lengths[s] keys. Any number
  * of query rows per sequence: one, or a chunk. Entries of the table past a
- * sequence's last page are not read. The v_scale of the keys that one query
- * sees lie within a factor of 2^90: sums of weights are kept in their units.
- * E4M3 elements beyond the range of FP16 rows may count as fpk_cache_read gives
- * them. */
+ * sequence's last page are not read. E4M3: probabilities may be rounded to FP16
+ * in units of the v_scale, so that a key's product of weight and v_scale counts
+ * down to 2^-25 of the largest such product. The v_scale of the keys that one
+ * query sees lie within a factor of 2^90. A row of zeros counts as one of scale
+ * 2^-48 for both, whatever its scale is. E4M3 elements beyond the range of FP16
+ * rows may count as fpk_cache_read gives them. */
 typedef struct fpk_attention_paged_desc {
   fpk_heads_t q, out;
   fpk_kv_cache_t cache;

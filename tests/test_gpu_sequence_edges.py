@@ -7,11 +7,11 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from fp_b200 import kernels as K  # noqa: E402
-from seq_util import Cache, HeadRows, starts, within  # noqa: E402
-from test_gpu_sequences import copy_desc, flag, gen, paged_desc, reference, rotary_desc, run_packed, same_bits, stream  # noqa: E402
+from seq_util import DT, Cache, HeadRows, starts, within  # noqa: E402
+from test_gpu_sequences import copy_desc, flag, gen, paged_desc, reference, rotary_desc, run_packed, run_paged, same_bits, stream  # noqa: E402
 
 pytestmark = pytest.mark.gpu
-BF16 = K.FPK_DTYPE_BF16
+F16, BF16 = K.FPK_DTYPE_F16, K.FPK_DTYPE_BF16
 DEV = "cuda"
 
 
@@ -83,3 +83,61 @@ def test_calls_read_what_the_call_before_wrote(fpk, nq, e4m3, layout):
     for _ in range(5):
         for a, b in zip(run(False), want):
             assert same_bits(a, b)
+
+
+def one_cached(keys, k, v, dtype, page, g, e4m3=True):
+    """One sequence in a paged cache: (cache, table, length, slots)."""
+    pages = -(-keys // page)
+    cache = Cache(pages, page, k.shape[1], k.shape[2], dtype, e4m3)
+    table = torch.randperm(pages, device=DEV, generator=g).to(torch.int32)[None]
+    at = torch.arange(keys, device=DEV)
+    slots = table[0].long()[at // page] * page + at % page
+    cache.put(0, slots, k.to(DT[dtype]))
+    cache.put(1, slots, v.to(DT[dtype]))
+    return cache, table, torch.tensor([keys], dtype=torch.int32, device=DEV), slots
+
+
+def value_step(cache, slots):
+    """448 times the largest scale of a row of values that is not all zeros: what attention64's bound counts
+    the rounding of probabilities in. A row of zeros brings nothing to a product, whatever its scale is."""
+    values = cache.values(1, slots)
+    p, r = slots.long() // cache.page_rows, slots.long() % cache.page_rows
+    scale = cache.scale[1][p, :, r].double()
+    return 448.0 * float((scale * (values.abs().amax(-1) > 0)).max())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("nq,n", [(1, 300), (4, 300), (20, 300), (1, 20011), (150, 9000)])
+@pytest.mark.parametrize("size", [1e-2, 1e-3, 1e-5])
+@pytest.mark.parametrize("top", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_of_zeros_beside_small_values(fpk, dtype, nq, n, size, top, d):
+    """Values of `size` with some rows of zeros (their scale is 1, far above the others'), the first, the
+    last and more, which may have the highest scores. Values are positive, so that the bound is relative
+    to each output."""
+    hq, hk, page = 4, 2, 64
+    g = gen(nq + n)
+    q = HeadRows(nq, hq, d, dtype).set(0.75 + 0.5 * torch.rand(nq, hq, d, device=DEV, generator=g))
+    k = 0.3 * torch.randn(n, hk, d, device=DEV, generator=g)
+    v = size * (0.5 + torch.rand(n, hk, d, device=DEV, generator=g))
+    rows = torch.tensor([0, 1, 17, n // 2, n // 2 + 40, n - 1], device=DEV)
+    v[rows] = 0
+    v[3, 0], v[n // 3, 1] = 0, 0  # in one head only
+    if top:
+        k[rows] = 0.05 * 128 / d ** 0.5 + 0.1 * torch.rand(len(rows), hk, d, device=DEV, generator=g)
+    cache, table, length, slots = one_cached(n, k, v, dtype, page, g)
+    out, err = run_paged(fpk, q, cache, [nq], length, table, False, dtype)
+    ref, bound = reference(q, cache.values(0, slots), cache.values(1, slots), [nq], [n], False, d, dtype, v_step=value_step(cache, slots))
+    # fp16's own rounding of an output below its normal range.
+    bound = bound - 2.0 ** -24 + (2.0 ** -25 if dtype == F16 else 0.0)
+    assert err == 0 and within(out.get(), ref, bound) <= 1
+
+
+@pytest.mark.parametrize("nq,n", [(1, 300), (1, 20011), (150, 9000)])
+def test_only_rows_of_zeros(fpk, nq, n):
+    g = gen(n)
+    q = HeadRows(nq, 4, 128, BF16).set(torch.randn(nq, 4, 128, device=DEV, generator=g))
+    k = torch.randn(n, 2, 128, device=DEV, generator=g)
+    cache, table, length, _ = one_cached(n, k, torch.zeros_like(k), BF16, 64, g)
+    out, err = run_paged(fpk, q, cache, [nq], length, table, True, BF16)
+    assert err == 0 and torch.count_nonzero(out.get()) == 0
