@@ -18,14 +18,14 @@
 //   readings are free of bank conflicts.
 // * e4m3 records become fp16 (exact) in registers. The key's scale multiplies
 //   its scores; the value's scale v joins the exponent: P' = 2^(s + log2 v - m),
-//   O = sum P' code, l = sum P'/v, so P' is at most 2^8 whatever the scales are.
+//   O = sum P' code, l = sum P'/v, so P' is at most 2^15 whatever the scales are.
 //   A product with V keeps P' to 2^-25, so a key counts against the largest weight
 //   times value, not the largest weight. A row of zeros would set m by a scale
 //   that stands for nothing, and the others' P' would fall out of fp16: it counts
 //   as 2^-48 there, and its weight in l alone. Queries become fp16 with a power of
 //   two taken out of each row, exact down to 2^-14 of its maximum.
 // * Softmax in one pass, statistics and sums in fp32. A row's reference m moves
-//   only when a score exceeds it by 2^8, a warp vote, so most steps need no
+//   only when a score exceeds it by 2^15, a warp vote, so most steps need no
 //   shuffle.
 // * The key axis is split evenly: all (sequence, row tile, key head) units of 64
 //   keys form one line that the CTAs share out, each finding its part from the
@@ -59,7 +59,12 @@ constexpr int kUnitKeys = 64;     // one unit of the split: 16 keys of each warp
 // Shares of 128 keys or more. One token over 6,000 keys: 16.9 us with 64, 14.4
 // with 128, 15.0 with 256, 17.2 with 512.
 constexpr int kMinUnits = 2;
-constexpr float kGrowLog2 = 8.0f;
+// A row's reference lies 2^7 below the maximum it was set by and stays until a
+// score is 2^15 above it: probabilities up to 2^15 use fp16's range on both sides
+// of 1, so that weights down to 2^-32 of the largest reach a product (2^-25 with
+// the maximum itself as the reference).
+constexpr float kHeadLog2 = 7.0f;
+constexpr float kGrowLog2 = 15.0f;
 // e4m3: a row of zeros moves the reference only when its score is this far above.
 constexpr float kZerosLog2 = 48.0f;
 constexpr int kClusterKeys = 512;  // a cluster's most keys to a CTA
@@ -543,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         for (int c = 0; c < kCols; ++c) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float m_new = fmaxf(m[c][i], fmaxf(x[c][0][i], x[c][1][i]));
+            float m_new = fmaxf(m[c][i], fmaxf(x[c][0][i], x[c][1][i]) - kHeadLog2);
 #pragma unroll
             for (int z = 4; z < 32; z <<= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, z));
             const float f = m[c][i] == m_new ? 1.0f : exp2Approx(m[c][i] - m_new);  // -inf stays: nothing to scale

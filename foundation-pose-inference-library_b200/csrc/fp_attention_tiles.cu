@@ -13,7 +13,7 @@
 //                   row's 128 scores from TMEM, 64 at a time: running maximum
 //                   and sum in fp32, P = 2^(s - m) rounded to the element type
 //                   over the scores' own TMEM columns. O is rescaled only when a
-//                   row's maximum grows by more than 2^8. After the last, O / l.
+//                   row's maximum grows by more than 2^8 (reference: 2^7 below it). After the last, O / l.
 //   warps 8-11      loads of Q, K and V rows, K and V in four stages of 128 rows.
 //                   Two layouts in shared memory, each the one that its source
 //                   fills line by line (the other way round the copies take
@@ -78,7 +78,11 @@ constexpr uint32_t kChunk = kKeys * 128;      // 128 rows of 64 channels
 constexpr uint32_t kPlane = kKeys * 16;       // 128 rows of 8 channels
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
-constexpr float kGrowLog2 = 8.0f;
+// A row's reference lies 2^7 below the maximum it was set by and stays until a
+// score is 2^15 above it: fp16 probabilities down to 2^-32 of the largest reach
+// the products.
+constexpr float kHeadLog2 = 7.0f;
+constexpr float kGrowLog2 = 15.0f;
 // A tile's work beside its keys, in keys (of 192 to 384 none is better).
 constexpr int kTileCost = 384;
 // Least share, in keys. One prompt of 100 rows: 13.6 us with 256, 17.6 with 512.
@@ -949,9 +953,9 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           for (int e = 0; e < 64; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
           const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * a.scale_log2;
           if (j == it.jb && c == 0) {
-            m = top;
+            m = top - kHeadLog2;
           } else if (__any_sync(0xffffffffu, top > m + kGrowLog2)) {
-            const float m_new = top > m + kGrowLog2 ? top : m;
+            const float m_new = top > m + kGrowLog2 ? top - kHeadLog2 : m;
             const float f = m_new == m ? 1.0f : exp2Approx(m - m_new);
             // O takes in the products of the 64 keys before these.
             ok = wait(c == 0 ? &sm.pv_done[t] : &sm.pv_half[t], (c == 0 ? count - 1 : count) & 1, sm, err, 59);

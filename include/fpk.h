@@ -416,7 +416,7 @@ FP_API int fpk_attention_packed(const fpk_attention_packed_desc_t* desc, void* s
  * of query rows per sequence: one, or a chunk. Entries of the table past a
  * sequence's last page are not read. E4M3: probabilities may be rounded to FP16
  * in units of the v_scale, so that a key's product of weight and v_scale counts
- * down to 2^-25 of the largest such product. The v_scale of the keys that one
+ * down to 2^-32 of the largest such product. The v_scale of the keys that one
  * query sees lie within a factor of 2^90. A row of zeros counts as one of scale
  * 2^-48 for both, whatever its scale is. E4M3 elements beyond the range of FP16
  * rows may count as fpk_cache_read gives them. */

@@ -141,3 +141,38 @@ def test_only_rows_of_zeros(fpk, nq, n):
     cache, table, length, _ = one_cached(n, k, torch.zeros_like(k), BF16, 64, g)
     out, err = run_paged(fpk, q, cache, [nq], length, table, True, BF16)
     assert err == 0 and torch.count_nonzero(out.get()) == 0
+
+
+@pytest.mark.parametrize("nq,n", [(1, 300), (5, 900), (1, 20011), (150, 9000)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("cached", ["packed", "same", "e4m3"])
+def test_small_weights_beside_a_large_one_fp16(fpk, nq, n, d, first, cached):
+    """One key with a score 19 above the others (their weights are some 2^-27 of its) and small values: the
+    output is the others'. Their probabilities count to 2^-32 of the largest one: attention64's bound
+    with its 2^-25 taken by 2^-7."""
+    hq, hk = 4, 2
+    g = gen(n)
+    q = HeadRows(nq, hq, d, F16).set(torch.ones(nq, hq, d, device=DEV) + 0.05 * torch.randn(nq, hq, d, device=DEV, generator=g))
+    k = 0.05 * torch.randn(n, hk, d, device=DEV, generator=g)
+    v = 0.5 + torch.rand(n, hk, d, device=DEV, generator=g)
+    at = 0 if first else n - 1
+    k[at] += 19.0 / d ** 0.5
+    v[at] *= 2.0 ** -24
+    if cached == "packed":
+        kr, vr = HeadRows(n, hk, d, F16).set(k), HeadRows(n, hk, d, F16).set(v)
+        out, err = run_packed(fpk, q, kr, vr, [nq], [n], False, F16)
+        kk, vv, step = kr.get().double(), vr.get().double(), 1.5
+    else:
+        cache, table, length, slots = one_cached(n, k, v, F16, 64, g, cached == "e4m3")
+        out, err = run_paged(fpk, q, cache, [nq], length, table, False, F16)
+        kk, vv = cache.values(0, slots), cache.values(1, slots)
+        step = 1.5
+    if cached == "e4m3":  # units of a row's scale: the largest product of weight and scale is the bound's unit
+        p = torch.softmax(torch.einsum("qhd,khd->hqk", q.get().double(), kk.repeat_interleave(hq // hk, 1)) * d ** -0.5, -1)
+        pg, r = slots.long() // cache.page_rows, slots.long() % cache.page_rows
+        scale = cache.scale[1][pg, :, r].double().repeat_interleave(hq // hk, 1).T[:, None]
+        step = 448.0 * float((p * scale).max())
+    ref, bound = reference(q, kk, vv, [nq], [n], False, d, F16, v_step=step * 2.0 ** -7)
+    bound = bound - 2.0 ** -24 + 2.0 ** -25
+    assert err == 0 and within(out.get(), ref, bound) <= 1
