@@ -167,6 +167,10 @@ __device__ __forceinline__ uint2 halves(uint32_t four) {
   return r;
 }
 
+// A row's output. One that saw no key gets zeros, whatever the values held that
+// its tile's other rows saw.
+__device__ __forceinline__ float normalised(float o, float l) { return l == 0.0f ? 0.0f : o * (1.0f / l); }
+
 // Shapes of one 16-key step in a warp's ring.
 template <int D, bool kE4m3>
 struct Step {
@@ -683,9 +687,8 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         for (int e = 0; e < 8; ++e) acc[e] = fmaf(o_s[w][rr][grp * 8 + e], f, acc[e]);
       }
       if (whole) {
-        const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] *= inv;
+        for (int e = 0; e < 8; ++e) acc[e] = normalised(acc[e], ll);
         const int r = tile * R + rr;  // below 2^31: checked by the host
         const int token = r / q_heads_per;
         const int h = head * q_heads_per + r - token * q_heads_per;
@@ -719,9 +722,8 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = fmaf(v[e], f, x[e]);
           }
-          const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= inv;
+          for (int e = 0; e < 8; ++e) x[e] = normalised(x[e], l_all);
           const int r = tile * R + rr;
           const int token = r / q_heads_per;
           *reinterpret_cast<uint4*>(record(a.out, head * q_heads_per + r - token * q_heads_per, q.q0 + token, grp)) = pack8<T>(x);
@@ -825,9 +827,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) joinStreamKernel(const Args a
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = fmaf(acc_s[rr * per_row + w][grp * 8 + e], f, x[e]);
     }
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= inv;
+    for (int e = 0; e < 8; ++e) x[e] = normalised(x[e], ll);
     const int r = split.tile * R + rr;
     const int token = r / a.group;
     const int h = split.head * a.group + r - token * a.group;

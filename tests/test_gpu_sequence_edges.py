@@ -2,6 +2,8 @@
 in 64 bits with the bound of seq_util.attention64, or with what the call gives without the odd rows."""
 from __future__ import annotations
 
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -176,3 +178,51 @@ def test_small_weights_beside_a_large_one_fp16(fpk, nq, n, d, first, cached):
     ref, bound = reference(q, kk, vv, [nq], [n], False, d, F16, v_step=step * 2.0 ** -7)
     bound = bound - 2.0 ** -24 + 2.0 ** -25
     assert err == 0 and within(out.get(), ref, bound) <= 1
+
+
+# (query rows, key rows) of a sequence whose first queries see nothing, and what it takes: the streaming
+# kernel's clusters (one CTA, several) and shares with a join, the tile kernel whole and cut.
+BLIND = [([7], [3]), ([16, 2], [10, 1]), ([900], [860]), ([30] * 140, [21] * 140), ([600] * 40, [560] * 40), ([250], [9000]), ([300] + [1] * 199, [292] + [1] * 199)]
+
+
+def with_bad_rows(x, rows, kind):
+    """NaN, infinities or both in `rows` of x [n, heads, d]: one channel, or all of them."""
+    x = x.clone()
+    d = x.shape[2]
+    if kind == "nan":
+        x[rows, :, 5] = math.nan
+    elif kind == "inf":
+        x[rows, 0, d - 1], x[rows, -1, 8] = math.inf, -math.inf
+    else:
+        x[rows] = math.nan
+    return x
+
+
+@pytest.mark.parametrize("case", range(len(BLIND)))
+@pytest.mark.parametrize("kind", ["nan", "inf", "all"])
+@pytest.mark.parametrize("paged", [False, True])
+def test_rows_that_see_nothing_are_zero_beside_bad_values(fpk, case, kind, paged):
+    nq, nk = BLIND[case]
+    hq, hk, d = 4, 2, 64
+    g = gen(case)
+    q = HeadRows(sum(nq), hq, d, F16).set(torch.randn(sum(nq), hq, d, device=DEV, generator=g))
+    k = torch.randn(sum(nk), hk, d, device=DEV, generator=g)
+    last = torch.tensor(nk, device=DEV).cumsum(0) - 1
+    v = with_bad_rows(torch.randn(sum(nk), hk, d, device=DEV, generator=g), last, kind)
+    if paged:
+        width = -(-max(nk) // 16)
+        cache = Cache(width * len(nk), 16, hk, d, F16)
+        table = torch.randperm(width * len(nk), device=DEV, generator=g).to(torch.int32).reshape(len(nk), width)
+        seq = torch.repeat_interleave(torch.arange(len(nk), device=DEV), torch.tensor(nk, device=DEV))
+        i = torch.arange(sum(nk), device=DEV) - starts(nk)[seq].long()
+        slots = table.long()[seq, i // 16] * 16 + i % 16
+        cache.put(0, slots, k.half())
+        cache.put(1, slots, v.half())
+        out, err = run_paged(fpk, q, cache, nq, torch.tensor(nk, dtype=torch.int32, device=DEV), table, True, F16)
+    else:
+        out, err = run_packed(fpk, q, HeadRows(sum(nk), hk, d, F16).set(k), HeadRows(sum(nk), hk, d, F16).set(v), nq, nk, True, F16)
+    got, at = out.get(), 0
+    for x, y in zip(nq, nk):
+        assert torch.count_nonzero(got[at:at + max(x - y, 0)]) == 0
+        at += x
+    assert err == 0
