@@ -31,6 +31,9 @@
 //   keys form one line that the CTAs share out, each finding its part from the
 //   lengths on the device. A tile that crosses CTAs leaves fp32 partials that a
 //   second launch joins in order (deterministic, no atomics).
+// * Under a causal mask 0 * v of a key that a row does not see is NaN where v is an
+//   infinity or NaN. A tile with NaN in its output and with such keys is done again,
+//   token by token.
 // * Short sequences instead take a cluster of CTAs for each tile, which share its
 //   keys out evenly and join over distributed shared memory: no second launch.
 //
@@ -68,6 +71,14 @@ constexpr float kGrowLog2 = 15.0f;
 // e4m3: a row of zeros moves the reference only when its score is this far above.
 constexpr float kZerosLog2 = 48.0f;
 constexpr int kClusterKeys = 512;  // a cluster's most keys to a CTA
+
+// A pass over a tile: its rows lo .. hi - 1 (all, or those of one token, see `nan`).
+struct Pass {
+  int again;  // first row of the pass in a tile that is done again, else -1
+  int lo, hi;
+  int hides;  // a row of the pass does not see some keys of it
+  int nan;    // and the output holds NaN
+};
 
 // The tile that a CTA's range begins inside, for the joining launch.
 struct Split {
@@ -196,18 +207,22 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
   constexpr int kCols = R / 8;  // blocks of 8 query rows
   using S = Step<D, kE4m3>;
   using M = std::conditional_t<kE4m3, __half, T>;  // type of the products
-  extern __shared__ __align__(16) unsigned char ring_raw[];
+  // On a line of shared memory: 96 bytes past one, one token over 8 x 131,072 e4m3
+  // keys takes 169 us, on one 154.
+  extern __shared__ __align__(128) unsigned char ring_raw[];
   auto o_s = reinterpret_cast<float(*)[kStreamRows][D + 4]>(ring_raw);  // [kWarps], once the ring is empty
   __shared__ float ml_s[kWarps][2][kStreamRows];
   __shared__ long long scan_s[kWarps + 1];
   __shared__ long long found_s[2];
   __shared__ int owner_s;                     // clusters: the sequence, the last that has this tile
   __shared__ float joined_s[2][kStreamRows];  // clusters: this CTA's m and l
+  __shared__ Pass pass_s;
 
   tc::pdlTrigger();
   tc::pdlWait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
+  if (tid == 0) pass_s.again = -1;
 
   Split* splits = reinterpret_cast<Split*>(a.workspace);
   float* partials = reinterpret_cast<float*>(a.workspace + sizeof(Split) * kStreamCtas);
@@ -316,6 +331,9 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
       b1 = static_cast<int>(min(static_cast<long long>(blocks), end - tile_first));
     }
     const int rows = min(R, q.nq * a.group - tile * R);
+    // Rows of this pass: the tile's, or those of a token.
+    const int lo = max(pass_s.again, 0);
+    const int hi = pass_s.again < 0 ? rows : min(rows, ((tile * R + lo) / q_heads_per + 1) * q_heads_per - tile * R);
 
     // This thread's score columns are rows 8 n + 2t and 8 n + 2t + 1 of the tile.
     int vis[kCols][2];
@@ -325,13 +343,19 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int rr = 8 * n + 2 * t + i;  // tile * R + rr is below 2^31: checked by the host
-        vis[n][i] = rr < rows ? visible(a, q, (tile * R + rr) / q_heads_per) : q.nk;
+        vis[n][i] = rr >= lo && rr < hi ? visible(a, q, (tile * R + rr) / q_heads_per) : q.nk;
         min_vis = min(min_vis, vis[n][i]);
       }
     }
-    const int last_vis = visible(a, q, (tile * R + rows - 1) / q_heads_per);
+    const int last_vis = visible(a, q, (tile * R + hi - 1) / q_heads_per);
     min_vis = min(min_vis, __shfl_xor_sync(0xffffffffu, min_vis, 1));
     min_vis = min(min_vis, __shfl_xor_sync(0xffffffffu, min_vis, 2));
+    if (tid == 0) {
+      pass_s.lo = lo;
+      pass_s.hi = hi;
+      pass_s.hides = min_vis < last_vis;
+      pass_s.nan = 0;
+    }
 
     // Steps of 16 keys, one warp after the other, up to the last visible key.
     const int step_end = min(b1 * (kUnitKeys / 16), (last_vis + 15) >> 4);
@@ -673,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
     }
     for (int i = tid; i < R * (D / 8); i += kThreads) {
       const int rr = i / (D / 8), grp = i % (D / 8);
-      if (rr >= rows) continue;
+      if (rr < pass_s.lo || rr >= pass_s.hi) continue;
       float mm = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml_s[w][0][rr]);
@@ -685,6 +709,12 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         ll = fmaf(ml_s[w][1][rr], f, ll);
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = fmaf(o_s[w][rr][grp * 8 + e], f, acc[e]);
+      }
+      if (pass_s.hides) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (acc[e] != acc[e]) pass_s.nan = 1;
+        }
       }
       if (whole) {
 #pragma unroll
@@ -703,6 +733,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         }
       }
     }
+    bool nan = false;
     if constexpr (kCluster) {
       if (cluster > 1) {
         __syncwarp();  // the barrier is one of whole warps, and lanes leave the loop apart
@@ -710,6 +741,7 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
         const uint32_t part_at = tc::smemU32(part), ml_at = tc::smemU32(&joined_s[0][0]);
         for (int i = rank * kThreads + tid; i < rows * (D / 8); i += cluster * kThreads) {
           const int rr = i / (D / 8), grp = i % (D / 8);
+          if (rr < pass_s.lo || rr >= pass_s.hi) continue;
           float m_all = -INFINITY, l_all = 0.0f, x[8] = {};
           for (int c = 0; c < cluster; ++c) m_all = fmaxf(m_all, loadCluster4(tc::mapaShared(ml_at + rr * 4, c)));
           for (int c = 0; c < cluster; ++c) {
@@ -728,11 +760,28 @@ __global__ void __launch_bounds__(kThreads, 3) attentionStreamKernel(const Args 
           const int token = r / q_heads_per;
           *reinterpret_cast<uint4*>(record(a.out, head * q_heads_per + r - token * q_heads_per, q.q0 + token, grp)) = pack8<T>(x);
         }
+        if (pass_s.hides) {
+          for (int c = 0; c < cluster; ++c) nan |= __float_as_int(loadCluster4(tc::mapaShared(tc::smemU32(&pass_s.nan), c))) != 0;
+        }
         __syncwarp();
         tc::clusterSync();  // no CTA leaves while another reads its memory
       }
-      return;
     }
+    if (pass_s.hides && (!kCluster || cluster == 1)) {
+      __syncthreads();
+      nan = pass_s.nan != 0;
+    }
+    // Where a row does not see a key, an infinity or NaN among its values makes
+    // 0 * v NaN: the tile is done again token by token, whose rows see the same keys
+    // and the others are not read.
+    if (pass_s.again >= 0 || nan) {
+      const int next = pass_s.again < 0 ? 0 : pass_s.hi < min(R, q.nq * a.group - tile * R) ? pass_s.hi : -1;
+      __syncthreads();
+      if (tid == 0) pass_s.again = next;
+      __syncthreads();
+      if (next >= 0) continue;
+    }
+    if constexpr (kCluster) return;
     if (first_piece && tid == 0) {
       if (b0 > 0) {
         split->first_unit = tile_first;

@@ -32,6 +32,10 @@
 //   warp 13         the walk: the next pieces of work for the others.
 //   warp 14         the proxy fence between a load's arrival and the MMAs that
 //                   read it, which would cost the issuing warp 300-600 cycles.
+// Under a causal mask 0 * v of a key that a row does not see is NaN where v is an
+// infinity or NaN. An item with NaN in such a row is walked a second time, when
+// warp 14 takes these values out and the softmax warps add them to the rows that
+// see them (looked for in every item they cost prompts 1 to 8 %).
 // TMEM: S_0 S_1 (128 columns each) O_0 O_1 (d each), one CTA per SM.
 //
 // The work of all tiles is laid on one line (a tile's length: the keys that it
@@ -97,7 +101,7 @@ constexpr int kBulkRows = 32;
 constexpr int kSnap = 8;
 
 struct Item {
-  int halves;                  // halves with rows; 0: no more work
+  int halves;                  // halves with rows; 0: no more work, -1: none in this item
   int seq, head, tile;
   int q0, nq, k0, nk;
   int jb, je;                  // key blocks of this piece
@@ -120,6 +124,9 @@ struct Smem {
   uint64_t s_full[2], p_half[2], p_full[2], pv_half[2], pv_done[2], o_free[2];  // half: of a block's first 64 keys
   uint64_t drained[2];
   Item items[kItems];
+  int again[kItems];   // the item is done a second time: hidden values are taken out
+  int redo[kItems];    // it has to be
+  int hidden[kItems];  // its hidden values are in the table
   long long scan[kThreads / 32 + 1];
   long long found[2];
   uint32_t tmem;
@@ -312,6 +319,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
   return r;
 }
+__device__ __forceinline__ float max3Nan(float x, float y, float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
@@ -354,8 +366,103 @@ __device__ __forceinline__ void copyArrive(uint64_t* bar) {
 }
 __device__ __forceinline__ void copyDrain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+__device__ __forceinline__ uint4 loadShared16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
 __device__ __forceinline__ void storeShared16(uint32_t dst, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// ---- hidden values that are not finite, in items that are done again ----
+//
+// Such an element becomes 0, and the lowest key that held one is noted by channel.
+// As a row sees the keys below its limit, it sees one exactly if its limit is above
+// that key, and gets it at the end.
+
+// Whether a record of T holds an infinity or NaN: 1 carries the exponent's ones into bit 15.
+template <typename T>
+__device__ __forceinline__ bool hasNotFinite(const uint4& w) {
+  const uint32_t m = 0x7fff7fffu, one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+  return ((((w.x & m) + one) | ((w.y & m) + one) | ((w.z & m) + one) | ((w.w & m) + one)) & 0x80008000u) != 0;
+}
+
+constexpr int kNoKey = 0x7fffffff;
+
+// Record of `key` with such elements as zeros. first[c] is the lowest key with
+// +infinity or NaN in channel c of the record, first[negative + c] with -infinity or NaN.
+template <typename T>
+__device__ __noinline__ uint4 hideNotFinite(uint4 w, int key, int* first, int negative) {
+  const uint32_t exponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t h = (u[e / 2] >> (16 * (e & 1))) & 0xffffu;
+    if ((h & exponent) != exponent) continue;
+    const bool nan = (h & 0x7fffu) != exponent, minus = (h & 0x8000u) != 0;
+    if (nan || !minus) atomicMin(first + e, key);
+    if (nan || minus) atomicMin(first + negative + e, key);
+    u[e / 2] &= ~(0xffffu << (16 * (e & 1)));
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// What a row that sees the keys below `visible` adds to a channel's sum.
+__device__ __forceinline__ float seenNotFinite(int first_plus, int first_minus, int visible) {
+  if (first_plus < visible) return first_minus < visible ? __int_as_float(0x7fffffff) : __int_as_float(0x7f800000);
+  return first_minus < visible ? __int_as_float(static_cast<int>(0xff800000u)) : 0.0f;
+}
+
+// Record of row r and plane p of a tile. 32 rows of a plane give neither layout a bank conflict.
+__device__ __forceinline__ uint32_t recordAt(uint32_t tile, bool planar, int r, int p) {
+  return tile + (planar ? p * kPlane + r * 16 : (p >> 3) * kChunk + r * 128 + (((p ^ r) & 7) << 4));
+}
+
+// Whether keys edge .. lim - 1 of a V tile have any. This and the next two by a whole warp.
+template <typename T, int D>
+__device__ __noinline__ bool hasHidden(uint32_t tile, bool planar, int key0, int edge, int lim) {
+  const int lane = threadIdx.x & 31, rows = min(lim - key0, kKeys);
+  bool found = false;
+#pragma unroll 1
+  for (int r = max(edge - key0, 0) + lane; r < rows; r += 32) {
+    for (int p = 0; p < D / 8; ++p) found |= hasNotFinite<T>(loadShared16(recordAt(tile, planar, r, p)));
+  }
+  return __any_sync(0xffffffffu, found);
+}
+
+// Takes them out and notes them in a table of 2 x D, which `begun` says holds some already.
+template <typename T, int D>
+__device__ __noinline__ void hideValues(uint32_t tile, bool planar, int key0, int edge, int lim, int* table, bool begun) {
+  const int lane = threadIdx.x & 31, rows = min(lim - key0, kKeys);
+  if (!begun) {
+    for (int c = lane; c < 2 * D; c += 32) table[c] = kNoKey;
+    __syncwarp();
+  }
+#pragma unroll 1
+  for (int r = max(edge - key0, 0) + lane; r < rows; r += 32) {
+#pragma unroll 1
+    for (int p = 0; p < D / 8; ++p) {
+      const uint4 v = loadShared16(recordAt(tile, planar, r, p));
+      if (hasNotFinite<T>(v)) storeShared16(recordAt(tile, planar, r, p), hideNotFinite<T>(v, key0 + r, table + 8 * p, D));
+    }
+  }
+  __syncwarp();
+}
+
+// Adds to a row's O what those that it sees make of it.
+template <int D>
+__device__ __noinline__ void addHidden(uint32_t o, const volatile int* table, int visible) {
+#pragma unroll 1
+  for (int c = 0; c < D; c += 16) {
+    uint32_t x[16];
+    FPB_TMEM_LD16(o + c, x);
+    tmemWaitLd();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) + seenNotFinite(table[c + e], table[D + c + e], visible));
+    FPB_TMEM_ST16(o + c, x);
+  }
+  tmemStoreWait();
 }
 
 // An e4m3 record with NaN or an unusual scale, into two groups of a planar tile.
@@ -379,7 +486,6 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   Smem& sm = *reinterpret_cast<Smem*>(base);
   const uint32_t q_s = smemU32(base + 1024);
   const uint32_t kv_s = q_s + 2 * G::kTileBytes;
-
   tc::pdlTrigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -416,6 +522,8 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   // ---- this CTA's share of the line ----
   Cut* cuts = reinterpret_cast<Cut*>(a.workspace);
   float* partials = reinterpret_cast<float*>(a.workspace + sizeof(Cut) * kTileCtas);
+  // Hidden values of items done again. Not in shared memory, where 1 KB more costs L1.
+  int* table = reinterpret_cast<int*>(partials + 2 * kTileCtas * partialFloats(D)) + blockIdx.x * 2 * D;
   auto lengthOf = [&](int s) -> long long {
     if (s >= a.n_seq) return 0;
     const Line n = lineOf(a, sequence<kKind>(a, s));
@@ -568,6 +676,10 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
             }
           }
           ahead = scores;
+        } else if (sc.halves < 0) {
+          release(sc);
+          ++sc.item;
+          fetch = true;
         } else if (sc.halves > 0) {  // no rows here: the keys are the other half's
           for (; sc.j < sc.je && ok; ++sc.j, ++sc.block) {
             for (int side = 0; side < 2 && ok; ++side) {
@@ -659,42 +771,98 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
           it.part = it.jb == 0 && it.je == blocks ? -1 : 2 * static_cast<int>(blockIdx.x) + (it.jb > 0 ? 0 : 1);
         }
       };
-      bool ok = true;
-      for (int i = 0; ok; ++i) {
-        const int slot = i % kItems;
-        if (i >= kItems) ok = wait(&sm.item_empty[slot], ((i / kItems) - 1) & 1, sm, err, 51);
-        if (!ok) break;
+      // Items published and looked at once they are done: a causal item that asks
+      // for it is done a second time. So the walk waits for the last ones; an empty
+      // item lets the MMA warps finish them, who look one item ahead.
+      int i = 0, looked = 0, empty = -1;
+      bool more = true;
+      for (;;) {
         Item it{};
-        nextItem(it);
+        bool again = false;
+        if (i - looked == kItems || looked < empty) {
+          const int slot = looked % kItems;
+          if (!wait(&sm.item_empty[slot], (looked / kItems) & 1, sm, err, 51)) break;
+          ++looked;
+          if (*const_cast<volatile int*>(&sm.redo[slot]) == 0) continue;
+          it = sm.items[slot];
+          again = true;
+        } else if (more) {
+          nextItem(it);
+          more = it.halves > 0;
+          if (!more && a.causal && i > 0) {
+            it.halves = -1;
+            empty = i;
+          }
+        }
+        const int slot = i % kItems;
+        __syncwarp();
         if (lane == 0) {
           sm.items[slot] = it;
+          sm.again[slot] = again;
+          sm.redo[slot] = 0;
+          sm.hidden[slot] = 0;
           mbarArrive(&sm.item_full[slot]);
         }
         __syncwarp();
         if (it.halves == 0) break;
+        ++i;
       }
     } else if (warp == 14) {
       // ---------------- fences ----------------
       // What has landed becomes visible to the tensor core, in the order of the loads.
       bool ok = true;
       int n = 0, used0 = 0, used1 = 0;  // key blocks, loads of Q's halves
+      int table_item = -1;              // the last item that noted hidden values
       for (int i = 0; ok; ++i) {
         const int slot = i % kItems;
         ok = wait(&sm.item_full[slot], (i / kItems) & 1, sm, err, 52);
         if (!ok) break;
         const int halves = sm.items[slot].halves, blocks = sm.items[slot].je - sm.items[slot].jb;
+        const bool again = halves > 0 && sm.again[slot] != 0;
+        // In an item that is done again: values of the keys from `edge` on, which some
+        // row of the tile does not see, are looked through.
+        bool hidden = false;
+        int edge = 0, lim = 0, key0 = 0;
+        if (again) {
+          const Item& it = sm.items[slot];
+          edge = visible(a, Sequence{it.q0, it.nq, it.k0, it.nk}, it.tile * kTileRows / a.group);
+          lim = it.lim;
+          key0 = it.jb * kKeys;
+        }
         __syncwarp();
         if (lane == 0) mbarArrive(&sm.item_empty[slot]);
         if (halves == 0) break;
+        if (halves < 0) continue;
         // K, Q's halves, V, then K and V of each block.
-        for (int x = 0; x < 2 * blocks + halves && ok; ++x) {
+        auto pass = [&](int x, auto&& look) {
           const bool is_q = x >= 1 && x <= halves;
           const int t = x - 1, y = is_q ? 0 : x > halves ? x - halves : x;  // y: 2 * block + side
           const int m = n + (y >> 1), stage = (m & 1) * 2 + (y & 1);
           ok = wait(is_q ? &sm.q_full[t] : &sm.kv_full[stage], (is_q ? (t == 0 ? used0 : used1) : m >> 1) & 1, sm, err, 60);
+          if (ok && !is_q && (y & 1) == 1) look(y >> 1, kv_s + stage * G::kTileBytes);
           fenceProxyAsyncSmem();
           __syncwarp();
           if (ok && lane == 0) mbarArrive(is_q ? &sm.q_ready[t] : &sm.kv_ready[stage]);
+        };
+        if (!again) {
+          for (int x = 0; x < 2 * blocks + halves && ok; ++x) pass(x, [](int, uint32_t) {});
+        } else {
+#pragma unroll 1
+          for (int x = 0; x < 2 * blocks + halves && ok; ++x) {
+            pass(x, [&](int block, uint32_t tile) {
+              const int key = key0 + block * kKeys;
+              if (!hasHidden<T, D>(tile, v_planar, key, edge, lim)) return;
+              // The table is free once the softmax has let go of the item that used
+              // it last, an earlier one, which waits for nothing of this one.
+              if (!hidden && table_item >= 0 && i - table_item < kItems) {
+                ok = wait(&sm.item_empty[table_item % kItems], (table_item / kItems) & 1, sm, err, 60);
+              }
+              if (ok) hideValues<T, D>(tile, v_planar, key, edge, lim, table, hidden);
+              if (lane == 0) sm.hidden[slot] = 1;
+              hidden = true;
+              table_item = i;
+            });
+          }
         }
         n += blocks;
         ++used0;
@@ -725,6 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       __syncwarp();
       if (lane == 0) mbarArrive(&sm.item_empty[slot]);
       if (it.halves == 0) break;
+      if (it.halves < 0) continue;
 
       // Pages of a block: lane x holds that of its rows 16 x .. 16 x + 15.
       auto pagesOf = [&](int j) -> int {
@@ -911,9 +1080,11 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
       if (!ok) break;
       const Item it = sm.items[slot];
       __syncwarp();
-      if (lane == 0) mbarArrive(&sm.item_empty[slot]);
       if (it.halves == 0) break;
-      if (t >= it.halves) continue;
+      if (t >= it.halves) {
+        if (lane == 0) mbarArrive(&sm.item_empty[slot]);
+        continue;
+      }
       const Sequence q{it.q0, it.nq, it.k0, it.nk};
       const int row_first = it.tile * kTileRows + t * kHalf;
       const int r = row_first + rr;
@@ -996,19 +1167,26 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         }
         if (!ok) break;
       }
+      const Item end = sm.items[i % kItems];  // read again: registers are short in the loop above
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int h = end.head * a.group + (valid ? r - token * a.group : 0);
+      float* part_at = end.part >= 0 ? partials + static_cast<size_t>(end.part) * partialFloats(D) : nullptr;
+      const int tile_row = t * kHalf + rr;
       if (ok) ok = wait(&sm.pv_done[t], (count - 1) & 1, sm, err, 59);
       if (!ok) break;
       tcFenceAfter();
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int h = it.head * a.group + (valid ? r - token * a.group : 0);
-      float* part_at = it.part >= 0 ? partials + static_cast<size_t>(it.part) * partialFloats(D) : nullptr;
-      const int tile_row = t * kHalf + rr;
+      if (a.causal && *const_cast<volatile int*>(&sm.hidden[i % kItems]) != 0) addHidden<D>(o_base, table, vis);
+      float top = 0.0f;  // NaN if one of O is
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t ov[32];
         __syncwarp();  // the load is one of a whole warp, and lanes without a row skip the stores
         FPB_TMEM_LD32(o_base + c, ov);
         tmemWaitLd();
+        if (a.causal) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) top = max3Nan(top, __uint_as_float(ov[e]), __uint_as_float(ov[e + 1]));
+        }
         if (valid && part_at == nullptr) {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
@@ -1020,7 +1198,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
 #pragma unroll
               for (int e = 0; e < 8; ++e) x[e] = 0.0f;
             }
-            *reinterpret_cast<uint4*>(record(a.out, h, it.q0 + token, (c >> 3) + g)) = pack8<T>(x);
+            *reinterpret_cast<uint4*>(record(a.out, h, end.q0 + token, (c >> 3) + g)) = pack8<T>(x);
           }
         } else if (valid) {
 #pragma unroll
@@ -1034,9 +1212,15 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         part_at[kTileRows * D + tile_row] = m;
         part_at[kTileRows * D + kTileRows + tile_row] = l;
       }
+      // NaN may come from values that this row does not see (0 * v): the item is
+      // done again without them.
+      if (valid && top != top && vis < end.lim && sm.again[i % kItems] == 0) sm.redo[i % kItems] = 1;
       tcFenceBefore();
       __syncwarp();
-      if (lane == 0) mbarArrive(&sm.o_free[t]);
+      if (lane == 0) {
+        mbarArrive(&sm.o_free[t]);
+        mbarArrive(&sm.item_empty[i % kItems]);  // only now: the table is read, and whether to do it again known
+      }
     }
   }
   tcFenceBefore();
@@ -1135,7 +1319,7 @@ __global__ void __launch_bounds__(kTileRows) joinTilesKernel(const Args a, int n
 }
 
 long long tilesWorkspaceBytes(int head_dim) {
-  return static_cast<long long>(sizeof(Cut) * kTileCtas + 2 * kTileCtas * partialFloats(head_dim) * sizeof(float));
+  return static_cast<long long>(sizeof(Cut) * kTileCtas + 2 * kTileCtas * partialFloats(head_dim) * sizeof(float) + kTileCtas * 2 * head_dim * sizeof(int));
 }
 
 namespace {

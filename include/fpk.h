@@ -384,8 +384,8 @@ FP_API int fpk_cache_read(const fpk_cache_copy_desc_t* desc, void* stream);
  * hold. At most 2^31 - 1024 keys. scale 0 means 1/sqrt(head_dim). head_dim is 64 or 128, q_heads a
  * multiple of kv_heads, at most 128 query heads to a key head. Products run on
  * the tensor cores with probabilities rounded to the element type; scores,
- * softmax statistics and sums are fp32. An infinity or NaN in V reaches, besides the
- * queries that see its key, those of its tile whose causal mask hides it.
+ * softmax statistics and sums are fp32. What a key that a query does not see holds,
+ * an infinity or NaN too, does not reach the query's output.
  * How far sequences are split over the GPU follows the sizes in the descriptor,
  * so the last bits may; for one descriptor and lengths they do not change.
  * workspace (fpk_attention_packed_workspace_bytes, the same for every batch of

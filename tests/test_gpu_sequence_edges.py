@@ -226,3 +226,98 @@ def test_rows_that_see_nothing_are_zero_beside_bad_values(fpk, case, kind, paged
         assert torch.count_nonzero(got[at:at + max(x - y, 0)]) == 0
         at += x
     assert err == 0
+
+
+# (query rows, key rows, query heads, key heads, kernel): bad values among the keys that the last queries
+# alone see, for every way through the kernels.
+HIDDEN = {
+    "cluster": ([6], [300], 8, 2), "one-cta": ([5, 1, 9], [70, 3, 9], 4, 4), "cluster-16": ([16], [500], 4, 2),
+    "shares": ([7], [9000], 4, 2), "shares-many": ([13] * 150, [40] * 150, 2, 1), "shares-edge": ([300] + [1] * 199, [420] + [1] * 199, 4, 2),
+    "tiles": ([300, 70, 513] * 8, None, 4, 4), "tiles-grouped": ([90, 200, 333] * 8, [700, 200, 400] * 8, 16, 2), "tiles-cut": ([250], [9000], 4, 2),
+    "tiles-long": ([3000], None, 2, 1),
+}
+
+
+def seen_bad(v, first, hq, d):
+    """What queries add to their sums from bad values of v [n, hk, d]: query i sees keys below first[i]."""
+    n, hk, _ = v.shape
+    big = n + 1
+    key = torch.arange(n, device=v.device)[:, None, None]
+    plus = torch.where((v == math.inf) | v.isnan(), key, big).amin(0)
+    minus = torch.where((v == -math.inf) | v.isnan(), key, big).amin(0)
+    see = lambda t: (t[None] < first[:, None, None]).repeat_interleave(hq // hk, 1)  # noqa: E731
+    add = torch.zeros(len(first), hq, d, device=v.device)
+    add[see(plus)] = math.inf
+    add[see(minus)] += -math.inf
+    return add
+
+
+@pytest.mark.parametrize("name", HIDDEN)
+@pytest.mark.parametrize("kind", ["nan", "inf", "all"])
+@pytest.mark.parametrize("dtype,cached,layout,d,page", [(F16, "packed", "rows", 64, 0), (BF16, "packed", "planar", 128, 0), (BF16, "same", "rows", 128, 16),
+                                                       (F16, "same", "rows", 64, 64), (BF16, "e4m3", "planar", 128, 32), (F16, "e4m3", "rows", 64, 16)])
+def test_bad_values_reach_only_the_queries_that_see_them(fpk, name, kind, dtype, cached, layout, d, page):
+    """Against 64 bits with zeros in their place, and what an infinity or NaN makes of the channels of the
+    queries that see it."""
+    nq, nk, hq, hk = HIDDEN[name]
+    nk = list(nq) if nk is None else nk
+    g = gen(len(name) + d)
+    q = HeadRows(sum(nq), hq, d, dtype, layout).set(torch.randn(sum(nq), hq, d, device=DEV, generator=g))
+    k = torch.randn(sum(nk), hk, d, device=DEV, generator=g)
+    clean = torch.randn(sum(nk), hk, d, device=DEV, generator=g)
+    bad, rows, first, at = clean, [], [], 0
+    for x, y in zip(nq, nk):
+        # Keys that the last query, some of the last ones and half of them see first, and one that all do.
+        rows += [at + y - 1, at + y - 1 - (min(x, y) - 1) // 3, at + y - 1 - (min(x, y) - 1) // 2] + ([at] if len(rows) % 2 else [])
+        first.append(at + y - x + 1 + torch.arange(x, device=DEV))
+        at += y
+    rows = torch.tensor(sorted(set(rows)), device=DEV)
+    bad = with_bad_rows(clean, rows[::2], kind)
+    bad = with_bad_rows(bad, rows[1::2], "nan" if kind == "nan" else "inf")
+    if cached == "e4m3":
+        bad = torch.where(bad.isfinite(), bad, math.nan)  # as the cache holds them
+    zeroed = torch.where(bad.isfinite(), bad, 0.0)
+    if cached == "packed":
+        kr, vr = HeadRows(sum(nk), hk, d, dtype, layout).set(k), HeadRows(sum(nk), hk, d, dtype, layout).set(bad)
+        out, err = run_packed(fpk, q, kr, vr, nq, nk, True, dtype, layout)
+        kk, vv, step = kr.get().double(), zeroed.to(DT[dtype]).double(), None
+    else:
+        width = -(-max(nk) // page)
+        cache = Cache(width * len(nk), page, hk, d, dtype, cached == "e4m3")
+        table = torch.arange(width * len(nk) - 1, -1, -1, dtype=torch.int32, device=DEV).reshape(len(nk), width).contiguous()
+        seq = torch.repeat_interleave(torch.arange(len(nk), device=DEV), torch.tensor(nk, device=DEV))
+        i = torch.arange(sum(nk), device=DEV) - starts(nk)[seq].long()
+        slots = table.long()[seq, i // page] * page + i % page
+        cache.put(0, slots, k.to(DT[dtype]))
+        cache.put(1, slots, bad.to(DT[dtype]))
+        kk, vv = cache.values(0, slots), cache.values(1, slots).nan_to_num(0, 0, 0)
+        out, err = run_paged(fpk, q, cache, nq, torch.tensor(nk, dtype=torch.int32, device=DEV), table, True, dtype, layout)
+        step = 448.0 * float(cache.scale[1].nan_to_num(0).max()) if cached == "e4m3" else None
+    ref, bound = reference(q, kk, vv, nq, nk, True, d, dtype, v_step=step)
+    add, at_q, at_k = torch.empty(sum(nq), hq, d, device=DEV), 0, 0
+    for x, y, f in zip(nq, nk, first):
+        add[at_q:at_q + x] = seen_bad(bad[at_k:at_k + y], f - at_k, hq, d)
+        at_q, at_k = at_q + x, at_k + y
+    got, fine = out.get(), add == 0
+    assert err == 0 and fine.any() and not fine.all()
+    assert within(got[fine], ref[fine], bound[fine]) <= 1
+    assert torch.equal(got[~fine].float().nan_to_num(1.0, 2.0, 3.0), add[~fine].nan_to_num(1.0, 2.0, 3.0))
+
+
+@pytest.mark.parametrize("name", HIDDEN)
+@pytest.mark.parametrize("which", ["k", "v", "all"])
+def test_nothing_but_nan_comes_to_an_end(fpk, name, which):
+    nq, nk, hq, hk = HIDDEN[name]
+    nk = list(nq) if nk is None else nk
+    g = gen(1)
+    q, k, v = (HeadRows(n, h, 64, BF16).set(torch.randn(n, h, 64, device=DEV, generator=g)) for n, h in ((sum(nq), hq), (sum(nk), hk), (sum(nk), hk)))
+    for x, n in ((q, "q"), (k, "k"), (v, "v")):
+        if which in (n, "all"):
+            x.v.fill_(math.nan)
+    out, err = run_packed(fpk, q, k, v, nq, nk, True, BF16)
+    assert err == 0 and out.untouched_around()
+    at = 0
+    for x, y in zip(nq, nk):
+        blind = max(x - y, 0)
+        assert torch.count_nonzero(out.get()[at:at + blind]) == 0 and out.get()[at + blind:at + x].isnan().all()
+        at += x
