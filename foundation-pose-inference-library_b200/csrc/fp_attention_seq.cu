@@ -1,6 +1,7 @@
 // Host side of fpk_attention_packed and fpk_attention_paged (include/fpk.h):
 // checks and the choice of the kernel.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -14,6 +15,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr long long kMostKeys = (1LL << 31) - 1024;  // key counts round up to blocks in 32 bits
 constexpr const char* kMisaligned = "starts, lengths, page_table and error_flag must be 4-byte aligned";
+
+std::atomic<int> g_test_fail{-1};  // fpk_attention_test_fail_share
 
 struct Shape {
   int q_heads, kv_heads, head_dim, n_seq, q_rows;
@@ -139,6 +142,7 @@ extern "C" int fpk_attention_packed(const fpk_attention_packed_desc_t* d, void* 
   a.scale_log2 = scaleLog2(d->scale, d->head_dim);
   a.error_flag = d->error_flag;
   a.workspace = static_cast<unsigned char*>(d->workspace);
+  a.test_fail = g_test_fail.load();
   return launch(name, a, kPacked16, n, d->dtype, stream);
 }
 
@@ -195,5 +199,8 @@ extern "C" int fpk_attention_paged(const fpk_attention_paged_desc_t* d, void* st
   a.scale_log2 = scaleLog2(d->scale, c.head_dim);
   a.error_flag = d->error_flag;
   a.workspace = static_cast<unsigned char*>(d->workspace);
+  a.test_fail = g_test_fail.load();
   return launch(name, a, e4m3 ? kPagedE4m3 : kPaged16, n, d->dtype, stream);
 }
+
+extern "C" int fpk_attention_test_fail_share(int share) { return fpb::seqattn::g_test_fail.exchange(share < 0 ? -1 : share); }

@@ -35,6 +35,7 @@ struct Args {
   float scale_log2;           // scale * log2(e)
   int* error_flag;
   unsigned char* workspace;
+  int test_fail;              // tile kernel: this CTA counts as one whose wait ran out (tests), else -1
 };
 
 struct Sequence {

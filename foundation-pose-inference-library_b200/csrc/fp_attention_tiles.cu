@@ -113,7 +113,8 @@ struct Item {
 struct Cut {
   long long tile_at;           // the tile's place on the line, -1: nothing cut
   int jb, blocks;
-  int seq, head, tile, pad;
+  int seq, head, tile;
+  int failed;                  // a wait of this CTA ran out: its pieces may be missing
 };
 
 struct Smem {
@@ -722,6 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
         at += lengthBefore(line, tile);
       } else if (lane == 0) {
         cuts[blockIdx.x].tile_at = -1;
+        cuts[blockIdx.x].failed = 0;
       }
       const int snap = static_cast<int>(min(share / kSnap, 0x7fffffffLL));
       bool first = true;
@@ -1225,6 +1227,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   }
   tcFenceBefore();
   __syncthreads();
+  if (tid == 0 && (sm.stop != 0 || static_cast<int>(blockIdx.x) == a.test_fail)) cuts[blockIdx.x].failed = 1;
   if (warp == 12) {
     tcFenceAfter();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
@@ -1249,19 +1252,20 @@ __global__ void __launch_bounds__(kTileRows) joinTilesKernel(const Args a, int n
   const float* partials = reinterpret_cast<const float*>(a.workspace + sizeof(Cut) * kTileCtas);
   const int c = blockIdx.x;
   const Cut cut = cuts[c];
-  if (cut.tile_at < 0 || (c > 0 && cuts[c - 1].tile_at == cut.tile_at)) return;
+  if (c == 0 || cut.tile_at < 0 || cuts[c - 1].tile_at == cut.tile_at) return;
   const int row = threadIdx.x, grp = blockIdx.y * kJoinGroups;
   // Shares c + 1, ... that begin in the same tile: they follow one another.
   static_assert(kTileCtas <= kTileRows, "a thread to each share");
   const int d = c + 1 + row;
   const bool same = d < n_cta && cuts[d].tile_at == cut.tile_at;
   if (same) jb_s[row + 1] = cuts[d].jb;
+  const bool failed = (same && cuts[d].failed != 0) || (row == 0 && (cut.failed != 0 || cuts[c - 1].failed != 0));
   const int more = __syncthreads_count(same);
   if (row == 0) {
     jb_s[0] = cut.jb;
     jb_s[more + 1] = cut.blocks;
   }
-  __syncthreads();
+  if (__syncthreads_or(failed)) return;  // a piece is missing: the tile is not stored
   const Sequence q = sequence<kKind>(a, cut.seq);
   const int r = cut.tile * kTileRows + row;
   if (r >= q.nq * a.group) return;

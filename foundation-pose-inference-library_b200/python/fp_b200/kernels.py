@@ -87,6 +87,7 @@ _SIGS = {
     "fpk_attention_packed": (C.c_int, [_P, _P]),
     "fpk_attention_paged_workspace_bytes": (C.c_longlong, [_P]),
     "fpk_attention_paged": (C.c_int, [_P, _P]),
+    "fpk_attention_test_fail_share": (C.c_int, [C.c_int]),
     "fpk_net_create": (C.c_void_p, [C.c_char_p, C.c_char_p, C.c_int, C.c_int]),
     "fpk_net_destroy": (None, [_P]),
     "fpk_net_refine": (C.c_int, [_P, _P, _P, C.c_int, _P, _P, _P]),

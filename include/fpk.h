@@ -303,7 +303,8 @@ FP_API int fpk_attention(const void* qkv, long long qkv_plane_stride, int qkv_la
 #define FPK_ERROR_PAGE 42   /* a page number outside the cache: its keys were treated as masked */
 #define FPK_ERROR_STARTS 43 /* starts that decrease or pass the buffer: clamped */
 #define FPK_ERROR_LENGTH 44 /* a length outside [0, table_pages*page_rows]: clamped */
-/* 51..60: a bounded wait inside the tensor-core kernel ran out; the tile was not stored. */
+/* 51..60: a bounded wait inside the tensor-core kernel ran out; rows that were not
+ * finished, and tiles cut over several CTAs of which one failed, are not stored. */
 
 typedef struct fpk_heads {
   void* data;
@@ -435,6 +436,12 @@ typedef struct fpk_attention_paged_desc {
   void* workspace;
   long long workspace_bytes;
 } fpk_attention_paged_desc_t;
+
+/* Failure-injection test switch. With share >= 0 that CTA of every following
+ * tile launch of fpk_attention_packed / _paged reports itself as one whose wait
+ * ran out, although it finished: tiles that it has a piece of are not stored. -1
+ * ends it. Process-wide; returns the previous setting. For tests only. */
+FP_API int fpk_attention_test_fail_share(int share);
 
 FP_API long long fpk_attention_paged_workspace_bytes(const fpk_attention_paged_desc_t* desc);
 FP_API int fpk_attention_paged(const fpk_attention_paged_desc_t* desc, void* stream);

@@ -321,3 +321,37 @@ def test_nothing_but_nan_comes_to_an_end(fpk, name, which):
         blind = max(x - y, 0)
         assert torch.count_nonzero(out.get()[at:at + blind]) == 0 and out.get()[at + blind:at + x].isnan().all()
         at += x
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_a_cut_tile_of_a_failed_cta_is_not_stored(fpk, paged):
+    """A CTA that counts as one whose wait ran out (nothing waits here): the tiles that it has a piece of
+    keep what the output held, the others are as ever, and the next call is whole again."""
+    nq, n, hq, hk, d = 200, 9000, 6, 3, 64
+    g = gen(2)
+    q = HeadRows(nq, hq, d, F16).set(torch.randn(nq, hq, d, device=DEV, generator=g))
+    k, v = (torch.randn(n, hk, d, device=DEV, generator=g) for _ in range(2))
+    if paged:
+        cache, table, length, _ = one_cached(n, k, v, F16, 32, g, False)
+        run = lambda: run_paged(fpk, q, cache, [nq], length, table, True, F16)  # noqa: E731
+    else:
+        kr, vr = HeadRows(n, hk, d, F16).set(k), HeadRows(n, hk, d, F16).set(v)
+        run = lambda: run_packed(fpk, q, kr, vr, [nq], [n], True, F16)  # noqa: E731
+    whole = run()[0].get().clone()
+    missing = torch.zeros(nq, hq, dtype=torch.bool, device=DEV)
+    try:
+        for share in (0, 1, 5, 70, 147, 10 ** 6):
+            assert fpk.lib.fpk_attention_test_fail_share(share) == -1
+            out, err = run()
+            assert fpk.lib.fpk_attention_test_fail_share(-1) == share and err == 0
+            kept = (out.get() == 3.0).all(-1)  # what run_packed and run_paged fill in
+            assert torch.equal(torch.where(kept[..., None], whole, out.get()), whole)
+            # Tiles: 256 rows of (token, head of the group) of one key head; a share lies in one or two.
+            tiles = kept.reshape(nq, hk, hq // hk).permute(1, 0, 2).reshape(hk, -1)
+            count = sum(bool(tiles[h, a:a + 256].any()) for h in range(hk) for a in (0, 256))
+            assert all(tiles[h, a:a + 256].any() == tiles[h, a:a + 256].all() for h in range(hk) for a in (0, 256))
+            assert (1 <= count <= 2) if share < 148 else count == 0
+            missing |= kept
+    finally:
+        fpk.lib.fpk_attention_test_fail_share(-1)
+    assert missing.any() and not missing.all() and same_bits(run()[0].get(), whole)
