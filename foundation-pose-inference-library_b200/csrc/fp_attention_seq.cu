@@ -123,7 +123,11 @@ extern "C" int fpk_attention_packed(const fpk_attention_packed_desc_t* d, void* 
   if (d->q_starts == nullptr || d->kv_starts == nullptr) return fail(name + ": q_starts and kv_starts are required");
   if (!aligned4(d->q_starts) || !aligned4(d->kv_starts) || !aligned4(d->error_flag)) return fail(name + ": " + kMisaligned);
   p = workspaceProblem(d->workspace, d->workspace_bytes, workspaceBytes(n));
-  if (p.empty()) p = deviceProblem(d->q.data);
+  if (p.empty()) {
+    const bool keys = d->kv_rows > 0;
+    p = deviceProblem({d->q.data, d->out.data, keys ? d->k.data : nullptr, keys ? d->v.data : nullptr, d->q_starts, d->kv_starts,
+                       d->error_flag, d->workspace});
+  }
   if (!p.empty()) return fail(name + ": " + p);
   Args a{};
   a.q = d->q;
@@ -170,10 +174,13 @@ extern "C" int fpk_attention_paged(const fpk_attention_paged_desc_t* d, void* st
     return fail(name + ": " + kMisaligned);
   }
   p = workspaceProblem(d->workspace, d->workspace_bytes, workspaceBytes(n));
-  if (p.empty()) p = deviceProblem(d->q.data);
-  if (!p.empty()) return fail(name + ": " + p);
   const fpk_kv_cache_t& c = d->cache;
   const bool e4m3 = c.dtype == FPK_DTYPE_E4M3;
+  if (p.empty()) {
+    p = deviceProblem({d->q.data, d->out.data, c.k, c.v, e4m3 ? c.k_scale : nullptr, e4m3 ? c.v_scale : nullptr, d->q_starts, d->kv_lengths,
+                       d->table_pages > 0 ? d->page_table : nullptr, d->error_flag, d->workspace});
+  }
+  if (!p.empty()) return fail(name + ": " + p);
   Args a{};
   a.q = d->q;
   a.out = d->out;

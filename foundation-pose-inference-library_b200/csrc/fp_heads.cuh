@@ -9,12 +9,14 @@
 // lives.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 #include <type_traits>
 
@@ -186,17 +188,36 @@ inline std::string cacheProblem(const fpk_kv_cache_t& c, int dtype) {
   return std::string();
 }
 
-// The launch goes to the current device: memory of another one is refused here
-// instead of faulting there.
-inline std::string deviceProblem(const void* p) {
-  cudaPointerAttributes at{};
-  if (cudaPointerGetAttributes(&at, p) != cudaSuccess) return std::string("pointer: ") + cudaGetErrorString(cudaGetLastError());
+// The launch goes to the current device: memory of another one, or of the host, is
+// refused here instead of faulting there. Of all pointers of a call (NULL passes),
+// some 30 ns each: the first, its largest array, must be device memory; page-locked
+// host memory, which kernels reach, may hold the others.
+inline std::string deviceProblem(std::initializer_list<const void*> pointers) {
+  using Get = CUresult (*)(void*, CUpointer_attribute, CUdeviceptr);
+  static const Get get = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r{};
+    const bool ok = cudaGetDriverEntryPoint("cuPointerGetAttribute", &f, cudaEnableDefault, &r) == cudaSuccess && r == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<Get>(f) : nullptr;
+  }();
+  if (get == nullptr) return "cuPointerGetAttribute is not available";
   int dev = 0;
   const cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return std::string("current device: ") + cudaGetErrorString(e);
-  if (at.type == cudaMemoryTypeUnregistered || at.type == cudaMemoryTypeHost) return "data is not in device memory";
-  if (at.type == cudaMemoryTypeDevice && at.device != dev) {
-    return "data is on device " + std::to_string(at.device) + ", the current device is " + std::to_string(dev);
+  unsigned type = 0;
+  if (get(&type, CU_POINTER_ATTRIBUTE_MEMORY_TYPE, reinterpret_cast<CUdeviceptr>(*pointers.begin())) != CUDA_SUCCESS ||
+      type == CU_MEMORYTYPE_HOST) {
+    return "data is not in device memory";
+  }
+  for (const void* p : pointers) {
+    if (p == nullptr) continue;
+    int of = -1;
+    if (get(&of, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, reinterpret_cast<CUdeviceptr>(p)) != CUDA_SUCCESS) return "data is not in device memory";
+    if (of == dev) continue;
+    cudaPointerAttributes at{};  // managed and host memory may belong to any
+    if (cudaPointerGetAttributes(&at, p) == cudaSuccess && at.type == cudaMemoryTypeDevice) {
+      return "data is on device " + std::to_string(of) + ", the current device is " + std::to_string(dev);
+    }
   }
   return std::string();
 }

@@ -395,7 +395,9 @@ int copy(const char* name, const fpk_cache_copy_desc_t* d, bool write, void* str
   }
   if (d->slots == nullptr) return fail(std::string(name) + ": slots are required");
   if (!aligned4(d->slots) || !aligned4(d->error_flag)) return fail(std::string(name) + ": slots and error_flag must be 4-byte aligned");
-  const std::string where = deviceProblem(d->cache.k);
+  const bool e4m3 = d->cache.dtype == FPK_DTYPE_E4M3;
+  const std::string where = deviceProblem({d->cache.k, d->cache.v, d->k.data, d->v.data, d->slots, d->error_flag,
+                                           e4m3 ? d->cache.k_scale : nullptr, e4m3 ? d->cache.v_scale : nullptr});
   if (!where.empty()) return fail(std::string(name) + ": " + where);
   Args a{};
   a.cache[0] = static_cast<unsigned char*>(d->cache.k);
@@ -411,7 +413,6 @@ int copy(const char* name, const fpk_cache_copy_desc_t* d, bool write, void* str
   a.total = static_cast<uint32_t>(d->cache.n_pages) * static_cast<uint32_t>(d->cache.page_rows);
   a.slots = d->slots;
   a.error_flag = d->error_flag;
-  const bool e4m3 = d->cache.dtype == FPK_DTYPE_E4M3;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = d->dtype == FPK_DTYPE_BF16 ? launchType<__nv_bfloat16>(a, d->cache.head_dim, e4m3, write, s)
                                                    : launchType<__half>(a, d->cache.head_dim, e4m3, write, s);

@@ -312,7 +312,10 @@ extern "C" int fpk_qk_norm_rotary(const fpk_qk_rotary_desc_t* d, void* stream) {
     return fail("fpk_qk_norm_rotary: positions, inv_freq and weights must be 4-byte aligned");
   }
   if ((d->q_weight != nullptr || d->k_weight != nullptr) && !(d->eps >= 0.0f)) return fail("fpk_qk_norm_rotary: eps must not be negative");
-  const std::string where = heads::deviceProblem(d->q_heads > 0 ? d->q.data : d->k.data);
+  const bool q = d->q_heads > 0, k = d->kv_heads > 0, turn = d->rotary_dim > 0;
+  const std::string where = heads::deviceProblem({q ? d->q.data : d->k.data, q ? d->q_out.data : nullptr, k ? d->k.data : nullptr,
+                                                  k ? d->k_out.data : nullptr, q ? d->q_weight : nullptr, k ? d->k_weight : nullptr,
+                                                  turn ? d->positions : nullptr, turn ? d->inv_freq : nullptr});
   if (!where.empty()) return fail("fpk_qk_norm_rotary: " + where);
   rotary::Args a{};
   a.q = d->q;

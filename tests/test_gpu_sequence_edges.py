@@ -10,7 +10,7 @@ torch = pytest.importorskip("torch")
 
 from fp_b200 import kernels as K  # noqa: E402
 from seq_util import DT, Cache, HeadRows, starts, within  # noqa: E402
-from test_gpu_sequences import copy_desc, flag, gen, paged_desc, reference, rotary_desc, run_packed, run_paged, same_bits, stream  # noqa: E402
+from test_gpu_sequences import copy_desc, flag, gen, packed_desc, paged_desc, reference, rotary_desc, run_packed, run_paged, same_bits, stream  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 F16, BF16 = K.FPK_DTYPE_F16, K.FPK_DTYPE_BF16
@@ -355,3 +355,35 @@ def test_a_cut_tile_of_a_failed_cta_is_not_stored(fpk, paged):
     finally:
         fpk.lib.fpk_attention_test_fail_share(-1)
     assert missing.any() and not missing.all() and same_bits(run()[0].get(), whole)
+
+
+def test_every_pointer_must_be_on_the_device(fpk):
+    """A host array in the place of any pointer of a call is refused before a kernel could read it."""
+    host = torch.zeros(1 << 16, dtype=torch.uint8)
+    address = -(-host.data_ptr() // 16) * 16
+    d, n = 64, 20
+    q, k, v, out, ko = (HeadRows(n, h, d, F16).set(torch.zeros(n, h, d, device=DEV)) for h in (4, 2, 2, 4, 2))
+    g = gen(1)
+    ints = torch.zeros(n, dtype=torch.int32, device=DEV)
+    floats = torch.ones(d, device=DEV)
+    err, qs = flag(), starts([n])
+    cache, table, length, slots = one_cached(n, k.get(), v.get(), F16, 16, g)
+    rotary = lambda: rotary_desc(q, k, out, ko, F16, d, False, (floats, floats), ints, floats)  # noqa: E731
+    copy = lambda: copy_desc(cache, k, v, slots.to(torch.int32), F16, err)  # noqa: E731
+    packed = lambda: packed_desc(fpk, q, k, v, out, qs, qs, True, F16, err)[0]  # noqa: E731
+    paged = lambda: paged_desc(fpk, q, out, cache, qs, length, table, True, F16, err)[0]  # noqa: E731
+    scales = ["cache.k", "cache.v", "cache.k_scale", "cache.v_scale"]
+    for call, make, names in ((K.qk_norm_rotary, rotary, ["q.data", "k.data", "q_out.data", "k_out.data", "q_weight", "k_weight", "positions", "inv_freq"]),
+                              (K.cache_write, copy, scales + ["k.data", "v.data", "slots", "error_flag"]),
+                              (K.cache_read, copy, scales + ["k.data", "v.data", "slots", "error_flag"]),
+                              (K.attention_packed, packed, ["q.data", "k.data", "v.data", "out.data", "q_starts", "kv_starts", "error_flag", "workspace"]),
+                              (K.attention_paged, paged, scales + ["q.data", "out.data", "q_starts", "kv_lengths", "page_table", "error_flag", "workspace"])):
+        for name in names:
+            desc = make()
+            at = desc
+            for part in name.split(".")[:-1]:
+                at = getattr(at, part)
+            setattr(at, name.split(".")[-1], address)
+            with pytest.raises(K.FpkError, match="device memory"):
+                call(fpk, desc, stream())
+    torch.cuda.synchronize()
