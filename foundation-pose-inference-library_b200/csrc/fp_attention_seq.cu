@@ -13,7 +13,6 @@ namespace seqattn {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr long long kMostKeys = (1LL << 31) - 1024;  // key counts round up to blocks in 32 bits
 constexpr const char* kMisaligned = "starts, lengths, page_table and error_flag must be 4-byte aligned";
 
 std::atomic<int> g_test_fail{-1};  // fpk_attention_test_fail_share
@@ -29,14 +28,15 @@ std::string shapeProblem(const Shape& n) {
     return "q_heads must be a multiple of kv_heads, at most 128 to each";
   }
   if (n.n_seq < 0 || n.q_rows < 0) return "sizes must not be negative";
-  if (static_cast<long long>(n.q_rows) * (n.q_heads / n.kv_heads) + static_cast<long long>(n.n_seq) * 128 >= (1LL << 31)) {
-    return "too many query rows (q_rows * q_heads / kv_heads must be below 2^31)";
+  if (static_cast<long long>(n.q_rows) * (n.q_heads / n.kv_heads) + static_cast<long long>(n.n_seq) * 128 > kMost) {
+    return "too many query rows (q_rows * q_heads / kv_heads + 128 * n_seq must be at most 2^31 - 1024)";
   }
   return std::string();
 }
 
 std::string scaleProblem(float scale) {
-  return scale >= 0.0f && std::isfinite(scale) ? std::string() : std::string("scale must be finite and not negative");
+  // In the units of exp2 too.
+  return scale >= 0.0f && std::isfinite(scale * kLog2e) ? std::string() : std::string("scale must be finite and not negative (at most 2^127)");
 }
 
 float scaleLog2(float scale, int head_dim) {
@@ -113,7 +113,7 @@ extern "C" int fpk_attention_packed(const fpk_attention_packed_desc_t* d, void* 
   std::string p = shapeProblem(n);
   if (p.empty()) p = scaleProblem(d->scale);
   if (p.empty() && d->kv_rows < 0) p = "sizes must not be negative";
-  if (p.empty() && d->kv_rows > kMostKeys) p = "kv_rows must be at most 2^31 - 1024";
+  if (p.empty() && d->kv_rows > kMost) p = "kv_rows must be at most 2^31 - 1024";
   if (!p.empty()) return fail(name + ": " + p);
   if (d->n_seq == 0 || d->q_rows == 0) return 0;
   for (const fpk_heads_t* v : {&d->q, &d->out, &d->k, &d->v}) {
@@ -161,7 +161,7 @@ extern "C" int fpk_attention_paged(const fpk_attention_paged_desc_t* d, void* st
   if (p.empty()) p = shapeProblem(n);
   if (p.empty()) p = scaleProblem(d->scale);
   if (p.empty() && d->table_pages < 0) p = "sizes must not be negative";
-  if (p.empty() && n.keys > kMostKeys) p = "table_pages * page_rows must be at most 2^31 - 1024";
+  if (p.empty() && n.keys > kMost) p = "table_pages * page_rows must be at most 2^31 - 1024";
   if (!p.empty()) return fail(name + ": " + p);
   if (d->n_seq == 0 || d->q_rows == 0) return 0;
   for (const fpk_heads_t* v : {&d->q, &d->out}) {

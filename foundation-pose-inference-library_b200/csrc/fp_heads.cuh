@@ -171,6 +171,10 @@ inline const char* headsProblem(const fpk_heads_t& v) {
   return nullptr;
 }
 
+// Most rows of a call, and most rows times heads or keys of a sequence: kernels round
+// them up to blocks in 32 bits.
+constexpr long long kMost = (1LL << 31) - 1024;
+
 inline bool is16Bit(int dtype) { return dtype == FPK_DTYPE_F16 || dtype == FPK_DTYPE_BF16; }
 
 inline std::string cacheProblem(const fpk_kv_cache_t& c, int dtype) {

@@ -389,6 +389,7 @@ int copy(const char* name, const fpk_cache_copy_desc_t* d, bool write, void* str
   const std::string p = cacheProblem(d->cache, d->dtype);
   if (!p.empty()) return fail(std::string(name) + ": " + p);
   if (d->rows < 0 || d->cache.kv_heads > 4096) return fail(std::string(name) + ": bad sizes");
+  if (d->rows > kMost) return fail(std::string(name) + ": rows must be at most 2^31 - 1024");
   if (d->rows == 0) return 0;
   for (const fpk_heads_t* v : {&d->k, &d->v}) {
     if (const char* q = headsProblem(*v)) return fail(std::string(name) + ": " + q);

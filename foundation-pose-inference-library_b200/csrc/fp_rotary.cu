@@ -298,6 +298,7 @@ extern "C" int fpk_qk_norm_rotary(const fpk_qk_rotary_desc_t* d, void* stream) {
   if (d->rotary_dim < 0 || d->rotary_dim > d->head_dim || d->rotary_dim % 16) {
     return fail("fpk_qk_norm_rotary: rotary_dim must be a multiple of 16 up to head_dim");
   }
+  if (d->rows > heads::kMost) return fail("fpk_qk_norm_rotary: rows must be at most 2^31 - 1024");
   if (d->rows == 0 || d->q_heads + d->kv_heads == 0) return 0;
   for (int i = 0; i < 4; ++i) {
     const bool is_q = i % 2 == 0;

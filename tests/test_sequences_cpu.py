@@ -149,3 +149,18 @@ def test_key_counts_that_would_overflow_are_refused(fl):
         K.attention_packed(fl, packed(kv_rows=2 ** 31 - 1))
     with pytest.raises(K.FpkError, match="2\\^31 - 1024"):
         K.attention_paged(fl, paged(table_pages=(1 << 27) - 1))  # pages of 16 rows
+
+
+@pytest.mark.parametrize("call,make,change,match", [
+    (K.qk_norm_rotary, rotary, dict(rows=2 ** 31 - 1), "2\\^31 - 1024"), (K.qk_norm_rotary, rotary, dict(rows=2 ** 31 - 1023), "2\\^31 - 1024"),
+    (K.cache_write, copy, dict(rows=2 ** 31 - 1), "2\\^31 - 1024"), (K.cache_read, copy, dict(rows=2 ** 31 - 1023), "2\\^31 - 1024"),
+    # 4 query heads to a key head: 2^31 - 200 rows of tiles, which 255 more would take past 2^31.
+    (K.attention_packed, packed, dict(q_rows=2 ** 29 - 50 - 64, n_seq=2), "too many"),
+    (K.attention_packed, packed, dict(q_rows=2 ** 29 - 256, n_seq=0), None), (K.attention_packed, packed, dict(q_rows=2 ** 29 - 255, n_seq=0), "too many"),
+    (K.attention_packed, packed, dict(scale=3e38), "scale"), (K.attention_paged, paged, dict(scale=2.5e38), "scale")])
+def test_sizes_at_the_end_of_32_bits(fl, call, make, change, match):
+    if match is None:
+        call(fl, make(**change))
+        return
+    with pytest.raises(K.FpkError, match=match):
+        call(fl, make(**change))
