@@ -417,8 +417,10 @@ FP_API int fpk_attention_packed(const fpk_attention_packed_desc_t* desc, void* s
  * fpk_attention_packed, with key j of sequence s in row j % page_rows of page
  * page_table[s*table_pages + j / page_rows] and kv_lengths[s] keys. Any number
  * of query rows per sequence: one, or a chunk. Entries of the table past a
- * sequence's last page are not read. E4M3: probabilities may be rounded to FP16
- * in units of the v_scale, so that a key's product of weight and v_scale counts
+ * sequence's last page are not read. E4M3: queries may be rounded to FP16 with a
+ * power of two taken out of each row and head (by at most 2^-25 of the row's
+ * largest element, which is exact for BF16 down to 2^-17 of it), probabilities to
+ * FP16 in units of the v_scale, so that a key's product of weight and v_scale counts
  * down to 2^-32 of the largest such product. The v_scale of the keys that one
  * query sees lie within a factor of 2^90. A row of zeros counts as one of scale
  * 2^-48 for both, whatever its scale is. E4M3 elements beyond the range of FP16
