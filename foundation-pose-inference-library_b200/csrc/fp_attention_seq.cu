@@ -13,6 +13,9 @@ namespace seqattn {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// A CTA walks over sequences without rows one by one, some half a microsecond each,
+// which the bounded waits (2 s) of those that it feeds have to outlast.
+constexpr int kMostSequences = 1 << 20;
 constexpr const char* kMisaligned = "starts, lengths, page_table and error_flag must be 4-byte aligned";
 
 std::atomic<int> g_test_fail{-1};  // fpk_attention_test_fail_share
@@ -28,6 +31,7 @@ std::string shapeProblem(const Shape& n) {
     return "q_heads must be a multiple of kv_heads, at most 128 to each";
   }
   if (n.n_seq < 0 || n.q_rows < 0) return "sizes must not be negative";
+  if (n.n_seq > kMostSequences) return "at most 2^20 sequences";
   if (static_cast<long long>(n.q_rows) * (n.q_heads / n.kv_heads) + static_cast<long long>(n.n_seq) * 128 > kMost) {
     return "too many query rows (q_rows * q_heads / kv_heads + 128 * n_seq must be at most 2^31 - 1024)";
   }

@@ -295,7 +295,7 @@ FP_API int fpk_attention(const void* qkv, long long qkv_plane_stride, int qkv_la
  * where an entry point says so, nor themselves.
  *
  * Rows of a call are at most 2^31 - 1024, for attention times the query heads to a
- * key head and with 128 more for each sequence.
+ * key head and with 128 more for each sequence, of which there are 2^20 at most.
  * Row indexes, lengths and page numbers are read on the device, so captured
  * graphs follow their current values. Kernels check them against the sizes of
  * the descriptor: a call never reads or writes outside the buffers it was

@@ -9,7 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from fp_b200 import kernels as K  # noqa: E402
-from seq_util import DT, Cache, HeadRows, starts, within  # noqa: E402
+from seq_util import DT, Cache, HeadRows, attention64, starts, within  # noqa: E402
 from test_gpu_sequences import copy_desc, flag, gen, packed_desc, paged_desc, reference, rotary_desc, run_packed, run_paged, same_bits, stream  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -387,3 +387,28 @@ def test_every_pointer_must_be_on_the_device(fpk):
             with pytest.raises(K.FpkError, match="device memory"):
                 call(fpk, desc, stream())
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("tiles", [False, True])
+def test_most_sequences_nearly_all_empty(fpk, tiles):
+    """2^20 sequences of which the first and the last have rows: a walk over all the others ends in time."""
+    n_seq, d, hk = 1 << 20, 64, 1
+    hq = 128 if tiles else 2
+    nq = [70000, 62000] if tiles else [300, 200]
+    g = gen(1)
+    q = HeadRows(sum(nq), hq, d, F16, around=0.0).set(torch.randn(sum(nq), hq, d, device=DEV, generator=g))
+    # Many rows of keys, of which 400 are some sequence's: the choice of the kernel goes by the average.
+    k, v = (HeadRows(300000, hk, d, F16).set(torch.randn(300000, hk, d, device=DEV, generator=g)) for _ in range(2))
+    out = HeadRows(sum(nq), hq, d, F16, around=3.0)
+    qs, ks = torch.full((n_seq + 1,), nq[0], dtype=torch.int32, device=DEV), torch.full((n_seq + 1,), 250, dtype=torch.int32, device=DEV)
+    qs[0], qs[-1], ks[0], ks[-1] = 0, sum(nq), 0, 400
+    err = flag()
+    desc, ws = packed_desc(fpk, q, k, v, out, qs, ks, False, F16, err)
+    K.attention_packed(fpk, desc, stream())
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    few = torch.randperm(sum(nq), device=DEV, generator=g)[:200].sort().values
+    for rows, keys in ((few[few < nq[0]], slice(0, 250)), (few[few >= nq[0]], slice(250, 400))):
+        kk, vv = (x.get()[keys].double() for x in (k, v))
+        ref, bound = attention64(q.get()[rows].double(), kk, vv, False, d ** -0.5, F16)
+        assert within(out.get()[rows], ref, bound) <= 1

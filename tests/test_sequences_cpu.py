@@ -157,6 +157,7 @@ def test_key_counts_that_would_overflow_are_refused(fl):
     # 4 query heads to a key head: 2^31 - 200 rows of tiles, which 255 more would take past 2^31.
     (K.attention_packed, packed, dict(q_rows=2 ** 29 - 50 - 64, n_seq=2), "too many"),
     (K.attention_packed, packed, dict(q_rows=2 ** 29 - 256, n_seq=0), None), (K.attention_packed, packed, dict(q_rows=2 ** 29 - 255, n_seq=0), "too many"),
+    (K.attention_packed, packed, dict(n_seq=2 ** 20 + 1), "sequences"), (K.attention_paged, paged, dict(n_seq=2 ** 20 + 1), "sequences"),
     (K.attention_packed, packed, dict(scale=3e38), "scale"), (K.attention_paged, paged, dict(scale=2.5e38), "scale")])
 def test_sizes_at_the_end_of_32_bits(fl, call, make, change, match):
     if match is None:
