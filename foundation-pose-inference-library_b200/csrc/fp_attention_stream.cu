@@ -38,9 +38,9 @@
 //   keys out evenly and join over distributed shared memory: no second launch.
 //
 // Measured (32 query heads over 8 key heads of 128, bf16): one token of each of 8
-// sequences of 8,000 to 131,072 keys 151 us over e4m3 (941 MB, 6.2 TB/s, 95 % of
-// the copy rate; 164 under the power cap) and 278 us over 16 bits (1.82 GB, the
-// copy rate); of each of 4 sequences of 40 to 1,000 keys 8.9 us, launch and latency.
+// sequences of 8,000 to 131,072 keys 154 us over e4m3 (941 MB, 6.1 TB/s, 93 % of
+// the copy rate; 169 under the power cap) and 280 us over 16 bits (1.82 GB, the
+// copy rate); of each of 4 sequences of 40 to 1,000 keys 8.8 us, launch and latency.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

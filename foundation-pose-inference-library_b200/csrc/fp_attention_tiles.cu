@@ -45,12 +45,12 @@
 // move to tile ends and nothing is joined. All mbarrier waits are bounded.
 //
 // Measured: 4 causal prompts of 700 to 8,192 tokens, 16 heads over 2 of 128, bf16,
-// 555 us = 936 TFLOP/s, without a mask 970; 252 sequences of 400, 4 heads of 128,
-// fp16, 150 us = 551 TFLOP/s (a fifth of the rows of its tiles are empty). A block of 128 keys takes some 3,900 cycles
+// 542 us = 958 TFLOP/s, without a mask 1,028; 252 sequences of 400, 4 heads of 128,
+// fp16, 153 us = 540 TFLOP/s (a fifth of the rows of its tiles are empty). A block of 128 keys takes some 3,900 cycles
 // for the 256 rows, of 2,048 that either the tensor core or the exponentials
 // need: each half waits for its scores (1,200), then for its own 2 x 64
 // exponentials (2,400, the other half's among them). Tried and not kept: the
-// halves in turns, a quarter of the exponentials as polynomials (slower by 3 to 8
+// halves in turns (with a separate pass for the maximum), a quarter of the exponentials as polynomials (slower by 3 to 8
 // %), both halves of a block unrolled with loads ahead (no gain, crops 8 % slower),
 // two threads to a row in 16 warps of 80 registers (13 to 30 % slower), scores of 64
 // keys two parts ahead in either half of their columns (prompts the same, crops

@@ -2,8 +2,8 @@
 // fpk_cache_read, include/fpk.h).
 //
 // A cache page holds, per head, planes of 16-byte records (8 channels of a
-// 16-bit cache, 16 of an e4m3 cache) over its rows: the tile that the attention
-// kernels read without reordering it. e4m3 rows carry one power-of-two scale:
+// 16-bit cache, 16 of an e4m3 cache) over its rows: a 16-bit tile is what the
+// attention kernels read without reordering it. e4m3 rows carry one power-of-two scale:
 //   e = min{ e >= -100 : max|x| <= 448 * 2^e },  code = e4m3(x * 2^-e)
 // A power of two costs e4m3, a floating format, no precision within its range,
 // and makes code * scale exact in bf16, so that attention over the cache and
@@ -14,10 +14,12 @@
 // and 32 rows where the rows do (planar); the cache side is reached in 16-byte
 // records either way, because slots are arbitrary.
 //
-// Measured (8 heads of 128, bf16 rows, e4m3 cache, pages of 64): 16,384 rows written
-// to random slots 71 us, to slots in order 28; 20,011 read back from random slots 38
-// us, in order 29. Floors are 15.5 and 19: a random slot touches half of each
-// 32-byte sector, and those touches, not bytes, are what the L2 is busy with.
+// Measured (8 heads of 128, bf16 rows, pages of 64; us): e4m3 cache, 16,384 rows
+// written to random slots 71, to slots in order 28; 20,011 read back from random
+// slots 35, in order 28 (floors 15.5 and 19). 16-bit cache 139, 41, 70 and 31 (floors
+// 20.5 and 25). A random slot touches half of each 32-byte sector, and those touches,
+// not bytes, are what the L2 is busy with; in order too a row's records are stored
+// and read by themselves, page_rows x 16 bytes apart.
 #include <algorithm>
 #include <cfloat>
 #include <cstdint>
