@@ -12,8 +12,9 @@
 //   warps 0-3, 4-7  softmax of half 0 and 1, one query row per thread: the
 //                   row's 128 scores from TMEM, 64 at a time: running maximum
 //                   and sum in fp32, P = 2^(s - m) rounded to the element type
-//                   over the scores' own TMEM columns. O is rescaled only when a
-//                   row's maximum grows by more than 2^8 (reference: 2^7 below it). After the last, O / l.
+//                   over the scores' own TMEM columns. m lies 2^7 below a row's
+//                   maximum; O is rescaled only when that grows by more than 2^8.
+//                   After the last, O / l.
 //   warps 8-11      loads of Q, K and V rows, K and V in four stages of 128 rows.
 //                   Two layouts in shared memory, each the one that its source
 //                   fills line by line (the other way round the copies take
@@ -32,6 +33,7 @@
 //   warp 13         the walk: the next pieces of work for the others.
 //   warp 14         the proxy fence between a load's arrival and the MMAs that
 //                   read it, which would cost the issuing warp 300-600 cycles.
+//
 // Under a causal mask 0 * v of a key that a row does not see is NaN where v is an
 // infinity or NaN. An item with NaN in such a row is walked a second time, when
 // warp 14 takes these values out and the softmax warps add them to the rows that
@@ -46,12 +48,13 @@
 //
 // Measured: 4 causal prompts of 700 to 8,192 tokens, 16 heads over 2 of 128, bf16,
 // 542 us = 958 TFLOP/s, without a mask 1,028; 252 sequences of 400, 4 heads of 128,
-// fp16, 153 us = 540 TFLOP/s (a fifth of the rows of its tiles are empty). A block of 128 keys takes some 3,900 cycles
-// for the 256 rows, of 2,048 that either the tensor core or the exponentials
-// need: each half waits for its scores (1,200), then for its own 2 x 64
-// exponentials (2,400, the other half's among them). Tried and not kept: the
-// halves in turns (with a separate pass for the maximum), a quarter of the exponentials as polynomials (slower by 3 to 8
-// %), both halves of a block unrolled with loads ahead (no gain, crops 8 % slower),
+// fp16, 153 us = 540 TFLOP/s (a fifth of the rows of its tiles are empty). A block
+// of 128 keys takes some 3,900 cycles for the 256 rows, of 2,048 that either the
+// tensor core or the exponentials need: each half waits for its scores (1,200), then
+// for its own 2 x 64 exponentials (2,400, the other half's among them). Tried and not
+// kept: the halves in turns (with a separate pass for the maximum), a quarter of the
+// exponentials as polynomials (slower by 3 to 8 %), both halves of a block unrolled
+// with loads ahead (no gain, crops 8 % slower),
 // two threads to a row in 16 warps of 80 registers (13 to 30 % slower), scores of 64
 // keys two parts ahead in either half of their columns (prompts the same, crops
 // 164: a product with 64 keys takes 53 cycles for half of the 64 that 128 take).
@@ -487,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) attentionTilesKernel(const Args a
   Smem& sm = *reinterpret_cast<Smem*>(base);
   const uint32_t q_s = smemU32(base + 1024);
   const uint32_t kv_s = q_s + 2 * G::kTileBytes;
+
   tc::pdlTrigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {

@@ -388,7 +388,8 @@ FP_API int fpk_cache_read(const fpk_cache_copy_desc_t* desc, void* stream);
  * multiple of kv_heads, at most 128 query heads to a key head. Products run on
  * the tensor cores with probabilities rounded to the element type; scores,
  * softmax statistics and sums are fp32. What a key that a query does not see holds,
- * an infinity or NaN too, does not reach the query's output.
+ * an infinity or NaN too, does not reach the query's output. (An infinity that it
+ * sees with a weight below the range of the products makes NaN.)
  * How far sequences are split over the GPU follows the sizes in the descriptor,
  * so the last bits may; for one descriptor and lengths they do not change.
  * workspace (fpk_attention_packed_workspace_bytes, the same for every batch of
